@@ -1,4 +1,4 @@
-"""ctypes view of libfa8_b200.so (declared in include/fa8_b200.h).
+"""ctypes view of libfa8_b200.so (declared in include/fa8_b200.h and include/fa8_kv_cache.h).
 
 There is no fallback: if the library is missing or a symbol cannot be bound,
 loading raises, and so does every operator call.
@@ -15,6 +15,7 @@ FA8_ERR_BAD_ARG = -1
 FA8_ERR_UNSUPPORTED = -2
 FA8_ERR_CUDA = -3
 FA8_ERR_DEVICE_TIMEOUT = -4
+FA8_ERR_BAD_INDEX = -5
 
 FA8_V_TRANSPOSED = 0
 FA8_V_NATURAL = 1
@@ -29,6 +30,8 @@ EXPORTED_SYMBOLS = ("fa8_fwd", "fa8_check_status", "fa8_supported", "fa8_error_s
                     "fa8_quantize_e4m3", "fa8_quantize_e4m3_segments", "fa8_quantize_e4m3_segments_noalloc",
                     "fa8_work_plan")
 FA8_NOALLOC_MAX_SEGMENTS = 4096
+# Every symbol include/fa8_kv_cache.h declares.
+KV_SYMBOLS = ("fa8_kv_append", "fa8_kv_read", "fa8_kv_attention", "fa8_kv_attention_workspace", "fa8_kv_version")
 
 
 class Fa8FwdParams(ctypes.Structure):
@@ -42,6 +45,28 @@ class Fa8FwdParams(ctypes.Structure):
         ("descale_q", ctypes.c_void_p), ("descale_k", ctypes.c_void_p), ("descale_v", ctypes.c_void_p),
         ("fp8_format", ctypes.c_int32), ("seqlen_k", ctypes.c_int32),
         ("descale_per_head", ctypes.c_int32),
+    ]
+
+
+class Fa8KvCache(ctypes.Structure):
+    """struct fa8_kv_cache of include/fa8_kv_cache.h."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_descale", ctypes.c_void_p), ("v_descale", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int32), ("heads_kv", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("fp8_format", ctypes.c_int32), ("batch", ctypes.c_int32),
+        ("page_table", ctypes.c_void_p), ("table_width", ctypes.c_int32), ("table_stride", ctypes.c_int32),
+        ("seqlens", ctypes.c_void_p), ("cu_seqlens", ctypes.c_void_p), ("tokens", ctypes.c_int32),
+        ("status_word", ctypes.c_void_p),
+    ]
+
+
+class Fa8KvAttentionParams(ctypes.Structure):
+    """struct fa8_kv_attention_params of include/fa8_kv_cache.h."""
+    _fields_ = [
+        ("cache", Fa8KvCache), ("q", ctypes.c_void_p), ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("heads", ctypes.c_int32),
+        ("is_causal", ctypes.c_int32), ("softmax_scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
     ]
 
 
@@ -84,6 +109,16 @@ def load() -> ctypes.CDLL:
     lib.fa8_error_string.restype = ctypes.c_char_p
     lib.fa8_last_error_detail.argtypes = []
     lib.fa8_last_error_detail.restype = ctypes.c_char_p
+    lib.fa8_kv_append.argtypes = [ctypes.POINTER(Fa8KvCache)] + 2 * [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64] + [ctypes.c_int32, ctypes.c_void_p]
+    lib.fa8_kv_append.restype = ctypes.c_int
+    lib.fa8_kv_read.argtypes = [ctypes.POINTER(Fa8KvCache), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]
+    lib.fa8_kv_read.restype = ctypes.c_int
+    lib.fa8_kv_attention.argtypes = [ctypes.POINTER(Fa8KvAttentionParams), ctypes.c_void_p]
+    lib.fa8_kv_attention.restype = ctypes.c_int
+    lib.fa8_kv_attention_workspace.argtypes = [ctypes.c_int32] * 8
+    lib.fa8_kv_attention_workspace.restype = ctypes.c_int64
+    lib.fa8_kv_version.argtypes = []
+    lib.fa8_kv_version.restype = ctypes.c_int
     lib.fa8_version.argtypes = []
     lib.fa8_version.restype = ctypes.c_int
     _lib = lib

@@ -20,8 +20,10 @@ LIB_PATH = os.path.join(PKG_DIR, "libfa8_b200.so")
 # Digest of the sources the library was built from, written next to it: a copy of the tree keeps
 # file contents but not necessarily modification times, so staleness is decided by content.
 HASH_PATH = os.path.join(PKG_DIR, "libfa8_b200.srchash")
-SOURCES = ["fa8_fwd_sm100.cu", "fa8_decode_sm100.cu", "fa8_quant.cu", "fa8_capi.cu"]
-HEADERS = ["fa8_kernel.h", "phase_rule.h", "ptx_sm100.cuh", os.path.join(REPO_DIR, "include", "fa8_b200.h")]
+SOURCES = ["fa8_fwd_sm100.cu", "fa8_decode_sm100.cu", "fa8_quant.cu", "fa8_capi.cu",
+           "fa8_kv_cache.cu", "fa8_kv_attend.cu", "fa8_kv_capi.cu"]
+HEADERS = ["fa8_kernel.h", "fa8_kv.h", "kv_common.cuh", "phase_rule.h", "ptx_sm100.cuh",
+           os.path.join(REPO_DIR, "include", "fa8_b200.h"), os.path.join(REPO_DIR, "include", "fa8_kv_cache.h")]
 
 
 def nvcc_path() -> str:
@@ -61,7 +63,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB_PATH
     if os.path.exists(HASH_PATH):
         os.remove(HASH_PATH)
-    cmd = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
+    cmd = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--threads", "0",
            "-I" + os.path.join(REPO_DIR, "include"), "-I" + CSRC,
            "-Xcompiler", "-fPIC", "-shared", "-o", LIB_PATH]
     if verbose:
@@ -109,7 +111,7 @@ def binding_is_stale() -> bool:
 
 def _binding_digest() -> str:
     h = hashlib.sha256()
-    for d in (BINDING_SRC, os.path.join(REPO_DIR, "include", "fa8_b200.h")):
+    for d in (BINDING_SRC, os.path.join(REPO_DIR, "include", "fa8_b200.h"), os.path.join(REPO_DIR, "include", "fa8_kv_cache.h")):
         with open(d, "rb") as f:
             h.update(f.read())
     return h.hexdigest()

@@ -17,6 +17,8 @@
 
 #include "fa8_b200.h"
 #include "fa8_kernel.h"
+#include "fa8_kv.h"
+#include "fa8_kv_cache.h"
 
 namespace {
 
@@ -181,7 +183,35 @@ int collect_earlier_failure(DeviceState* st, int32_t* caller_word, cudaStream_t 
   return code;
 }
 
+// Error code of what a kernel left in a status word.
+int error_of(int code) { return code == fa8::kBadIndex ? FA8_ERR_BAD_INDEX : FA8_ERR_DEVICE_TIMEOUT; }
+
+// The same for entry points: 0 = nothing, an error code (and its detail) otherwise.
+int refuse_after_failure(DeviceState* st, int32_t* caller_word, cudaStream_t stream) {
+  const int code = collect_earlier_failure(st, caller_word, stream);
+  if (code == 0) return FA8_OK;
+  char buf[96];
+  std::snprintf(buf, sizeof(buf), "device code 0x%x; this call was not enqueued", code);
+  set_detail(code == fa8::kBadIndex ? "an earlier launch on this device reported an index out of range"
+                                    : "an earlier launch on this device reported an expired wait", buf);
+  return error_of(code);
+}
+
 }  // namespace
+
+// For the entry points of the paged cache (fa8_kv_capi.cu).
+namespace fa8 {
+
+void status_words(int** dev_word, int** host_word) {
+  DeviceState* st = device_state();
+  *dev_word = st ? st->dev_word : nullptr;
+  *host_word = st ? st->host_flag_dev : nullptr;
+}
+int earlier_failure(int32_t* caller_word, cudaStream_t stream) { return refuse_after_failure(device_state(), caller_word, stream); }
+void clear_error_detail() { g_detail[0] = '\0'; }
+void set_error_detail(const char* what, const char* msg) { set_detail(what, msg); }
+
+}  // namespace fa8
 
 extern "C" {
 
@@ -196,6 +226,7 @@ const char* fa8_error_string(int code) {
              "key/value length must be a multiple of 16)";
     case FA8_ERR_CUDA: return "CUDA call failed";
     case FA8_ERR_DEVICE_TIMEOUT: return "a bounded wait inside a kernel expired";
+    case FA8_ERR_BAD_INDEX: return "a kernel found a page number, length or token range out of range";
     default: return "unknown fa8 status";
   }
 }
@@ -259,12 +290,7 @@ int fa8_fwd(const fa8_fwd_params* p, void* cuda_stream) {
   // A launch that went wrong earlier on this device is reported now, before anything new is
   // enqueued (the reference's only error path is exit(), include/attention_api.cuh:20-29).
   DeviceState* dstate = device_state();
-  if (const int code = collect_earlier_failure(dstate, p->status_word, stream)) {
-    char buf[96];
-    std::snprintf(buf, sizeof(buf), "device code 0x%x; this call was not enqueued", code);
-    set_detail("an earlier launch on this device reported an expired wait", buf);
-    return FA8_ERR_DEVICE_TIMEOUT;
-  }
+  if (const int rc = refuse_after_failure(dstate, p->status_word, stream)) return rc;
   // one work item per 128 query rows is the finest plan the launcher can choose
   if (bh_q * ((static_cast<int64_t>(p->seqlen) + 127) / 128) > 0x7fffffff) return FA8_ERR_UNSUPPORTED;
   // Without a causal mask the query heads that share a key/value head see the same keys, and their
@@ -499,7 +525,7 @@ int fa8_check_status(const int32_t* status_word, void* cuda_stream, int32_t* cod
     }
   }
   if (code_out) *code_out = host;
-  return host == 0 ? FA8_OK : FA8_ERR_DEVICE_TIMEOUT;
+  return host == 0 ? FA8_OK : error_of(host);
 }
 
 }  // extern "C"

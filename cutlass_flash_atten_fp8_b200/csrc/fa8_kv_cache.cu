@@ -1,0 +1,308 @@
+// Writing new keys and values into the pages of the fp8 cache, and reading them back.
+//
+// A unit of work is what one sequence's new tokens touch of one page and head, of K or of V: at most
+// page_size rows of head_dim.  Units own their page, head and scale, so the scale can be raised and
+// the page's older tokens rounded anew by the unit alone, with no atomics.
+//
+//   a = max |x| of the new rows,  2^e = the smallest power of two with a <= MAX 2^e,
+//   d = 2^e in a page that starts anew, max(d, 2^e) otherwise;  older x8 <- fp8(x8 d_old / d),  x8 = fp8(x / d)
+//
+// Bound by memory: two bytes in and one out per element (append; the reverse for read).
+#include <cuda_runtime.h>
+
+#include "fa8_kernel.h"
+#include "fa8_kv.h"
+#include "kv_common.cuh"
+
+namespace fa8 {
+
+namespace {
+
+constexpr int kHold = 4;               // chunks of sixteen elements that a thread keeps in registers
+constexpr int kWarpWork = 32 * kHold * 16;
+constexpr int kMaxThreads = 512;
+constexpr int kWarpsPerCta = 4;        // units of a CTA where a warp takes one
+
+// The part of a page that a unit is about.
+struct Unit {
+  int head;
+  bool of_v;
+  int page;                            // -1: nothing to do, or (read) zeros are due
+  int off, rows;                       // slots off .. off + rows - 1
+  int row0;                            // first row of the token-major tensors
+};
+
+template <bool kRead>
+__device__ __forceinline__ Unit find_unit(const KvArgs& a, int64_t u) {
+  Unit r{};
+  const int64_t slot = u / (2 * a.heads);
+  const int i = static_cast<int>(u - slot * (2 * a.heads));
+  r.of_v = i >= a.heads;
+  r.head = r.of_v ? i - a.heads : i;
+  r.page = -1;
+  int b, j;
+  kv_find_slot(a, slot, a.page_shift, 2, &b, &j);
+  const KvSeq s = kv_seq(a, b);
+  const int P = 1 << a.page_shift;
+  if (s.bad || s.n > s.len) {
+    if (i == 0 && j == 0) report_bad_index(a);
+    const int64_t lo = static_cast<int64_t>(j) * P;
+    if (kRead && lo < s.n) {
+      r.rows = min(P, s.n - static_cast<int>(lo));
+      r.row0 = s.first + static_cast<int>(lo);
+    }
+    return r;
+  }
+  const int start = s.len - s.n;
+  const int64_t pi = static_cast<int64_t>(start >> a.page_shift) + j;
+  const int64_t lo = max(static_cast<int64_t>(start), pi * P), hi = min(static_cast<int64_t>(s.len), (pi + 1) * P);
+  if (lo >= hi) return r;
+  r.off = static_cast<int>(lo) & (P - 1);
+  r.rows = static_cast<int>(hi - lo);
+  r.row0 = s.first + static_cast<int>(lo - start);
+  r.page = kv_page(a, b, static_cast<int>(pi));
+  return r;
+}
+
+// Row of chunk i where a row has `per_row` <= 16 chunks, i < 2048: magic = 65536 / per_row + 1.
+__device__ __forceinline__ int row_of(int i, uint32_t magic) { return static_cast<int>((static_cast<uint32_t>(i) * magic) >> 16); }
+
+template <bool kE5M2>
+__device__ __forceinline__ float scale_for(float amax) {
+  // MAX = 1.75 * 2^8 (e4m3) or 1.75 * 2^15 (e5m2): the exponent follows from amax's own and whether
+  // its significand is above 1.75
+  const uint32_t bits = __float_as_uint(amax);
+  int e = static_cast<int>(bits >> 23) - 127 - (kE5M2 ? 15 : 8) + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = min(max(e, -64), 64);
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+__device__ __forceinline__ uint32_t pair_max(uint32_t m, uint32_t w, bool bf16) {
+  w &= 0x7fff7fffu;                                       // max drops NaN
+  if (bf16) asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w));
+  else asm("max.f16x2 %0, %0, %1;" : "+r"(m) : "r"(w));
+  return m;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ float abs_max(const uint4& x) {
+  uint32_t m = 0;
+  m = pair_max(m, x.x, kBf16);
+  m = pair_max(m, x.y, kBf16);
+  m = pair_max(m, x.z, kBf16);
+  m = pair_max(m, x.w, kBf16);
+  const float2 f = half_pair<kBf16>(m);
+  float r = fmaxf(f.x, f.y);
+  if (r == INFINITY) {                                    // infinities saturate and do not count
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    r = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = half_pair<kBf16>(w[i] & 0x7fff7fffu);
+      if (p.x < INFINITY) r = fmaxf(r, p.x);
+      if (p.y < INFINITY) r = fmaxf(r, p.y);
+    }
+  }
+  return r;
+}
+
+template <bool kBf16, bool kE5M2>
+__device__ __forceinline__ uint2 to_fp8x8(const uint4& x, float inv) {
+  const float2 a = half_pair<kBf16>(x.x), b = half_pair<kBf16>(x.y), c = half_pair<kBf16>(x.z), d = half_pair<kBf16>(x.w);
+  return make_uint2(fp8_pair<kE5M2>(a.x * inv, a.y * inv) | (fp8_pair<kE5M2>(b.x * inv, b.y * inv) << 16),
+                    fp8_pair<kE5M2>(c.x * inv, c.y * inv) | (fp8_pair<kE5M2>(d.x * inv, d.y * inv) << 16));
+}
+
+// kWarp: a unit to a warp, several a CTA; otherwise a unit to a CTA.
+template <bool kBf16, bool kE5M2, bool kWarp>
+__global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_append_kernel(const KvArgs a, const KvRows kin, const KvRows vin,
+                                                                                            int64_t units, uint32_t magic) {
+  __shared__ float part[kMaxThreads / 32];
+  start_after_predecessor();
+  let_successor_start();
+  const int tid = kWarp ? threadIdx.x & 31 : threadIdx.x, n_threads = kWarp ? 32 : blockDim.x;
+  const int64_t u = kWarp ? static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5) : blockIdx.x;
+  if (u >= units) return;
+  const Unit w = find_unit<false>(a, u);
+  if (w.page < 0) return;                                 // the same for all threads of the unit
+  const int D = a.head_dim, per_row = D >> 4, chunks = w.rows * per_row;
+  const KvRows& in = w.of_v ? vin : kin;
+  const uint16_t* x = static_cast<const uint16_t*>(in.x) + w.row0 * in.token_stride + w.head * in.head_stride;
+  const int64_t page_head = static_cast<int64_t>(w.page) * a.heads + w.head;
+  uint8_t* const y = (w.of_v ? a.v : a.k) + (page_head << a.page_shift) * D;
+  float* const descale = (w.of_v ? a.v_descale : a.k_descale) + page_head;
+  const float old = w.off > 0 ? ld_global(descale) : 0.f;
+  auto src = [&](int i) {
+    const int r = row_of(i, magic);
+    return reinterpret_cast<const uint4*>(x + r * in.token_stride + 16 * (i - r * per_row));
+  };
+  uint4 hold[kHold][2];
+  float amax = 0.f;
+#pragma unroll
+  for (int h = 0; h < kHold; ++h) {
+    const int i = tid + h * n_threads;
+    hold[h][0] = hold[h][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (i < chunks) {
+      const uint4* p = src(i);
+      hold[h][0] = ld_global(p);
+      hold[h][1] = ld_global(p + 1);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < kHold; ++h) amax = fmaxf(amax, fmaxf(abs_max<kBf16>(hold[h][0]), abs_max<kBf16>(hold[h][1])));
+  for (int i = tid + kHold * n_threads; i < chunks; i += n_threads) {
+    const uint4* p = src(i);
+    amax = fmaxf(amax, fmaxf(abs_max<kBf16>(ld_global(p)), abs_max<kBf16>(ld_global(p + 1))));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if (!kWarp) {
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
+    __syncthreads();
+    for (int i = 0; i < (blockDim.x >> 5); ++i) amax = fmaxf(amax, part[i]);
+  }
+  float d = scale_for<kE5M2>(amax);
+  if (w.off > 0) {
+    d = fmaxf(old, d);
+    if (d > old) {
+      const float f = old / d;
+      uint4* const older = reinterpret_cast<uint4*>(y);
+      for (int i = tid; i < w.off * per_row; i += n_threads) {
+        const uint4 c = ld_global(older + i);
+        const uint32_t in4[4] = {c.x, c.y, c.z, c.w};
+        uint32_t out4[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t lo, hi;
+          fp8_to_half4<kE5M2>(in4[k], lo, hi);
+          const float2 p = half_pair<false>(lo), q = half_pair<false>(hi);
+          out4[k] = fp8_pair<kE5M2>(p.x * f, p.y * f) | (fp8_pair<kE5M2>(q.x * f, q.y * f) << 16);
+        }
+        older[i] = make_uint4(out4[0], out4[1], out4[2], out4[3]);
+      }
+    }
+  }
+  if (tid == 0) *descale = d;                             // every thread has read the old one: the reduction lies between
+  const float inv = 1.f / d;
+  uint4* const dst = reinterpret_cast<uint4*>(y + w.off * D);
+#pragma unroll
+  for (int h = 0; h < kHold; ++h) {
+    const int i = tid + h * n_threads;
+    if (i < chunks) {
+      const uint2 lo = to_fp8x8<kBf16, kE5M2>(hold[h][0], inv), hi = to_fp8x8<kBf16, kE5M2>(hold[h][1], inv);
+      dst[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+  }
+  for (int i = tid + kHold * n_threads; i < chunks; i += n_threads) {
+    const uint4* p = src(i);
+    const uint2 lo = to_fp8x8<kBf16, kE5M2>(ld_global(p), inv), hi = to_fp8x8<kBf16, kE5M2>(ld_global(p + 1), inv);
+    dst[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+  }
+}
+
+template <bool kBf16, bool kE5M2, bool kWarp>
+__global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_read_kernel(const KvArgs a, uint16_t* k_out, uint16_t* v_out,
+                                                                                          int64_t units, uint32_t magic) {
+  start_after_predecessor();
+  let_successor_start();
+  const int tid = kWarp ? threadIdx.x & 31 : threadIdx.x, n_threads = kWarp ? 32 : blockDim.x;
+  const int64_t u = kWarp ? static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5) : blockIdx.x;
+  if (u >= units) return;
+  const Unit w = find_unit<true>(a, u);
+  const int D = a.head_dim, per_row = D >> 4, chunks = w.rows * per_row;
+  if (chunks == 0) return;
+  const int64_t page_head = static_cast<int64_t>(w.page < 0 ? 0 : w.page) * a.heads + w.head;
+  const uint8_t* x = (w.of_v ? a.v : a.k) + ((page_head << a.page_shift) + w.off) * D;
+  const float d = w.page < 0 ? 0.f : ld_global((w.of_v ? a.v_descale : a.k_descale) + page_head);
+  const int64_t row = static_cast<int64_t>(a.heads) * D;
+  uint16_t* const y = (w.of_v ? v_out : k_out) + w.row0 * row + w.head * D;
+  for (int i0 = tid; i0 < chunks; i0 += kHold * n_threads) {
+    uint4 c[kHold];
+#pragma unroll
+    for (int h = 0; h < kHold; ++h) {
+      const int i = i0 + h * n_threads;
+      c[h] = make_uint4(0u, 0u, 0u, 0u);
+      if (i < chunks && w.page >= 0) c[h] = ld_stream16(x + 16 * static_cast<int64_t>(i));
+    }
+#pragma unroll
+    for (int h = 0; h < kHold; ++h) {
+      const int i = i0 + h * n_threads;
+      if (i >= chunks) continue;
+      const uint32_t in4[4] = {c[h].x, c[h].y, c[h].z, c[h].w};
+      uint32_t out8[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t lo, hi;
+        fp8_to_half4<kE5M2>(in4[k], lo, hi);
+        const float2 p = half_pair<false>(lo), q = half_pair<false>(hi);
+        out8[2 * k] = pack_pair<kBf16>(p.x * d, p.y * d);
+        out8[2 * k + 1] = pack_pair<kBf16>(q.x * d, q.y * d);
+      }
+      const int r = row_of(i, magic);
+      uint16_t* const p = y + r * row + 16 * (i - r * per_row);
+      st_global_v4(p, out8[0], out8[1], out8[2], out8[3]);
+      st_global_v4(p + 8, out8[4], out8[5], out8[6], out8[7]);
+    }
+  }
+}
+
+// Threads of a unit: enough to hold what an average one has to move.
+struct UnitPlan {
+  int64_t units;
+  int threads;                       // of a CTA; a warp's unit below that
+  bool warp;
+  uint32_t magic;
+  cudaLaunchConfig_t cfg;
+};
+bool plan_units(const KvArgs& a, cudaStream_t stream, cudaLaunchAttribute* attr, UnitPlan* p) {
+  p->units = kv_slots(a.batch, a.tokens, a.even, a.cu != nullptr, a.page_shift, 2) * 2 * a.heads;
+  const int P = 1 << a.page_shift;
+  const int mean = a.cu != nullptr ? (a.tokens + a.batch - 1) / a.batch : a.even;
+  const int work = (mean < P ? mean : P) * a.head_dim;
+  p->warp = work <= kWarpWork;
+  p->threads = p->warp ? 32 * kWarpsPerCta : (work / (kHold * 16) + 31) / 32 * 32;
+  if (p->threads > kMaxThreads) p->threads = kMaxThreads;
+  p->magic = 65536u / static_cast<uint32_t>(a.head_dim / 16) + 1u;
+  const int64_t ctas = p->warp ? (p->units + kWarpsPerCta - 1) / kWarpsPerCta : p->units;
+  if (ctas > 0x7fffffff) return false;
+  p->cfg = cudaLaunchConfig_t{};
+  p->cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
+  p->cfg.blockDim = dim3(static_cast<unsigned>(p->threads), 1, 1);
+  p->cfg.stream = stream;
+  attr[0] = overlap_attribute();
+  p->cfg.attrs = attr;
+  p->cfg.numAttrs = 1;
+  return true;
+}
+
+template <bool kBf16, bool kE5M2>
+cudaError_t append(const KvArgs& a, const KvRows& k, const KvRows& v, cudaStream_t stream) {
+  cudaLaunchAttribute attr[1];
+  UnitPlan p;
+  if (!plan_units(a, stream, attr, &p)) return cudaErrorInvalidConfiguration;
+  return cudaLaunchKernelEx(&p.cfg, p.warp ? &kv_append_kernel<kBf16, kE5M2, true> : &kv_append_kernel<kBf16, kE5M2, false>, a, k, v,
+                            p.units, p.magic);
+}
+
+template <bool kBf16, bool kE5M2>
+cudaError_t read(const KvArgs& a, void* k_out, void* v_out, cudaStream_t stream) {
+  cudaLaunchAttribute attr[1];
+  UnitPlan p;
+  if (!plan_units(a, stream, attr, &p)) return cudaErrorInvalidConfiguration;
+  return cudaLaunchKernelEx(&p.cfg, p.warp ? &kv_read_kernel<kBf16, kE5M2, true> : &kv_read_kernel<kBf16, kE5M2, false>, a,
+                            static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out), p.units, p.magic);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_append(const KvArgs& a, const KvRows& k, const KvRows& v, bool bf16, bool e5m2, cudaStream_t stream) {
+  if (bf16) return e5m2 ? append<true, true>(a, k, v, stream) : append<true, false>(a, k, v, stream);
+  return e5m2 ? append<false, true>(a, k, v, stream) : append<false, false>(a, k, v, stream);
+}
+
+cudaError_t launch_kv_read(const KvArgs& a, void* k_out, void* v_out, bool bf16, bool e5m2, cudaStream_t stream) {
+  if (bf16) return e5m2 ? read<true, true>(a, k_out, v_out, stream) : read<true, false>(a, k_out, v_out, stream);
+  return e5m2 ? read<false, true>(a, k_out, v_out, stream) : read<false, false>(a, k_out, v_out, stream);
+}
+
+}  // namespace fa8

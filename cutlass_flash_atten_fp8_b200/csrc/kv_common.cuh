@@ -1,0 +1,138 @@
+// Device code shared by the kernels of the paged fp8 cache: which tokens and pages a sequence has,
+// with every number that comes from device memory checked, and fp8 conversions.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "fa8_kv.h"
+#include "ptx_sm100.cuh"
+
+namespace fa8 {
+
+__device__ __forceinline__ int ld_int(const int* p) {
+  int v;
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ void report_bad_index(const KvArgs& a) {
+  if (a.status != nullptr) atomicCAS(a.status, 0, kBadIndex);
+  if (a.host_status != nullptr && *reinterpret_cast<volatile int*>(a.host_status) == 0)
+    *reinterpret_cast<volatile int*>(a.host_status) = kBadIndex;
+}
+
+// New tokens of sequence b: rows first .. first + n - 1 of the token-major tensors; len tokens in
+// all.  A range or length that is out of range is `bad` and comes back as n = 0 (range) or len = 0.
+struct KvSeq {
+  int first, n, len;
+  bool bad;
+};
+__device__ __forceinline__ KvSeq kv_seq(const KvArgs& a, int b) {
+  KvSeq s;
+  s.len = ld_int(a.seqlens + b);
+  s.bad = false;
+  if (a.cu != nullptr) {
+    const int lo = ld_int(a.cu + b), hi = ld_int(a.cu + b + 1);
+    s.first = lo;
+    s.n = hi - lo;
+    if (lo < 0 || hi < lo || hi > a.tokens) {
+      s.bad = true;
+      s.first = s.n = 0;
+    }
+  } else {
+    s.first = b * a.even;
+    s.n = a.even;
+  }
+  if (s.len < 0 || s.len > (static_cast<int64_t>(a.table_width) << a.page_shift)) {
+    s.bad = true;
+    s.len = 0;
+  }
+  return s;
+}
+
+// Work is dealt out in slots of a host-known number, a slot being one block of 2^shift tokens of one
+// sequence at most.  Even batches: `per_seq` slots each.  Otherwise sequence b has the slots from
+// cu[b] / 2^shift + extra * b on.  extra = 1 covers blocks counted from a sequence's first new token
+// (ceil(n / T) <= floor(cu[b+1] / T) - floor(cu[b] / T) + 1), extra = 2 blocks at fixed places of the
+// sequence, which the new tokens may enter and leave in the middle.
+__host__ __device__ inline int64_t kv_slots(int batch, int tokens, int even, bool ragged, int shift, int extra) {
+  if (ragged) return (static_cast<int64_t>(tokens) >> shift) + static_cast<int64_t>(extra) * batch;
+  const int T = 1 << shift;
+  return batch * ((static_cast<int64_t>(even) + T - 1) / T + (extra - 1));
+}
+
+// Sequence of a slot and the slot's number within it, by the calling warp (all lanes alike).
+// A search over 32 places at a time: two rounds of loads up to 1024 sequences.
+__device__ __forceinline__ void kv_find_slot(const KvArgs& a, int64_t slot, int shift, int extra, int* seq, int* j) {
+  if (a.cu == nullptr) {
+    const int T = 1 << shift;
+    const int per_seq = (a.even + T - 1) / T + (extra - 1);
+    *seq = static_cast<int>(slot / per_seq);
+    *j = static_cast<int>(slot - static_cast<int64_t>(*seq) * per_seq);
+    return;
+  }
+  // largest b in [0, batch) whose first slot is not past `slot` (cu may hold anything: it is clamped,
+  // and then checked by kv_seq)
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = a.batch;
+  while (n > 1) {
+    const int step = (n + 31) >> 5;
+    const int at = lo + lane * step;
+    bool before = false;
+    if (at < lo + n) {
+      const int t = min(max(ld_int(a.cu + at), 0), a.tokens);
+      before = (t >> shift) + static_cast<int64_t>(extra) * at <= slot;
+    }
+    const int count = __popc(__ballot_sync(0xffffffffu, before));
+    const int from = lo + max(count - 1, 0) * step;
+    n = min(step, lo + n - from);
+    lo = from;
+  }
+  const int t = min(max(ld_int(a.cu + lo), 0), a.tokens);
+  *seq = lo;
+  const int64_t d = slot - ((t >> shift) + static_cast<int64_t>(extra) * lo);
+  *j = d < 0 ? 0x3fffffff : static_cast<int>(d < 0x3fffffff ? d : 0x3fffffff);
+}
+
+// Page p of sequence b (p < table_width), or -1 with a report.
+__device__ __forceinline__ int kv_page(const KvArgs& a, int b, int p) {
+  const int page = ld_int(a.table + static_cast<int64_t>(b) * a.table_stride + p);
+  if (static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages)) return page;
+  report_bad_index(a);
+  return -1;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ float2 half_pair(uint32_t w) {
+  if (kBf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  uint32_t r;
+  if (kBf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Four fp8 -> two pairs of fp16, ascending (exact).
+template <bool kE5M2>
+__device__ __forceinline__ void fp8_to_half4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (kE5M2) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e5m2x2 %0, l;\n\tcvt.rn.f16x2.e5m2x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  }
+}
+// Two fp32 -> two fp8, to the nearest, saturating.
+template <bool kE5M2>
+__device__ __forceinline__ uint32_t fp8_pair(float lo, float hi) {
+  uint16_t r;
+  if (kE5M2) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+}  // namespace fa8

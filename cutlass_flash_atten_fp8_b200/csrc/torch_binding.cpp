@@ -12,6 +12,7 @@
 // synchronise the device, and every failure is a C++ exception (RuntimeError in Python) instead
 // of exit().  Two keyword arguments are added after the reference's five: v_layout
 // ("transposed", the reference's [batch, heads, head_dim, seqlen], or "natural") and o_scale.
+#include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -22,6 +23,7 @@
 #include <vector>
 
 #include "fa8_b200.h"
+#include "fa8_kv_cache.h"
 
 namespace {
 
@@ -219,6 +221,151 @@ py::object quantize(const torch::Tensor& x, bool per_head) {
   return py::make_tuple(x8, scal.slice(0, n_seg));
 }
 
+// ---- the package's paged cache (paged_kv.py), the same way --------------------------------
+
+// Everything but the tables: fp8 pools alike, fp32 scales.
+bool fill_cache(fa8_kv_cache& c, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& kd, const torch::Tensor& vd) {
+  const auto dev = k.device();
+  const auto dtype = k.scalar_type();
+  if (!dev.is_cuda() || !plain(k, dev) || !plain(v, dev) || !plain(kd, dev) || !plain(vd, dev)) return false;
+  if ((dtype != at::kFloat8_e4m3fn && dtype != at::kFloat8_e5m2) || v.scalar_type() != dtype) return false;
+  if (k.dim() != 4 || k.sizes() != v.sizes() || k.numel() == 0) return false;
+  for (int i = 0; i < 4; ++i)
+    if (k.size(i) > INT32_MAX) return false;
+  const int64_t P = k.size(2), D = k.size(3);
+  if ((P != 16 && P != 32 && P != 64 && P != 128) || D % 32 != 0 || D > 256) return false;
+  for (const torch::Tensor* d : {&kd, &vd})
+    if (d->scalar_type() != at::kFloat || d->dim() != 2 || d->size(0) != k.size(0) || d->size(1) != k.size(1)) return false;
+  c.k = k.data_ptr();
+  c.v = v.data_ptr();
+  c.k_descale = static_cast<float*>(kd.data_ptr());
+  c.v_descale = static_cast<float*>(vd.data_ptr());
+  c.num_pages = static_cast<int32_t>(k.size(0));
+  c.heads_kv = static_cast<int32_t>(k.size(1));
+  c.page_size = static_cast<int32_t>(k.size(2));
+  c.head_dim = static_cast<int32_t>(k.size(3));
+  c.fp8_format = dtype == at::kFloat8_e5m2 ? FA8_FP8_E5M2 : FA8_FP8_E4M3;
+  const int64_t word = dev.index() >= 0 && dev.index() < kMaxDevices ? g_status_words[dev.index()].load() : 0;
+  c.status_word = reinterpret_cast<int32_t*>(word);
+  return word != 0;
+}
+
+bool fill_tables(fa8_kv_cache& c, const c10::Device& dev, const torch::Tensor& table, const torch::Tensor& seqlens,
+                 const std::optional<torch::Tensor>& cu, int64_t tokens) {
+  if (table.device() != dev || seqlens.device() != dev || table.scalar_type() != at::kInt || seqlens.scalar_type() != at::kInt) return false;
+  if (table.dim() != 2 || seqlens.dim() != 1 || !seqlens.is_contiguous()) return false;
+  const int64_t batch = seqlens.size(0), width = table.size(1);
+  if (tokens <= 0 || tokens > INT32_MAX || batch <= 0 || batch > INT32_MAX || width <= 0 || width > INT32_MAX) return false;
+  if (table.size(0) != batch || (table.stride(1) != 1 && width > 1)) return false;
+  const int64_t stride = batch > 1 ? table.stride(0) : width;
+  if (stride < width || stride > INT32_MAX) return false;
+  if (cu) {
+    if (cu->device() != dev || cu->scalar_type() != at::kInt || cu->dim() != 1 || !cu->is_contiguous() || cu->size(0) != batch + 1) return false;
+  } else if (tokens % batch != 0) {
+    return false;
+  }
+  c.batch = static_cast<int32_t>(batch);
+  c.page_table = static_cast<const int32_t*>(table.data_ptr());
+  c.table_width = static_cast<int32_t>(width);
+  c.table_stride = static_cast<int32_t>(stride);
+  c.seqlens = static_cast<const int32_t*>(seqlens.data_ptr());
+  c.cu_seqlens = cu ? static_cast<const int32_t*>(cu->data_ptr()) : nullptr;
+  c.tokens = static_cast<int32_t>(tokens);
+  return true;
+}
+
+bool rows_of(const torch::Tensor& x, const c10::Device& dev, int64_t head_dim) {
+  if (x.device() != dev || (x.scalar_type() != at::kHalf && x.scalar_type() != at::kBFloat16)) return false;
+  if (x.dim() != 3 || x.size(2) != head_dim || x.stride(2) != 1 || x.stride(0) % 8 != 0 || x.stride(1) % 8 != 0) return false;
+  return reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && !(at::GradMode::is_enabled() && x.requires_grad());
+}
+
+int32_t half_of(const torch::Tensor& x) { return x.scalar_type() == at::kBFloat16 ? FA8_DTYPE_BF16 : FA8_DTYPE_FP16; }
+
+py::object kv_append(const torch::Tensor& k8, const torch::Tensor& v8, const torch::Tensor& kd, const torch::Tensor& vd,
+                     const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& table, const torch::Tensor& seqlens,
+                     const std::optional<torch::Tensor>& cu) {
+  fa8_kv_cache c{};
+  if (!fill_cache(c, k8, v8, kd, vd)) return py::none();
+  const auto dev = k8.device();
+  if (!rows_of(k, dev, c.head_dim) || !rows_of(v, dev, c.head_dim) || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type()) return py::none();
+  if (k.size(1) != c.heads_kv || !fill_tables(c, dev, table, seqlens, cu, k.size(0))) return py::none();
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  int rc;
+  {
+    const py::gil_scoped_release nogil;
+    rc = fa8_kv_append(&c, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), half_of(k),
+                       c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  }
+  return py::int_(rc);
+}
+
+py::object kv_read(const torch::Tensor& k8, const torch::Tensor& v8, const torch::Tensor& kd, const torch::Tensor& vd,
+                   const torch::Tensor& table, const torch::Tensor& seqlens, int64_t tokens, const std::optional<torch::Tensor>& cu, bool bf16) {
+  fa8_kv_cache c{};
+  if (!fill_cache(c, k8, v8, kd, vd) || !fill_tables(c, k8.device(), table, seqlens, cu, tokens)) return py::none();
+  const auto dev = k8.device();
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  const auto opt = k8.options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
+  torch::Tensor k = at::empty({tokens, c.heads_kv, c.head_dim}, opt), v = at::empty({tokens, c.heads_kv, c.head_dim}, opt);
+  int rc;
+  {
+    const py::gil_scoped_release nogil;
+    rc = fa8_kv_read(&c, k.data_ptr(), v.data_ptr(), half_of(k), c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  }
+  if (rc != FA8_OK) return py::int_(rc);
+  return py::make_tuple(k, v);
+}
+
+py::object kv_attention(const torch::Tensor& q, const torch::Tensor& k8, const torch::Tensor& v8, const torch::Tensor& kd,
+                        const torch::Tensor& vd, const torch::Tensor& table, const torch::Tensor& seqlens, bool is_causal,
+                        double softmax_scale, const std::optional<torch::Tensor>& cu, const std::optional<torch::Tensor>& out_given,
+                        bool return_lse) {
+  fa8_kv_attention_params p{};
+  if (!fill_cache(p.cache, k8, v8, kd, vd)) return py::none();
+  const auto dev = k8.device();
+  if (!rows_of(q, dev, p.cache.head_dim) || !fill_tables(p.cache, dev, table, seqlens, cu, q.size(0))) return py::none();
+  const int64_t T = q.size(0), H = q.size(1);
+  if (H <= 0 || H > INT32_MAX || H % p.cache.heads_kv != 0) return py::none();
+  torch::Tensor out;
+  if (out_given) {
+    out = *out_given;
+    if (!plain(out, dev) || out.scalar_type() != q.scalar_type() || out.sizes() != q.sizes() ||
+        reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 != 0)
+      return py::none();
+  }
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  const int64_t need = fa8_kv_attention_workspace(p.cache.batch, p.cache.tokens, static_cast<int32_t>(H), p.cache.heads_kv, p.cache.head_dim,
+                                                  p.cache.page_size, p.cache.table_width,
+                                                  at::cuda::getDeviceProperties(dev.index())->multiProcessorCount);
+  if (need < 0) return py::int_(static_cast<int>(need));
+  if (!out_given) out = at::empty({T, H, p.cache.head_dim}, q.options());
+  torch::Tensor lse, workspace;
+  if (return_lse) lse = at::empty({T, H}, q.options().dtype(at::kFloat));
+  if (need > 0) workspace = at::empty({need}, q.options().dtype(at::kByte));
+  p.q = q.data_ptr();
+  p.q_token_stride = q.stride(0);
+  p.q_head_stride = q.stride(1);
+  p.o = out.data_ptr();
+  p.lse = return_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
+  p.dtype = half_of(q);
+  p.heads = static_cast<int32_t>(H);
+  p.is_causal = is_causal ? 1 : 0;
+  p.softmax_scale = static_cast<float>(softmax_scale);
+  p.workspace = need > 0 ? workspace.data_ptr() : nullptr;
+  p.workspace_bytes = need;
+  int rc;
+  {
+    const py::gil_scoped_release nogil;
+    rc = fa8_kv_attention(&p, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  }
+  if (rc != FA8_OK) return py::int_(rc);
+  py::list result;
+  result.append(out);
+  if (return_lse) result.append(lse);
+  return std::move(result);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -231,6 +378,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("device_index") = -1);
   m.def("_forward", &forward, "the package's operator: a list of outputs, None (something is wrong with the call) or an error code");
   m.def("_quantize", &quantize, "the package's quantize_e4m3, the same way");
+  m.def("_kv_append", &kv_append, "the package's paged_kv_append: an error code (0 = done) or None (something is wrong with the call)");
+  m.def("_kv_read", &kv_read, "the package's paged_kv_read: (k, v), None or an error code");
+  m.def("_kv_attention", &kv_attention, "the package's flash_attention_paged_kv: a list of outputs, None or an error code");
   m.def("_set_status_word", &set_status_word);
   m.def("abi_version", [] { return fa8_version(); }, "version of the C ABI the module was linked against");
 }

@@ -54,7 +54,7 @@ setup(
                 "weishengying/cutlass_flash_atten_fp8",
     packages=[PKG],
     package_data={PKG: ["csrc/*", "*.so", "*.srchash"]},
-    data_files=[("include", ["include/fa8_b200.h"])],
+    data_files=[("include", ["include/fa8_b200.h", "include/fa8_kv_cache.h"])],
     # one placeholder so that build_ext runs; BuildNative.run does the work
     ext_modules=[Extension("attention_cutlass_fp8", sources=[])],
     cmdclass={"build_ext": BuildNative},
