@@ -208,6 +208,9 @@ void status_words(int** dev_word, int** host_word) {
   *host_word = st ? st->host_flag_dev : nullptr;
 }
 int earlier_failure(int32_t* caller_word, cudaStream_t stream) { return refuse_after_failure(device_state(), caller_word, stream); }
+bool make_byte_map(CUtensorMap* out, const void* base, uint64_t inner, uint64_t mid, uint64_t outer, uint32_t box_inner, uint32_t box_mid) {
+  return make_map_3d(out, base, inner, mid, outer, box_inner, box_mid, box_inner == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+}
 void clear_error_detail() { g_detail[0] = '\0'; }
 void set_error_detail(const char* what, const char* msg) { set_detail(what, msg); }
 

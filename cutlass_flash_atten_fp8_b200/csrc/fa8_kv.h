@@ -51,9 +51,25 @@ struct KvAttendArgs {
   int heads_q;
   int group;                      // heads_q / heads
   int causal;
+  int bf16;                       // of q and o; fp16 otherwise
   float scale_log2;               // softmax_scale * log2(e)
+  // In the workspace, filled in by launch_kv_attend: see fa8_kv_attend.cu.
+  int64_t* bases;                 // [batch + 1]
+  float* partial;
 };
-cudaError_t launch_kv_attend(const KvAttendArgs& a, bool bf16, bool e5m2, cudaStream_t stream);
+// tk, tv: the pools as 3-D byte tensors {head_dim, page_size, num_pages * heads} with a box of
+// kv_box_bytes(head_dim) x min(page_size, 32) x 1, swizzled over the box's row.
+cudaError_t launch_kv_attend(const CUtensorMap& tk, const CUtensorMap& tv, KvAttendArgs a, void* workspace, bool e5m2, int sms,
+                             cudaStream_t stream);
+struct KvAttendSizes {
+  int batch, tokens, heads_q, heads, head_dim;
+};
+int64_t kv_attend_workspace(const KvAttendSizes& z, int sms);
+inline int kv_box_bytes(int head_dim) { return head_dim <= 64 ? 64 : 128; }
+
+// fa8_capi.cu: a 3-D byte tensor {inner, mid, outer} with a {box_inner, box_mid, 1} tile, swizzled over
+// box_inner bytes (64 or 128).  False, with the detail string set, on failure.
+bool make_byte_map(CUtensorMap* out, const void* base, uint64_t inner, uint64_t mid, uint64_t outer, uint32_t box_inner, uint32_t box_mid);
 
 // fa8_capi.cu: the library's status words on the current device (null where there are none), a
 // failure that an earlier launch left there (0 = none, an FA8_ERR code otherwise, words cleared), and

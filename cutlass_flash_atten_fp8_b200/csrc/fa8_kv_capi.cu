@@ -107,7 +107,8 @@ int64_t fa8_kv_attention_workspace(int32_t batch, int32_t tokens, int32_t heads,
   if (batch <= 0 || tokens < 0 || heads <= 0 || heads_kv <= 0 || heads % heads_kv != 0 || head_dim <= 0 || page_size <= 0 ||
       table_width <= 0 || sm_count <= 0)
     return FA8_ERR_BAD_ARG;
-  return 0;
+  if (head_dim > 256) return FA8_ERR_UNSUPPORTED;
+  return tokens == 0 ? 0 : fa8::kv_attend_workspace({batch, tokens, heads, heads_kv, head_dim}, sm_count);
 }
 
 int fa8_kv_attention(const fa8_kv_attention_params* p, void* cuda_stream) {
@@ -127,10 +128,43 @@ int fa8_kv_attention(const fa8_kv_attention_params* p, void* cuda_stream) {
   a.heads_q = p->heads;
   a.group = p->heads / p->cache.heads_kv;
   a.causal = p->is_causal != 0;
+  a.bf16 = p->dtype == FA8_DTYPE_BF16;
   a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
+  cudaError_t e = cudaSuccess;
+  const int sms = fa8::current_sm_count(&e);
+  if (sms <= 0) {
+    fa8::set_error_detail("SM count", cudaGetErrorString(e));
+    return FA8_ERR_CUDA;
+  }
+  if (!p->workspace || !aligned(p->workspace, 256) ||
+      p->workspace_bytes < fa8::kv_attend_workspace({a.c.batch, a.c.tokens, a.heads_q, a.c.heads, a.c.head_dim}, sms))
+    return FA8_ERR_BAD_ARG;
+  // The pool's tensor maps depend on its address and shape only: a thread keeps those of its last call.
+  struct Maps {
+    const void *k, *v;
+    int64_t slices;
+    int32_t page_size, head_dim;
+    bool valid;
+    CUtensorMap tk, tv;
+  };
+  thread_local Maps m{};
+  const fa8_kv_cache& c = p->cache;
+  const int64_t slices = static_cast<int64_t>(c.num_pages) * c.heads_kv;
+  if (!(m.valid && m.k == c.k && m.v == c.v && m.slices == slices && m.page_size == c.page_size && m.head_dim == c.head_dim)) {
+    m.valid = false;
+    const uint32_t inner = static_cast<uint32_t>(fa8::kv_box_bytes(c.head_dim)), rows = c.page_size < 32 ? 16u : 32u;
+    if (!fa8::make_byte_map(&m.tk, c.k, c.head_dim, c.page_size, slices, inner, rows)) return FA8_ERR_CUDA;
+    if (!fa8::make_byte_map(&m.tv, c.v, c.head_dim, c.page_size, slices, inner, rows)) return FA8_ERR_CUDA;
+    m.k = c.k;
+    m.v = c.v;
+    m.slices = slices;
+    m.page_size = c.page_size;
+    m.head_dim = c.head_dim;
+    m.valid = true;
+  }
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   if (const int rc = begin(&p->cache, &a.c, stream)) return rc;
-  return launched(fa8::launch_kv_attend(a, p->dtype == FA8_DTYPE_BF16, p->cache.fp8_format == FA8_FP8_E5M2, stream));
+  return launched(fa8::launch_kv_attend(m.tk, m.tv, a, p->workspace, c.fp8_format == FA8_FP8_E5M2, sms, stream));
 }
 
 }  // extern "C"
