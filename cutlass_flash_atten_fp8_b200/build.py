@@ -21,7 +21,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libfa8_b200.so")
 # file contents but not necessarily modification times, so staleness is decided by content.
 HASH_PATH = os.path.join(PKG_DIR, "libfa8_b200.srchash")
 SOURCES = ["fa8_fwd_sm100.cu", "fa8_decode_sm100.cu", "fa8_quant.cu", "fa8_capi.cu",
-           "fa8_kv_cache.cu", "fa8_kv_attend.cu", "fa8_kv_capi.cu"]
+           "fa8_kv_cache.cu", "fa8_kv_attend.cu", "fa8_kv_prefill.cu", "fa8_kv_capi.cu"]
 HEADERS = ["fa8_kernel.h", "fa8_kv.h", "kv_common.cuh", "phase_rule.h", "ptx_sm100.cuh",
            os.path.join(REPO_DIR, "include", "fa8_b200.h"), os.path.join(REPO_DIR, "include", "fa8_kv_cache.h")]
 

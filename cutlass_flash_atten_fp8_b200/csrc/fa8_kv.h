@@ -57,14 +57,31 @@ struct KvAttendArgs {
   int64_t* bases;                 // [batch + 1]
   float* partial;
 };
-// tk, tv: the pools as 3-D byte tensors {head_dim, page_size, num_pages * heads} with a box of
-// kv_box_bytes(head_dim) x min(page_size, 32) x 1, swizzled over the box's row.
-cudaError_t launch_kv_attend(const CUtensorMap& tk, const CUtensorMap& tv, KvAttendArgs a, void* workspace, bool e5m2, int sms,
-                             cudaStream_t stream);
 struct KvAttendSizes {
   int batch, tokens, heads_q, heads, head_dim;
+  bool ragged;                    // cu_seqlens given
+  int64_t keys_most;              // that a sequence can have: table_width * page_size
 };
+// tk, tv: the pools as 3-D byte tensors {head_dim, page_size, num_pages * heads} with a box of
+// kv_box_bytes(head_dim) x min(page_size, 32) x 1, swizzled over the box's row.
+cudaError_t launch_kv_attend(const CUtensorMap& tk, const CUtensorMap& tv, KvAttendArgs a, const KvAttendSizes& z, void* workspace,
+                             bool e5m2, int sms, cudaStream_t stream);
 int64_t kv_attend_workspace(const KvAttendSizes& z, int sms);
+
+// Many rows per sequence and K/V head (fa8_kv_prefill.cu).
+struct KvPrefillPlan {
+  int64_t items;                  // sequence, block of new tokens, K/V head, part
+  int block_tokens;
+  int parts;                      // that an item's keys are cut into
+  float* partial_o;               // [parts, tokens, heads_q, head_dim]
+  float* partial_ml;              // [parts, tokens, heads_q, 2]
+};
+KvPrefillPlan kv_prefill_plan(const KvAttendSizes& z, int sms);
+int64_t kv_prefill_workspace(const KvAttendSizes& z, int sms);
+cudaError_t launch_kv_prefill(const CUtensorMap& tk, const CUtensorMap& tv, const KvAttendArgs& a, const KvAttendSizes& z, void* workspace,
+                              bool e5m2, int sms, cudaStream_t stream);
+// Whether a call is one for launch_kv_prefill.
+bool kv_prefill_takes(const KvAttendSizes& z);
 inline int kv_box_bytes(int head_dim) { return head_dim <= 64 ? 64 : 128; }
 
 // fa8_capi.cu: a 3-D byte tensor {inner, mid, outer} with a {box_inner, box_mid, 1} tile, swizzled over

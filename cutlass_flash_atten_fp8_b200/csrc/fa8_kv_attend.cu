@@ -1,11 +1,11 @@
 // Attention of a few new tokens' queries over the pages of the fp8 cache (decoding), sm_100a.
 //
-//   x_j = c (q . k8_j) dk_j,   m >= x_j + log2 dv_j - 8,   O = sum_j 2^(x_j - m) dv_j v8_j / sum_j 2^(x_j - m)
+//   x_j = c (q . k8_j) dk_j,   m >= x_j + log2 dv_j - 14,   O = sum_j 2^(x_j - m) dv_j v8_j / sum_j 2^(x_j - m)
 //
 // with c = softmax_scale log2(e) and dk_j, dv_j the scales of key j's page.  The reference m of a row is taken over x + log2 dv,
-// so that what is rounded to fp16, P_j = 2^(x_j - m) dv_j, is at most 2^8 whatever the pages' scales; the sum of the
-// denominators is of unrounded fp32 numbers.  m is raised, and what was summed rescaled, only when some P would pass
-// 2^8: fp16 keeps its relative precision up to there.  Keys and queries enter the products exactly: every fp8 value is an
+// so that what is rounded to fp16, P_j = 2^(x_j - m) dv_j, is at most 2^14 whatever the pages' scales; the sum of the
+// denominators is of unrounded fp32 numbers.  m starts 6 below the first keys' maximum, so that P has its full precision twenty
+// binades down, and is raised to 6 below the maximum so far, and what was summed rescaled, only when some P would pass 2^14.  Keys and queries enter the products exactly: every fp8 value is an
 // fp16 value, and bf16 queries are brought into fp16's range by a power of two per row (what that cuts off is below
 // 2^-39 of the row's largest).
 //
@@ -37,7 +37,7 @@ namespace fa8 {
 namespace {
 
 constexpr int kStepKeys = 32;
-constexpr float kRaiseBy = 8.f;                        // log2 of the largest P
+constexpr float kHeadroom = 6.f, kRaiseBy = 14.f;       // log2 of the largest P under a fresh reference, and at all
 constexpr float kLog2Least = -100.f;                   // log2 of the smallest scale of V that the reference m follows
 constexpr unsigned long long kLimitNs = 2000000000ull; // bound of every wait
 
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
           float mx = fmaxf(top[b], __shfl_xor_sync(0xffffffffu, top[b], 1));
-          mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)), m_row[b]);
+          mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) - kHeadroom, m_row[b]);
           const float nm_new = mx == -INFINITY ? 0.f : -mx;
           const float alpha = m_row[b] == -INFINITY ? 0.f : ex2_approx(nm_new - nm[b]);
           l_row[b] *= alpha;
@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) kv_combine_kernel(const Kv
   if (token >= a.c.tokens) return;                        // kParts > 1: the returns are the whole CTA's
   int b, unused;
   if (a.c.cu == nullptr) b = token / a.c.even;
-  else kv_find_slot(a.c, token, 0, 0, &b, &unused);
+  else kv_find_slot(a.c, token, 1, 0, &b, &unused);
   const KvSeq s = kv_seq(a.c, b);
   if (token < s.first || token >= s.first + s.n) return;
   const volatile int64_t* bases = a.bases;
@@ -717,8 +717,8 @@ int64_t kv_attend_workspace(const KvAttendSizes& z, int sms) {
   return round256((static_cast<int64_t>(z.batch) + 1) * 8) + slots * block_rows(z) * (z.head_dim + 2) * 4;
 }
 
-cudaError_t launch_kv_attend(const CUtensorMap& tk, const CUtensorMap& tv, KvAttendArgs a, void* workspace, bool e5m2, int sms, cudaStream_t stream) {
-  const KvAttendSizes z{a.c.batch, a.c.tokens, a.heads_q, a.c.heads, a.c.head_dim};
+cudaError_t launch_kv_attend(const CUtensorMap& tk, const CUtensorMap& tv, KvAttendArgs a, const KvAttendSizes& z, void* workspace, bool e5m2, int sms,
+                             cudaStream_t stream) {
   a.bases = static_cast<int64_t*>(workspace);
   a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256((static_cast<int64_t>(a.c.batch) + 1) * 8));
   const int rows = block_rows(z);

@@ -41,7 +41,7 @@ __device__ __forceinline__ Unit find_unit(const KvArgs& a, int64_t u) {
   r.head = r.of_v ? i - a.heads : i;
   r.page = -1;
   int b, j;
-  kv_find_slot(a, slot, a.page_shift, 2, &b, &j);
+  kv_find_slot(a, slot, 1 << a.page_shift, 2, &b, &j);
   const KvSeq s = kv_seq(a, b);
   const int P = 1 << a.page_shift;
   if (s.bad || s.n > s.len) {
@@ -255,7 +255,7 @@ struct UnitPlan {
   cudaLaunchConfig_t cfg;
 };
 bool plan_units(const KvArgs& a, cudaStream_t stream, cudaLaunchAttribute* attr, UnitPlan* p) {
-  p->units = kv_slots(a.batch, a.tokens, a.even, a.cu != nullptr, a.page_shift, 2) * 2 * a.heads;
+  p->units = kv_slots(a.batch, a.tokens, a.even, a.cu != nullptr, 1 << a.page_shift, 2) * 2 * a.heads;
   const int P = 1 << a.page_shift;
   const int mean = a.cu != nullptr ? (a.tokens + a.batch - 1) / a.batch : a.even;
   const int work = (mean < P ? mean : P) * a.head_dim;

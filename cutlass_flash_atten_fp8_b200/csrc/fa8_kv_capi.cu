@@ -3,6 +3,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -64,6 +65,10 @@ int begin(const fa8_kv_cache* c, fa8::KvArgs* a, cudaStream_t stream) {
   return FA8_OK;
 }
 
+int64_t workspace_of(const fa8::KvAttendSizes& z, int sms) {
+  return fa8::kv_prefill_takes(z) ? fa8::kv_prefill_workspace(z, sms) : fa8::kv_attend_workspace(z, sms);
+}
+
 int launched(cudaError_t e) {
   if (e == cudaSuccess) return FA8_OK;
   fa8::set_error_detail("kernel launch", cudaGetErrorString(e));
@@ -108,7 +113,12 @@ int64_t fa8_kv_attention_workspace(int32_t batch, int32_t tokens, int32_t heads,
       table_width <= 0 || sm_count <= 0)
     return FA8_ERR_BAD_ARG;
   if (head_dim > 256) return FA8_ERR_UNSUPPORTED;
-  return tokens == 0 ? 0 : fa8::kv_attend_workspace({batch, tokens, heads, heads_kv, head_dim}, sm_count);
+  if (tokens == 0) return 0;
+  // evenly divided or not: the larger of what either needs
+  int64_t most = 0;
+  for (const bool ragged : {false, true})
+    most = std::max(most, workspace_of({batch, tokens, heads, heads_kv, head_dim, ragged, static_cast<int64_t>(table_width) * page_size}, sm_count));
+  return most;
 }
 
 int fa8_kv_attention(const fa8_kv_attention_params* p, void* cuda_stream) {
@@ -120,6 +130,7 @@ int fa8_kv_attention(const fa8_kv_attention_params* p, void* cuda_stream) {
   if (p->heads <= 0 || p->heads % p->cache.heads_kv != 0) return FA8_ERR_BAD_ARG;
   if (!(p->softmax_scale > 0.f) || !std::isfinite(p->softmax_scale)) return FA8_ERR_BAD_ARG;
   if (!aligned(p->lse, 4)) return FA8_ERR_BAD_ARG;
+  if (static_cast<int64_t>(a.c.tokens) * p->heads > 0x7fffffff) return FA8_ERR_UNSUPPORTED;      // rows are 32-bit numbers
   if (a.c.tokens == 0) return FA8_OK;
   if (!rows_ok(p->q, p->q_token_stride, p->q_head_stride) || !rows_ok(p->o, 0, 0)) return FA8_ERR_BAD_ARG;
   a.q = {p->q, p->q_token_stride, p->q_head_stride};
@@ -136,9 +147,10 @@ int fa8_kv_attention(const fa8_kv_attention_params* p, void* cuda_stream) {
     fa8::set_error_detail("SM count", cudaGetErrorString(e));
     return FA8_ERR_CUDA;
   }
-  if (!p->workspace || !aligned(p->workspace, 256) ||
-      p->workspace_bytes < fa8::kv_attend_workspace({a.c.batch, a.c.tokens, a.heads_q, a.c.heads, a.c.head_dim}, sms))
-    return FA8_ERR_BAD_ARG;
+  const fa8::KvAttendSizes z{a.c.batch, a.c.tokens, a.heads_q, a.c.heads, a.c.head_dim, a.c.cu != nullptr,
+                             static_cast<int64_t>(a.c.table_width) << a.c.page_shift};
+  const int64_t need = workspace_of(z, sms);
+  if (need > 0 && (!p->workspace || !aligned(p->workspace, 256) || p->workspace_bytes < need)) return FA8_ERR_BAD_ARG;
   // The pool's tensor maps depend on its address and shape only: a thread keeps those of its last call.
   struct Maps {
     const void *k, *v;
@@ -164,7 +176,9 @@ int fa8_kv_attention(const fa8_kv_attention_params* p, void* cuda_stream) {
   }
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   if (const int rc = begin(&p->cache, &a.c, stream)) return rc;
-  return launched(fa8::launch_kv_attend(m.tk, m.tv, a, p->workspace, c.fp8_format == FA8_FP8_E5M2, sms, stream));
+  const bool e5m2 = c.fp8_format == FA8_FP8_E5M2;
+  return launched(fa8::kv_prefill_takes(z) ? fa8::launch_kv_prefill(m.tk, m.tv, a, z, p->workspace, e5m2, sms, stream)
+                                           : fa8::launch_kv_attend(m.tk, m.tv, a, z, p->workspace, e5m2, sms, stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,955 @@
+// Attention of many new tokens' queries over the pages of the fp8 cache (prompts, pieces of prompts), sm_100a.
+//
+// The formulas and the treatment of scales are those of fa8_kv_attend.cu; here a K/V head's query rows come in tiles of 128, and both
+// products run on the tensor cores in fp16 with fp32 accumulators in tensor memory (tcgen05.mma kind::f16): fp8 products would
+// need P, and Q, rounded to three bits.  What bounds it: per 128 keys and tile 1024 cycles of products and 1024 of
+// exponentials (16 per cycle and SM) at head dim 128.
+//
+// A CTA per SM, warps with roles, work items of two tiles (one at head dims above 128) of one sequence and K/V head:
+//   producer   looks up items and pages, copies K and V tiles of kN keys from the pages (fp8) into shared memory
+//   widening   four warps turn a tile into fp16, in the layout that the products want, times the power of two by which its pages' scales
+//              differ from the item's first page; keys past the last one become zeros (a NaN there must not meet a zero P)
+//   issuer     one thread: S = Q K^T into tensor memory, O += P V with P from tensor memory
+//   softmax    four warps a tile, a row to a thread: P = 2^(c s - m) over S as it lies, in halves of 64 keys that are handed over
+//              one by one; O to global memory at the end.
+// Two tiles keep the tensor cores and the exponentials busy in turns; at head dims above 128 O takes half of tensor memory
+// and the one tile has two score buffers instead.
+//
+// The row reference m lies 6 below the maximum over the item's first kN keys, so that P, at 2^6, has its full precision twenty
+// binades down, and is raised when a half's sum of P nears fp16's largest number, which is also when O is rescaled.  Scales that differ by more than fp16 can take in, or are no powers of two, go
+// through a slower form of the softmax that multiplies them in (`residual`).
+#include <cuda_runtime.h>
+
+#include <atomic>
+
+#include "fa8_kernel.h"
+#include "fa8_kv.h"
+#include "kv_common.cuh"
+
+namespace fa8 {
+
+namespace {
+
+constexpr int kTileM = 128;
+constexpr uint32_t kTmemCols = 512;
+constexpr unsigned long long kLimitNs = 2000000000ull;
+constexpr float kRaiseAbove = 60000.f;   // below fp16's largest number
+constexpr float kHeadroom = 6.f;         // a fresh reference puts the row's largest P at 2^6: fp16 is exact to half a step down to 2^-14
+constexpr float kLog2Least = -100.f;
+constexpr int kItemSlots = 4;
+constexpr int kBlockSlots = 8;           // blocks whose residual scales are kept: the producer is at most four ahead of the softmax
+
+template <int W>
+struct PCfg {
+  static constexpr int kTiles = W == 256 ? 1 : 2;
+  static constexpr int kN = W == 256 ? 64 : 128;               // keys of a block
+  static constexpr int kHalves = kN / 64;
+  static constexpr int kGroups = kN / 16;                      // of keys that share a page
+  static constexpr int kCols = W / 64;                         // column blocks of 64 fp16 (128 bytes)
+  static constexpr int kRawRow = W < 128 ? W : 128;            // bytes of a row of a raw (fp8) tile
+  static constexpr int kRawBlocks = W / kRawRow;
+  static constexpr int kRawBlockBytes = kN * kRawRow;
+  static constexpr int kRawBytes = kN * W;
+  static constexpr int kRaw = W == 64 ? 4 : 2;                 // raw tiles
+  static constexpr int kRing = 4;                              // widened tiles
+  static constexpr int kRingBytes = kN * W * 2;
+  static constexpr int kQBytes = kTileM * W * 2;               // of a tile
+  static constexpr int kOCol = W == 256 ? 128 : 256;           // O of tile i at kOCol + W i; S at 128 i, or 64 b
+  static constexpr int kSoftWarps = 4 * kTiles;
+  static constexpr int kWideWarp0 = kSoftWarps;
+  static constexpr int kLoadWarp = kWideWarp0 + 4;
+  static constexpr int kMmaWarp = kLoadWarp + 1;
+  static constexpr int kThreads = 32 * (kMmaWarp + 1);
+  static constexpr int kRawOffset = kTiles * kQBytes;
+  static constexpr int kRingOffset = kRawOffset + kRaw * kRawBytes;
+  static constexpr int kSharedOffset = kRingOffset + kRing * kRingBytes;
+  static_assert(kOCol + W * kTiles <= 512, "tensor memory");
+};
+
+struct Item {
+  int seq, head;
+  int first, n, len;                     // of the sequence
+  int token0, n_tokens;                  // its new tokens in the item
+  int blk0, blk1;                        // key blocks
+  int vis;                               // keys that the item's last row sees
+  int part;
+};
+
+template <int W>
+struct Shared {
+  using C = PCfg<W>;
+  uint64_t item_full[kItemSlots], item_empty[kItemSlots];
+  uint64_t raw_full[C::kRaw], raw_empty[C::kRaw];
+  uint64_t ring_full[C::kRing], ring_empty[C::kRing];
+  uint64_t q_full[2], s_full[2], p_full[2][2], o_half[2], o_final[2];
+  uint64_t blk_full[kBlockSlots];
+  uint64_t drain;
+  Item item[kItemSlots];                 // seq < 0: no more
+  uint32_t factor[C::kRaw][C::kGroups];  // fp16 pair to multiply a group of 16 keys by
+  int valid[C::kRaw];                    // rows of the tile that are keys
+  float residual[kBlockSlots][2][C::kGroups];   // of K and V; K's is -1 for a group without a page
+  float ref[kBlockSlots][2];             // reference scales of the item that the block is of
+  int flagged[kBlockSlots];              // some residual is not 1
+  uint32_t tmem;
+  int abort;
+};
+
+struct Wait {
+  volatile int* abort;
+  int* status;
+  volatile int* host_status;
+};
+__device__ __forceinline__ bool wait_bounded(const Wait& w, uint64_t* barrier, uint32_t parity, int code) {
+  const uint32_t bar = smem_u32(barrier);
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  uint32_t spins = 0;
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((++spins & 31u) == 0) {
+      if (*w.abort) return false;
+      if (global_timer_ns() - t0 > kLimitNs) {
+        *w.abort = 1;
+        if (w.status) atomicCAS(w.status, 0, code);
+        if (w.host_status) {
+          *w.host_status = code;
+          __threadfence_system();
+        }
+        return false;
+      }
+    }
+  }
+}
+
+// kind::f16 products: D[tmem] (+)= A B, fp16 operands, fp32 sums.
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+               ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+               ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Shared-memory matrix descriptors, 128-byte swizzle: low word (address, leading offset) and high word (stride offset 1024 bytes
+// between groups of eight rows, version 1, swizzle mode 2), all in units of 16 bytes.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t leading) { return ((addr & 0x3ffffu) >> 4) | ((leading >> 4) << 16); }
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint64_t desc(uint32_t lo) { return (static_cast<uint64_t>(kDescHi) << 32) | lo; }
+// Instruction descriptor: fp16 x fp16 -> fp32; bit 16: B with its columns (head dim) contiguous.
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTileM >> 4) << 24);
+}
+
+__device__ __forceinline__ void st_shared16(uint32_t addr, const uint4& v) { st_shared_v4(addr, v.x, v.y, v.z, v.w); }
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Sixteen fp8 -> fp16, times a pair of factors.
+template <bool kE5M2>
+__device__ __forceinline__ void widen16(const uint4& x, uint32_t f, uint4& lo, uint4& hi) {
+  uint32_t r[8];
+  fp8_to_half4<kE5M2>(x.x, r[0], r[1]);
+  fp8_to_half4<kE5M2>(x.y, r[2], r[3]);
+  fp8_to_half4<kE5M2>(x.z, r[4], r[5]);
+  fp8_to_half4<kE5M2>(x.w, r[6], r[7]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = hmul2(r[i], f);
+  lo = make_uint4(r[0], r[1], r[2], r[3]);
+  hi = make_uint4(r[4], r[5], r[6], r[7]);
+}
+
+// What the softmax of a row carries from block to block.
+struct Row {
+  float c;                               // scale_log2 * reference scale of K * what Q was scaled by
+  float m, nm, l;                        // reference (log2 units), its negative (0 while there is none), row sum
+  float most;                            // sum of P over a half above which the reference is raised: 0 while there is none
+  int lim;                               // keys that the row sees
+};
+
+// P of 64 keys (tensor-memory columns t_s ... t_s + 63) into pk, fp16 pairs; returns the sum of P and adds that of the
+// denominators to *l.  General: keys from `lim` on (counted from the first of these) are masked, residual scales are multiplied in.
+template <bool kGeneral>
+__device__ __forceinline__ float exponentials(uint32_t t_s, float c, float nm, int lim, const float* rk, const float* rv, uint32_t (&pk)[32],
+                                              float* l) {
+  f32x2_t sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+  float sum_p = 0.f, sum_l = 0.f;
+  const f32x2_t c2 = pack2(c, c), nm2 = pack2(nm, nm);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    uint32_t s[32];
+    tmem_ld_32x32b_x32(t_s + 32 * q, s);
+    tmem_wait_ld();
+    if (kGeneral) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        const int grp = (32 * q + i) >> 4;
+        const float k = rk[grp], v = rv[grp], ck = c * k;
+        float x0 = fmaf(__uint_as_float(s[i]), ck, nm), x1 = fmaf(__uint_as_float(s[i + 1]), ck, nm);
+        if (32 * q + i >= lim || k == -1.f) x0 = -INFINITY;
+        if (32 * q + i + 1 >= lim || k == -1.f) x1 = -INFINITY;
+        const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
+        sum_l += e0 + e1;
+        const float p0 = e0 * v, p1 = e1 * v;
+        sum_p += p0 + p1;
+        pk[16 * q + i / 2] = pack_half2(p0, p1);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        float x0, x1;
+        unpack2(fma2(pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, nm2), x0, x1);
+        const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
+        sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pack2(e0, e1));
+        pk[16 * q + i / 2] = pack_half2(e0, e1);
+      }
+    }
+  }
+  if (kGeneral) {
+    *l += sum_l;
+    return sum_p;
+  }
+  float a, b;
+  unpack2(add2(sum[0], sum[1]), a, b);
+  *l += a + b;
+  return a + b;
+}
+
+// Largest c s + log2(scale of V) over 64 keys.
+__device__ __noinline__ float half_max(uint32_t t_s, float c, int lim, const float* rk, const float* rv) {
+  float m = -INFINITY;
+#pragma unroll 1
+  for (int q = 0; q < 2; ++q) {
+    uint32_t s[32];
+    tmem_ld_32x32b_x32(t_s + 32 * q, s);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int grp = (32 * q + i) >> 4;
+      const float k = rk[grp];
+      const float x = fmaf(__uint_as_float(s[i]), c * k, fmaxf(__log2f(rv[grp]), kLog2Least));
+      if (32 * q + i < lim && k != -1.f) m = fmaxf(m, x);
+    }
+  }
+  return m;
+}
+
+template <int W, bool kE5M2>
+__global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                                                                          const KvAttendArgs a, const KvPrefillPlan plan) {
+  using C = PCfg<W>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const gen = smem_raw + (base - smem_u32(smem_raw));
+  Shared<W>& sh = *reinterpret_cast<Shared<W>*>(gen + C::kSharedOffset);
+  const uint32_t s_q = base, s_raw = base + C::kRawOffset, s_ring = base + C::kRingOffset;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Wait wctx{&sh.abort, a.c.status, a.c.host_status};
+  if (threadIdx.x == 0) {
+    auto init = [](uint64_t* b, int n, int count) {
+      for (int i = 0; i < n; ++i) mbar_init(smem_u32(b + i), count);
+    };
+    init(sh.item_full, kItemSlots, 1);
+    init(sh.item_empty, kItemSlots, C::kSoftWarps + 4 + 1);
+    init(sh.raw_full, C::kRaw, 1);
+    init(sh.raw_empty, C::kRaw, 4);
+    init(sh.ring_full, C::kRing, 4);
+    init(sh.ring_empty, C::kRing, 1);
+    init(sh.q_full, 2, 4);
+    init(sh.s_full, 2, 1);
+    init(&sh.p_full[0][0], 4, 4);
+    init(sh.o_half, 2, 1);
+    init(sh.o_final, 2, 1);
+    init(sh.blk_full, kBlockSlots, 1);
+    init(&sh.drain, 1, 1);
+    sh.abort = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == C::kLoadWarp && lane == 0) {
+    prefetch_tensormap(&tk);
+    prefetch_tensormap(&tv);
+  }
+  if (warp == C::kMmaWarp) {
+    tmem_alloc(smem_u32(&sh.tmem), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  start_after_predecessor();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
+
+  const int group = a.group, tile_tokens = kTileM / group;       // a token's rows lie in one tile
+  // Consumers of the item ring: the next item (false: no more, or a wait ran out).
+  int n_items = 0;
+  auto next_item = [&](Item& it) {
+    const int slot = n_items % kItemSlots;
+    if (!wait_bounded(wctx, &sh.item_full[slot], (n_items / kItemSlots) & 1, 0xb100)) return false;
+    it = sh.item[slot];
+    return true;
+  };
+  auto item_read = [&] { mbar_arrive(smem_u32(&sh.item_empty[n_items++ % kItemSlots])); };
+
+  if (warp == C::kLoadWarp) {
+    // ---------------------------------------------------------------- producer
+    bool ok = true;
+    uint32_t tiles = 0, blocks = 0;                              // raw tiles and blocks filled so far
+    if (blockIdx.x == 0)                                         // a bad range has no rows that would find it
+      for (int b = lane; b < a.c.batch; b += 32)
+        if (kv_seq(a.c, b).bad) report_bad_index(a.c);
+    auto push = [&](const Item& it) {
+      const int slot = n_items % kItemSlots;
+      ok = wait_bounded(wctx, &sh.item_empty[slot], ((n_items / kItemSlots) & 1) ^ 1, 0xb200);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      if (lane == 0) {
+        sh.item[slot] = it;
+        mbar_arrive(smem_u32(&sh.item_full[slot]));
+      }
+      ++n_items;
+    };
+    for (int64_t round = 0; ok; ++round) {
+      // a round deals one item to each CTA, every other one in the opposite order: the heavier ones come first
+      const int64_t at = (round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+      if (round * gridDim.x >= plan.items) break;
+      const int64_t id = round * gridDim.x + at;
+      if (id >= plan.items) continue;
+      Item it;
+      const int64_t sh_id = id / plan.parts;
+      it.part = static_cast<int>(id - sh_id * plan.parts);
+      const int64_t slot = sh_id / a.c.heads;
+      it.head = static_cast<int>(sh_id - slot * a.c.heads);
+      int j;
+      kv_find_slot(a.c, slot, plan.block_tokens, 1, &it.seq, &j);
+      const KvSeq s = kv_seq(a.c, it.seq);
+      const int tiles_of = (s.n + plan.block_tokens - 1) / plan.block_tokens;
+      if (j >= tiles_of) continue;
+      it.first = s.first;
+      it.n = s.n;
+      it.len = s.len;
+      it.token0 = (tiles_of - 1 - j) * plan.block_tokens;
+      it.n_tokens = min(plan.block_tokens, s.n - it.token0);
+      it.vis = a.causal ? max(0, min(s.len, s.len - s.n + it.token0 + it.n_tokens)) : s.len;
+      const int n_blk = max(1, (it.vis + C::kN - 1) / C::kN);
+      it.blk0 = static_cast<int>(static_cast<int64_t>(n_blk) * it.part / plan.parts);
+      it.blk1 = static_cast<int>(static_cast<int64_t>(n_blk) * (it.part + 1) / plan.parts);
+      if (it.blk0 == it.blk1) continue;
+      push(it);
+      if (!ok) break;
+
+      // Lane g < kGroups looks after the g-th sixteen keys of a block: page numbers are loaded two blocks ahead, scales one.
+      const int* const table = a.c.table + static_cast<int64_t>(it.seq) * a.c.table_stride;
+      auto load_page = [&](int blk) {
+        const int64_t key = static_cast<int64_t>(blk) * C::kN + 16 * lane;
+        return lane < C::kGroups && blk < it.blk1 && key < it.vis ? ld_int(table + (key >> a.c.page_shift)) : -2;
+      };
+      auto in_pool = [&](int page) { return static_cast<unsigned>(page) < static_cast<unsigned>(a.c.num_pages); };
+      auto load_scale = [&](const float* d, int page) { return in_pool(page) ? ld_global(d + static_cast<int64_t>(page) * a.c.heads + it.head) : 1.f; };
+      int page = load_page(it.blk0), page1 = load_page(it.blk0 + 1);
+      float kd = load_scale(a.c.k_descale, page), vd = load_scale(a.c.v_descale, page);
+      // the item's reference scales: its first page's, so that e5m2 (up to 2^15.8) keeps away from fp16's ends
+      const float margin = kE5M2 ? 16.f : 1.f;
+      auto reference = [&](float d) {
+        d = __shfl_sync(0xffffffffu, d, 0);
+        return (d >= 0x1p-100f && d <= 0x1p100f ? d : 1.f) * margin;
+      };
+      const float kref = reference(kd), vref = reference(vd);
+      for (int blk = it.blk0; blk < it.blk1 && ok; ++blk) {
+        const int page2 = load_page(blk + 2);
+        const float kd1 = load_scale(a.c.k_descale, page1), vd1 = load_scale(a.c.v_descale, page1);
+        const bool here = in_pool(page);
+        if (!here && page != -2) report_bad_index(a.c);
+        // factor 2^e that fp16 takes in exactly: e4m3 2^-15 ... 2^7, e5m2 2^-8 ... 1; the rest is residual
+        auto split = [&](float d, float ref, float* rest) {
+          const float f = d / ref;
+          const uint32_t bits = __float_as_uint(f);
+          const int e = static_cast<int>(bits >> 23) - 127;
+          const bool exact = (bits & 0x7fffffu) == 0 && e >= (kE5M2 ? -8 : -15) && e <= (kE5M2 ? 0 : 7);
+          const float take = exact ? f : (kE5M2 ? 0x1p-4f : 1.f);
+          *rest = exact ? 1.f : d / ref / take;
+          const uint32_t h = pack_half2(take, take);
+          return h;
+        };
+        const uint32_t n = blocks % kBlockSlots;
+        float rk = 1.f, rv = 1.f;
+        const uint32_t fk = split(kd, kref, &rk), fv = split(vd, vref, &rv);
+        if (!here) {
+          rv = 1.f;
+          rk = page == -2 ? 1.f : -1.f;                          // past the last key: masked by the row's limit
+        }
+        if (lane < C::kGroups) {
+          sh.residual[n][0][lane] = rk;
+          sh.residual[n][1][lane] = rv;
+        }
+        const bool flagged = __any_sync(0xffffffffu, lane < C::kGroups && (rk != 1.f || rv != 1.f));
+        if (lane == 0) {
+          sh.ref[n][0] = kref;
+          sh.ref[n][1] = vref;
+          sh.flagged[n] = flagged;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.blk_full[n]));
+        ++blocks;
+        // one copy per page part of the block (box_rows keys) and 128 columns
+        const int box_rows = min(1 << a.c.page_shift, 32);
+        const bool issues = here && (16 * lane) % box_rows == 0;
+        const int boxes = __popc(__ballot_sync(0xffffffffu, issues));
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const int st = tiles % C::kRaw;
+          ok = __all_sync(0xffffffffu, wait_bounded(wctx, &sh.raw_empty[st], ((tiles / C::kRaw) & 1) ^ 1, 0xb300 + st));
+          if (!ok) break;
+          if (lane < C::kGroups) sh.factor[st][lane] = here ? (kv ? fv : fk) : 0u;
+          if (lane == 0) sh.valid[st] = max(0, min(C::kN, it.vis - blk * C::kN));
+          __syncwarp();
+          const uint32_t bar = smem_u32(&sh.raw_full[st]);
+          if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_rows * C::kRawRow * C::kRawBlocks);
+          __syncwarp();
+          if (issues) {
+            const int row = (blk * C::kN + 16 * lane) & ((1 << a.c.page_shift) - 1);
+#pragma unroll
+            for (int b = 0; b < C::kRawBlocks; ++b)
+              tma_load_3d(s_raw + st * C::kRawBytes + b * C::kRawBlockBytes + 16 * lane * C::kRawRow, kv ? &tv : &tk, bar, 128 * b, row,
+                          page * a.c.heads + it.head);
+          }
+          ++tiles;
+        }
+        page = page1;
+        page1 = page2;
+        kd = kd1;
+        vd = vd1;
+      }
+    }
+    if (ok) {
+      Item none{};
+      none.seq = -1;
+      push(none);
+    }
+    if (!ok) {
+      // copies in flight land before the CTA's memory is given back (a wait each, with a limit)
+      for (uint32_t i = tiles > C::kRaw ? tiles - C::kRaw : 0; i < tiles; ++i) {
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(smem_u32(&sh.raw_full[i % C::kRaw]), (i / C::kRaw) & 1) && global_timer_ns() - t0 < 20000000ull) {}
+      }
+    }
+  } else if (warp == C::kMmaWarp) {
+    // ---------------------------------------------------------------- issuer
+    if (elect_one()) {
+      constexpr uint32_t kIdescQK = idesc(C::kN, false), kIdescPV = idesc(W, true);
+      constexpr uint32_t kColQ = kTileM * 128 / 16, kColK = C::kN * 128 / 16;     // column blocks of Q and K in 16 bytes
+      const uint32_t q_lo = desc_lo(s_q, 16), k_lo = desc_lo(s_ring, 16), v_lo = desc_lo(s_ring, C::kN * 128);
+      bool ok = true;
+      uint32_t ld = 0;                                           // widened tiles used so far: K, V, K, V ...
+      uint32_t qn[2] = {0, 0};                                   // q_full phases by tile
+      uint32_t pn[2] = {0, 0};                                   // p_full phases by tile (or score buffer)
+      auto ring_wait = [&](uint32_t i) { return wait_bounded(wctx, &sh.ring_full[i % C::kRing], (i / C::kRing) & 1, 0xb400); };
+      auto ring_release = [&](uint32_t i) { tc_commit(smem_u32(&sh.ring_empty[i % C::kRing])); };
+      auto issue_qk = [&](int tile, uint32_t col, uint32_t i) {
+        const uint32_t kk = k_lo + (i % C::kRing) * (C::kRingBytes / 16), qq = q_lo + tile * (C::kQBytes / 16);
+#pragma unroll
+        for (int k = 0; k < W / 16; ++k)
+          mma_f16_ss(tmem + col, desc(qq + (k >> 2) * kColQ + 2 * (k & 3)), desc(kk + (k >> 2) * kColK + 2 * (k & 3)), kIdescQK, k > 0);
+      };
+      auto issue_pv = [&](int tile, uint32_t col, uint32_t i, int half, bool first) {
+        const uint32_t vv = v_lo + (i % C::kRing) * (C::kRingBytes / 16);
+#pragma unroll
+        for (int k = 4 * half; k < 4 * half + 4; ++k)
+          mma_f16_ts(tmem + C::kOCol + tile * W, tmem + col + 8 * k, desc(vv + k * 128), kIdescPV, !(first && k == 0));
+      };
+      Item it;
+      while (ok && (ok = next_item(it))) {
+        item_read();
+        if (it.seq < 0) break;
+        const int nb = it.blk1 - it.blk0;
+        const int nt = C::kTiles == 2 && it.n_tokens > tile_tokens ? 2 : 1;
+        if constexpr (C::kTiles == 2) {
+          ok = ring_wait(ld);
+          for (int i = 0; i < nt && ok; ++i) {
+            ok = wait_bounded(wctx, &sh.q_full[i], qn[i]++ & 1, 0xb500 + i);
+            if (!ok) break;
+            tc_fence_after();
+            issue_qk(i, 128 * i, ld);
+            tc_commit(smem_u32(&sh.s_full[i]));
+          }
+          if (!ok) break;
+          ring_release(ld);
+          for (int j = 0; j < nb && ok; ++j) {
+            const uint32_t lv = ld + 2 * j + 1, lk = lv + 1;
+            const bool more = j + 1 < nb;
+            ok = ring_wait(lv);
+            for (int i = 0; i < nt && ok; ++i) {
+#pragma unroll
+              for (int half = 0; half < C::kHalves; ++half) {
+                if (ok) ok = wait_bounded(wctx, &sh.p_full[i][half], pn[i] & 1, 0xb600 + 2 * i + half);
+                if (!ok) break;
+                tc_fence_after();
+                issue_pv(i, 128 * i, lv, half, j == 0);
+                if (half == 0) tc_commit(smem_u32(&sh.o_half[i]));
+              }
+              if (!ok) break;
+              ++pn[i];
+              if (!more) tc_commit(smem_u32(&sh.o_final[i]));
+              if (more) {
+                if (i == 0) ok = ring_wait(lk);
+                if (!ok) break;
+                tc_fence_after();
+                issue_qk(i, 128 * i, lk);
+                tc_commit(smem_u32(&sh.s_full[i]));
+              }
+            }
+            if (!ok) break;
+            ring_release(lv);
+            if (more) ring_release(lk);
+          }
+        } else {
+          // one tile, score buffers in turn: S(j + 2) follows P V (j) into the buffer that it read
+          ok = wait_bounded(wctx, &sh.q_full[0], qn[0]++ & 1, 0xb500);
+          for (int j = 0; j < 2 && j < nb && ok; ++j) {
+            ok = ring_wait(ld + 2 * j);
+            if (!ok) break;
+            tc_fence_after();
+            issue_qk(0, 64 * ((pn[0] + j) & 1), ld + 2 * j);
+            tc_commit(smem_u32(&sh.s_full[(pn[0] + j) & 1]));
+            ring_release(ld + 2 * j);
+          }
+          for (int j = 0; j < nb && ok; ++j) {
+            const uint32_t lv = ld + 2 * j + 1, b = pn[0] & 1;
+            ok = ring_wait(lv);
+            if (ok) ok = wait_bounded(wctx, &sh.p_full[b][0], (pn[0] >> 1) & 1, 0xb600 + b);
+            if (!ok) break;
+            ++pn[0];
+            tc_fence_after();
+            issue_pv(0, 64 * b, lv, 0, j == 0);
+            tc_commit(smem_u32(&sh.o_half[0]));
+            if (j + 1 == nb) tc_commit(smem_u32(&sh.o_final[0]));
+            ring_release(lv);
+            if (j + 2 < nb) {
+              ok = ring_wait(ld + 2 * j + 4);
+              if (!ok) break;
+              tc_fence_after();
+              issue_qk(0, 64 * b, ld + 2 * j + 4);
+              tc_commit(smem_u32(&sh.s_full[b]));
+              ring_release(ld + 2 * j + 4);
+            }
+          }
+        }
+        ld += 2 * nb;
+      }
+      {
+        // products in flight, and their arrivals, end before tensor and shared memory are freed (with a limit)
+        tc_commit(smem_u32(&sh.drain));
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(smem_u32(&sh.drain), 0) && global_timer_ns() - t0 < 20000000ull) {}
+      }
+    }
+    __syncwarp();
+  } else if (warp >= C::kWideWarp0) {
+    // ---------------------------------------------------------------- widening
+    const int w = warp - C::kWideWarp0;
+    uint32_t tiles = 0;
+    Item it;
+    bool ok = true;
+    while (ok && (ok = next_item(it))) {
+      __syncwarp();
+      if (lane == 0) item_read();
+      else ++n_items;
+      if (it.seq < 0) break;
+      const int n_tiles = 2 * (it.blk1 - it.blk0);
+      for (int i = 0; i < n_tiles && ok; ++i, ++tiles) {
+        const uint32_t st = tiles % C::kRaw, rg = tiles % C::kRing;
+        ok = wait_bounded(wctx, &sh.raw_full[st], (tiles / C::kRaw) & 1, 0xb700 + st);
+        if (ok) ok = wait_bounded(wctx, &sh.ring_empty[rg], ((tiles / C::kRing) & 1) ^ 1, 0xb800 + rg);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int valid = sh.valid[st];
+        const uint32_t src = s_raw + st * C::kRawBytes, dst = s_ring + rg * C::kRingBytes;
+        // a warp takes eight rows and 64 columns at a time: eight lanes side by side read and write eight rows of one
+        // 16-byte column, which the swizzles spread over all banks
+        constexpr int kParts = (C::kN / 8) * C::kCols;
+#pragma unroll 4
+        for (int p = w; p < kParts; p += 4) {
+          const int cb = p % C::kCols, r = (p / C::kCols) * 8 + (lane & 7), q = lane >> 3;
+          uint32_t from;
+          if constexpr (W == 64) from = src + r * 64 + ((q ^ ((r >> 1) & 3)) << 4);
+          else from = src + (cb >> 1) * C::kRawBlockBytes + r * 128 + (((4 * (cb & 1) + q) ^ (r & 7)) << 4);
+          uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+          const uint32_t f = sh.factor[st][r >> 4];
+          if (r < valid && f != 0u) widen16<kE5M2>(ld_shared16(from), f, lo, hi);
+          const uint32_t to = dst + cb * (C::kN * 128) + r * 128;
+          st_shared16(to + (((2 * q) ^ (r & 7)) << 4), lo);
+          st_shared16(to + (((2 * q + 1) ^ (r & 7)) << 4), hi);
+        }
+        fence_proxy_async_smem();                                // what was written is for the products to read
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&sh.ring_full[rg]));
+          mbar_arrive(smem_u32(&sh.raw_empty[st]));
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const int tile = warp / 4, sub = warp % 4;                   // rows 32 sub ... of the tile = lanes of tensor memory
+    const uint32_t lanes = static_cast<uint32_t>(32 * sub) << 16;
+    const uint32_t t_o = tmem + lanes + C::kOCol + tile * W;
+    uint32_t blocks = 0;                                         // of all items (the residual ring), also those this tile sits out
+    uint32_t mine = 0;                                           // blocks this tile took part in
+    uint32_t taken = 0;                                          // items this tile took part in
+    Item it;
+    bool ok = true;
+    while (ok && (ok = next_item(it))) {
+      __syncwarp();
+      if (lane == 0) item_read();
+      else ++n_items;
+      if (it.seq < 0) break;
+      const int nb = it.blk1 - it.blk0;
+      const int tok0 = it.token0 + tile * tile_tokens;
+      const int n_rows = min(tile_tokens, it.n_tokens - tile * tile_tokens) * group;
+      if (n_rows <= 0) {
+        blocks += nb;
+        continue;
+      }
+      const int D = a.c.head_dim;
+      // ---- Q: this warp's 32 rows into shared memory, fp16 ----
+      float back = 1.f;
+      {
+        constexpr int kLanes = W / 8, kRowsAt = 32 / kLanes;     // lanes of a row (8 columns each), rows at a time
+        const int col = 8 * (lane % kLanes);
+#pragma unroll 4
+        for (int r0 = 0; r0 < 32; r0 += kRowsAt) {
+          const int r = 32 * sub + r0 + lane / kLanes;
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (r < n_rows && col < D) {
+            const int64_t token = it.first + tok0 + r / group;
+            const int head = it.head * group + r % group;
+            x = ld_global(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q.x) + token * a.q.token_stride + head * a.q.head_stride + col));
+          }
+          if (a.bf16) {
+            float big = 0.f;
+            uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = half_pair<true>(v[e] & 0x7fff7fffu);
+              big = fmaxf(big, fmaxf(f.x, f.y));
+            }
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
+            const float f = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
+            const float g = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 y = half_pair<true>(v[k]);
+              v[k] = pack_half2(y.x * f, y.y * f);
+            }
+            x = make_uint4(v[0], v[1], v[2], v[3]);
+#pragma unroll
+            for (int k = 0; k < kRowsAt; ++k) {
+              const float y = __shfl_sync(0xffffffffu, g, k * kLanes);
+              if (lane == r0 + k) back = y;
+            }
+          }
+          const int c = lane % kLanes;
+          st_shared16(s_q + tile * C::kQBytes + (c >> 3) * (kTileM * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), x);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[tile]));
+
+      const int r = 32 * sub + lane;
+      Row row{};
+      row.m = -INFINITY;
+      const int my_token = tok0 + min(r, n_rows - 1) / group;
+      row.lim = a.causal ? max(0, min(it.len, it.len - it.n + my_token + 1)) : it.len;
+      const int least = a.causal ? max(0, min(it.len, it.len - it.n + tok0 + 1)) : it.len;       // of the tile's first row
+      float vref = 1.f;
+      for (int j = 0; j < nb && ok; ++j, ++blocks, ++mine) {
+        const uint32_t n = blocks % kBlockSlots;
+        const int buf = C::kTiles == 2 ? tile : static_cast<int>(mine & 1);
+        const uint32_t t_s = tmem + lanes + (C::kTiles == 2 ? 128 * tile : 64 * buf);
+        ok = wait_bounded(wctx, &sh.blk_full[n], (blocks / kBlockSlots) & 1, 0xb900);
+        if (ok) ok = wait_bounded(wctx, &sh.s_full[buf], (C::kTiles == 2 ? mine : mine >> 1) & 1, 0xba00 + buf);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (j == 0) {
+          row.c = a.scale_log2 * back * sh.ref[n][0];
+          vref = sh.ref[n][1];
+        }
+        const int key0 = (it.blk0 + j) * C::kN;
+        const bool general = sh.flagged[n] != 0 || key0 + C::kN > least;
+        if (j == 0) {
+          // the exact maximum of the first block
+          float m = -INFINITY;
+          for (int half = 0; half < C::kHalves; ++half)
+            m = fmaxf(m, half_max(t_s + 64 * half, row.c, row.lim - key0 - 64 * half, &sh.residual[n][0][4 * half], &sh.residual[n][1][4 * half]));
+          row.m = m - kHeadroom;
+          row.nm = m == -INFINITY ? 0.f : -row.m;
+          row.most = m == -INFINITY ? 0.f : kRaiseAbove;
+        }
+#pragma unroll
+        for (int half = 0; half < C::kHalves; ++half) {
+          uint32_t pk[32];
+          const float* rk = &sh.residual[n][0][4 * half];
+          const float* rv = &sh.residual[n][1][4 * half];
+          const int lim = row.lim - key0 - 64 * half;
+          const uint32_t ts = t_s + 64 * half;
+          float l = 0.f;
+          float sum = general ? exponentials<true>(ts, row.c, row.nm, lim, rk, rv, pk, &l) : exponentials<false>(ts, row.c, row.nm, 0, rk, rv, pk, &l);
+          if (__any_sync(0xffffffffu, !(sum <= row.most))) {
+            // Some row has outgrown its reference (or holds a NaN): take this half's maximum in, and rescale O, for which the
+            // products before have to be done: those before this block's scores are, where the scores came after them.
+            const float top = half_max(ts, row.c, lim, rk, rv);
+            const float m = sum <= row.most ? row.m : fmaxf(row.m, top - kHeadroom);
+            const float nm = m == -INFINITY ? 0.f : -m;
+            const float alpha = row.m == -INFINITY ? 0.f : ex2_approx(nm - row.nm);
+            row.m = m;
+            row.nm = nm;
+            row.most = m == -INFINITY ? 0.f : kRaiseAbove;
+            row.l *= alpha;
+            const bool summed = C::kTiles == 2 ? (j > 0 || half > 0) : j > 0;
+            if (summed) {
+              if (C::kTiles == 2 && half > 0) ok = wait_bounded(wctx, &sh.o_half[tile], mine & 1, 0xbb00);
+              if (C::kTiles == 1) ok = wait_bounded(wctx, &sh.o_half[0], (mine - 1) & 1, 0xbb00);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < W; c += 32) {
+                uint32_t o[32];
+                tmem_ld_32x32b_x32(t_o + c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st_32x32b_x32(t_o + c, o);
+              }
+              tmem_wait_st();
+            }
+            l = 0.f;
+            exponentials<true>(ts, row.c, row.nm, lim, rk, rv, pk, &l);
+          }
+          row.l += l;
+          tmem_st_32x32b_x32(t_s + 32 * half, pk);               // over the scores, two to a column
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[buf][half]));
+        }
+      }
+      if (!ok) break;
+
+      // ---- O ----
+      ok = __all_sync(0xffffffffu, wait_bounded(wctx, &sh.o_final[tile], taken & 1, 0xbc00 + tile));
+      if (!ok) break;
+      ++taken;
+      tc_fence_after();
+      const bool whole = plan.parts == 1;
+      const float inv = (row.l == 0.f ? 0.f : (whole ? 1.f / row.l : 1.f)) * vref;
+      const int64_t out_row = (static_cast<int64_t>(it.first) + tok0 + r / group) * a.heads_q + it.head * group + r % group;
+      if (r < n_rows) {
+        if (whole) {
+          if (a.lse != nullptr) a.lse[out_row] = row.l == 0.f ? -INFINITY : (row.m + __log2f(row.l)) * 0.6931471805599453f;
+        } else {
+          float* const ml = plan.partial_ml + 2 * (static_cast<int64_t>(it.part) * a.c.tokens * a.heads_q + out_row);
+          ml[0] = row.m;
+          ml[1] = row.l;
+        }
+      }
+      float* const po = whole ? nullptr : plan.partial_o + (static_cast<int64_t>(it.part) * a.c.tokens * a.heads_q + out_row) * D;
+      // through this warp's rows of Q's shared memory, which the last scores have been made from: 16 bytes a lane side by side
+      const uint32_t stage = s_q + tile * C::kQBytes;
+#pragma unroll 1
+      for (int c = 0; c < W; c += 32) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(t_o + c, o);
+        tmem_wait_ld();
+        if (c >= D) continue;
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float x = __uint_as_float(o[i + 2 * k]) * inv, y = __uint_as_float(o[i + 2 * k + 1]) * inv;
+              v[k] = a.bf16 ? pack_pair<true>(x, y) : pack_pair<false>(x, y);
+            }
+            const int ch = (c + i) >> 3;
+            st_shared_v4(stage + (ch >> 3) * (kTileM * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), v[0], v[1], v[2], v[3]);
+          }
+        } else if (r < n_rows) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float4 v;
+            v.x = __uint_as_float(o[i]) * inv; v.y = __uint_as_float(o[i + 1]) * inv;
+            v.z = __uint_as_float(o[i + 2]) * inv; v.w = __uint_as_float(o[i + 3]) * inv;
+            *reinterpret_cast<float4*>(po + c + i) = v;
+          }
+        }
+      }
+      tc_fence_before();
+      if (whole) {
+        __syncwarp();
+        constexpr int kLanes = W / 8, kRowsAt = 32 / kLanes;
+        const int ch = lane % kLanes;
+#pragma unroll 4
+        for (int r0 = 0; r0 < 32; r0 += kRowsAt) {
+          const int q = 32 * sub + r0 + lane / kLanes;
+          if (q < n_rows && 8 * ch < D) {
+            const uint4 v = ld_shared16(stage + (ch >> 3) * (kTileM * 128) + q * 128 + (((ch & 7) ^ (q & 7)) << 4));
+            const int64_t orow = (static_cast<int64_t>(it.first) + tok0 + q / group) * a.heads_q + it.head * group + q % group;
+            st_global_v4(static_cast<uint16_t*>(a.o) + orow * D + 8 * ch, v.x, v.y, v.z, v.w);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+  let_successor_start();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == C::kMmaWarp) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Rows whose keys were cut into parts: a warp to a row.
+__global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a, const KvPrefillPlan plan, int block_keys) {
+  start_after_predecessor();
+  let_successor_start();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int token = static_cast<int>(row / a.heads_q);
+  if (token >= a.c.tokens) return;
+  int b, unused;
+  if (a.c.cu == nullptr) b = token / a.c.even;
+  else kv_find_slot(a.c, token, 1, 0, &b, &unused);
+  const KvSeq s = kv_seq(a.c, b);
+  if (token < s.first || token >= s.first + s.n) return;
+  const int token0 = (token - s.first) / plan.block_tokens * plan.block_tokens;
+  const int n_tokens = min(plan.block_tokens, s.n - token0);
+  const int vis = a.causal ? max(0, min(s.len, s.len - s.n + token0 + n_tokens)) : s.len;
+  const int64_t n_blk = max(1, (vis + block_keys - 1) / block_keys);
+  const int D = a.c.head_dim, quads = D >> 2;
+  const int64_t rows = static_cast<int64_t>(a.c.tokens) * a.heads_q;
+  auto empty = [&](int p) { return n_blk * p / plan.parts == n_blk * (p + 1) / plan.parts; };
+  float m = -INFINITY;
+  for (int p = 0; p < plan.parts; ++p)
+    if (!empty(p)) m = fmaxf(m, ld_global(plan.partial_ml + 2 * (p * rows + row)));
+  float l = 0.f;
+  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 4
+  for (int p = 0; p < plan.parts; ++p) {
+    if (empty(p)) continue;
+    const float* ml = plan.partial_ml + 2 * (p * rows + row);
+    const float mp = ld_global(ml);
+    const float f = mp == -INFINITY ? 0.f : ex2_approx(mp - m);
+    l += ld_global(ml + 1) * f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int q = lane + 32 * i;
+      if (q < quads) {
+        const uint4 u = ld_global(reinterpret_cast<const uint4*>(plan.partial_o + (p * rows + row) * D) + q);
+        acc[i].x += __uint_as_float(u.x) * f; acc[i].y += __uint_as_float(u.y) * f;
+        acc[i].z += __uint_as_float(u.z) * f; acc[i].w += __uint_as_float(u.w) * f;
+      }
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint2* const out = reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + row * D);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int q = lane + 32 * i;
+    if (q >= quads) continue;
+    const float4 v = acc[i];
+    out[q] = a.bf16 ? make_uint2(pack_pair<true>(v.x * inv, v.y * inv), pack_pair<true>(v.z * inv, v.w * inv))
+                    : make_uint2(pack_pair<false>(v.x * inv, v.y * inv), pack_pair<false>(v.z * inv, v.w * inv));
+  }
+  if (a.lse != nullptr && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+}
+
+int width_of(int head_dim) { return head_dim <= 64 ? 64 : (head_dim <= 128 ? 128 : 256); }
+
+template <int W, bool kE5M2>
+cudaError_t launch_one(const CUtensorMap& tk, const CUtensorMap& tv, const KvAttendArgs& a, const KvPrefillPlan& plan, int sms, cudaStream_t stream) {
+  using C = PCfg<W>;
+  auto kernel = &kv_prefill_kernel<W, kE5M2>;
+  constexpr int smem = C::kSharedOffset + static_cast<int>(sizeof(Shared<W>)) + 1024;
+  static_assert(smem <= 227 * 1024, "shared memory");
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const bool cached = dev >= 0 && dev < 64;
+  if (!cached || !ready[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (cached) ready[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(plan.items < sms ? plan.items : sms), 1, 1);
+  cfg.blockDim = dim3(C::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {overlap_attribute()};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, tk, tv, a, plan);
+  if (e != cudaSuccess || plan.parts == 1) return e;
+  const int64_t ctas = (static_cast<int64_t>(a.c.tokens) * a.heads_q + 7) / 8;
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, &kv_join_kernel, a, plan, C::kN);
+}
+
+}  // namespace
+
+bool kv_prefill_takes(const KvAttendSizes& z) {
+  const int64_t group = z.heads_q / z.heads;
+  return group <= kTileM && static_cast<int64_t>(z.tokens) * group > 64ll * z.batch;
+}
+
+KvPrefillPlan kv_prefill_plan(const KvAttendSizes& z, int sms) {
+  KvPrefillPlan p{};
+  const int width = width_of(z.head_dim), tiles = width == 256 ? 1 : 2;
+  p.block_tokens = kTileM / (z.heads_q / z.heads) * tiles;
+  p.items = kv_slots(z.batch, z.tokens, z.tokens / z.batch, z.ragged, p.block_tokens, 1) * z.heads;
+  p.parts = 1;
+  // Few items: their keys are cut into as many parts as fill the GPU once.
+  const int64_t blocks = (z.keys_most + PCfg<128>::kN - 1) / PCfg<128>::kN;
+  int64_t parts = sms / (p.items > 0 ? p.items : 1);
+  if (parts > 16) parts = 16;
+  if (parts > blocks / 4) parts = blocks / 4;
+  if (parts > 1) p.parts = static_cast<int>(parts);
+  p.items *= p.parts;
+  return p;
+}
+
+int64_t kv_prefill_workspace(const KvAttendSizes& z, int sms) {
+  const KvPrefillPlan p = kv_prefill_plan(z, sms);
+  return p.parts == 1 ? 0 : static_cast<int64_t>(p.parts) * z.tokens * z.heads_q * (z.head_dim + 2) * 4;
+}
+
+cudaError_t launch_kv_prefill(const CUtensorMap& tk, const CUtensorMap& tv, const KvAttendArgs& a, const KvAttendSizes& z, void* workspace,
+                              bool e5m2, int sms, cudaStream_t stream) {
+  KvPrefillPlan p = kv_prefill_plan(z, sms);
+  if (p.parts > 1) {
+    p.partial_o = static_cast<float*>(workspace);
+    p.partial_ml = p.partial_o + static_cast<int64_t>(p.parts) * z.tokens * z.heads_q * z.head_dim;
+  }
+  switch (width_of(a.c.head_dim)) {
+    case 64: return e5m2 ? launch_one<64, true>(tk, tv, a, p, sms, stream) : launch_one<64, false>(tk, tv, a, p, sms, stream);
+    case 128: return e5m2 ? launch_one<128, true>(tk, tv, a, p, sms, stream) : launch_one<128, false>(tk, tv, a, p, sms, stream);
+    default: return e5m2 ? launch_one<256, true>(tk, tv, a, p, sms, stream) : launch_one<256, false>(tk, tv, a, p, sms, stream);
+  }
+}
+
+}  // namespace fa8

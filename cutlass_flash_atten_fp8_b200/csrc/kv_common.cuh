@@ -50,22 +50,19 @@ __device__ __forceinline__ KvSeq kv_seq(const KvArgs& a, int b) {
   return s;
 }
 
-// Work is dealt out in slots of a host-known number, a slot being one block of 2^shift tokens of one
-// sequence at most.  Even batches: `per_seq` slots each.  Otherwise sequence b has the slots from
-// cu[b] / 2^shift + extra * b on.  extra = 1 covers blocks counted from a sequence's first new token
-// (ceil(n / T) <= floor(cu[b+1] / T) - floor(cu[b] / T) + 1), extra = 2 blocks at fixed places of the
-// sequence, which the new tokens may enter and leave in the middle.
-__host__ __device__ inline int64_t kv_slots(int batch, int tokens, int even, bool ragged, int shift, int extra) {
-  if (ragged) return (static_cast<int64_t>(tokens) >> shift) + static_cast<int64_t>(extra) * batch;
-  const int T = 1 << shift;
+// Work is dealt out in slots of a host-known number, a slot being one block of T tokens of one sequence at most.  Even
+// batches have the same number for each.  Otherwise sequence b has the slots from cu[b] / T + extra * b on.  extra = 1 covers blocks counted
+// from a sequence's first new token (ceil(n / T) <= floor(cu[b+1] / T) - floor(cu[b] / T) + 1), extra = 2 blocks at fixed places of
+// the sequence, which the new tokens may enter and leave in the middle; T = 1 and extra = 0 finds a token's sequence.
+__host__ __device__ inline int64_t kv_slots(int batch, int tokens, int even, bool ragged, int T, int extra) {
+  if (ragged) return static_cast<int64_t>(tokens) / T + static_cast<int64_t>(extra) * batch;
   return batch * ((static_cast<int64_t>(even) + T - 1) / T + (extra - 1));
 }
 
 // Sequence of a slot and the slot's number within it, by the calling warp (all lanes alike).
 // A search over 32 places at a time: two rounds of loads up to 1024 sequences.
-__device__ __forceinline__ void kv_find_slot(const KvArgs& a, int64_t slot, int shift, int extra, int* seq, int* j) {
+__device__ __forceinline__ void kv_find_slot(const KvArgs& a, int64_t slot, int T, int extra, int* seq, int* j) {
   if (a.cu == nullptr) {
-    const int T = 1 << shift;
     const int per_seq = (a.even + T - 1) / T + (extra - 1);
     *seq = static_cast<int>(slot / per_seq);
     *j = static_cast<int>(slot - static_cast<int64_t>(*seq) * per_seq);
@@ -81,7 +78,7 @@ __device__ __forceinline__ void kv_find_slot(const KvArgs& a, int64_t slot, int 
     bool before = false;
     if (at < lo + n) {
       const int t = min(max(ld_int(a.cu + at), 0), a.tokens);
-      before = (t >> shift) + static_cast<int64_t>(extra) * at <= slot;
+      before = t / T + static_cast<int64_t>(extra) * at <= slot;
     }
     const int count = __popc(__ballot_sync(0xffffffffu, before));
     const int from = lo + max(count - 1, 0) * step;
@@ -90,7 +87,7 @@ __device__ __forceinline__ void kv_find_slot(const KvArgs& a, int64_t slot, int 
   }
   const int t = min(max(ld_int(a.cu + lo), 0), a.tokens);
   *seq = lo;
-  const int64_t d = slot - ((t >> shift) + static_cast<int64_t>(extra) * lo);
+  const int64_t d = slot - (t / T + static_cast<int64_t>(extra) * lo);
   *j = d < 0 ? 0x3fffffff : static_cast<int>(d < 0x3fffffff ? d : 0x3fffffff);
 }
 
