@@ -43,6 +43,13 @@ struct KvRows {
 cudaError_t launch_kv_append(const KvArgs& a, const KvRows& k, const KvRows& v, bool bf16, bool e5m2, cudaStream_t stream);
 cudaError_t launch_kv_read(const KvArgs& a, void* k_out, void* v_out, bool bf16, bool e5m2, cudaStream_t stream);
 
+// Of an item that several CTAs share, written by the one that has its last part (first_cta -1: there is none).
+struct alignas(32) KvRecord {
+  int first_cta;
+  int first;                      // the sequence's first new token
+  int row0, n_rows, head;         // rows of the block; K/V head
+};
+
 struct KvAttendArgs {
   KvArgs c;
   KvRows q;
@@ -53,8 +60,11 @@ struct KvAttendArgs {
   int causal;
   int bf16;                       // of q and o; fp16 otherwise
   float scale_log2;               // softmax_scale * log2(e)
-  // In the workspace, filled in by launch_kv_attend: see fa8_kv_attend.cu.
-  int64_t* bases;                 // [batch + 1]
+  // Filled in by launch_kv_attend (see fa8_kv_attend.cu): CTAs of the cluster that has an item (0: shares of all steps), new tokens
+  // of an item; in the workspace the rest.
+  int n_split;
+  int block_tokens;
+  struct KvRecord* records;       // one per CTA
   float* partial;
 };
 struct KvAttendSizes {
@@ -62,8 +72,8 @@ struct KvAttendSizes {
   bool ragged;                    // cu_seqlens given
   int64_t keys_most;              // that a sequence can have: table_width * page_size
 };
-// tk, tv: the pools as 3-D byte tensors {head_dim, page_size, num_pages * heads} with a box of
-// kv_box_bytes(head_dim) x min(page_size, 32) x 1, swizzled over the box's row.
+// tk, tv: the pools as 3-D byte tensors {kv_map_bytes, page_size * head_dim / kv_map_bytes, num_pages * heads} with a box of
+// kv_box_bytes x kv_box_rows x 1, swizzled over the box's row.
 cudaError_t launch_kv_attend(const CUtensorMap& tk, const CUtensorMap& tv, KvAttendArgs a, const KvAttendSizes& z, void* workspace,
                              bool e5m2, int sms, cudaStream_t stream);
 int64_t kv_attend_workspace(const KvAttendSizes& z, int sms);
@@ -82,7 +92,20 @@ cudaError_t launch_kv_prefill(const CUtensorMap& tk, const CUtensorMap& tv, cons
                               bool e5m2, int sms, cudaStream_t stream);
 // Whether a call is one for launch_kv_prefill.
 bool kv_prefill_takes(const KvAttendSizes& z);
-inline int kv_box_bytes(int head_dim) { return head_dim <= 64 ? 64 : 128; }
+// Keys of a step of the kernel built for head dims up to `width`; the bytes of a row of the pools' maps (rows of 64 bytes are taken
+// two at a time) and of a box, and a box's rows: a step's keys, or a page's.
+#ifdef __CUDACC__
+#define FA8_HD __host__ __device__
+#else
+#define FA8_HD
+#endif
+FA8_HD constexpr int kv_step_keys(int width) { return width == 256 ? 16 : 32; }
+FA8_HD constexpr int kv_map_bytes(int head_dim) { return head_dim == 64 ? 128 : head_dim; }
+FA8_HD constexpr int kv_box_bytes(int head_dim) { return head_dim < 64 ? 64 : 128; }
+FA8_HD constexpr int kv_box_keys(int head_dim, int page_size) {
+  return page_size < kv_step_keys(head_dim <= 128 ? 128 : 256) ? page_size : kv_step_keys(head_dim <= 128 ? 128 : 256);
+}
+FA8_HD constexpr int kv_box_rows(int head_dim, int page_size) { return kv_box_keys(head_dim, page_size) * head_dim / kv_map_bytes(head_dim); }
 
 // fa8_capi.cu: a 3-D byte tensor {inner, mid, outer} with a {box_inner, box_mid, 1} tile, swizzled over
 // box_inner bytes (64 or 128).  False, with the detail string set, on failure.

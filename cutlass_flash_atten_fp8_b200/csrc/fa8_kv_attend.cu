@@ -24,6 +24,7 @@
 // Operand layouts are those of fa8_decode_sm100.cu: S = Q K^T with the query rows as M (16, eight of them padding
 // when there are eight) and eight keys as N, the k index permuted alike in both operands; O^T = V^T P^T with 16 output
 // columns as M, the rows as N and 16 keys as k.  tcgen05 would want 128 rows.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -36,26 +37,37 @@ namespace fa8 {
 
 namespace {
 
-constexpr int kStepKeys = 32;
+namespace cg = cooperative_groups;
+
 constexpr float kHeadroom = 6.f, kRaiseBy = 14.f;       // log2 of the largest P under a fresh reference, and at all
 constexpr float kLog2Least = -100.f;                   // log2 of the smallest scale of V that the reference m follows
 constexpr unsigned long long kLimitNs = 2000000000ull; // bound of every wait
+constexpr int kExpiredWait = 0xa77e;                   // code in the status words
 
 // Head dims up to W run in the instance built for W (the copies fill what is missing with zeros); RB blocks of eight rows.
 template <int W, int RB>
 struct ACfg {
+  static constexpr int kStepKeys = kv_step_keys(W);              // of a step: 4, 8 and 8 KB of K and V
+  static constexpr int kHalves = kStepKeys / 16;                 // of a step: sixteen keys lie in one page
   static constexpr int kRowBytes = W < 128 ? W : 128;            // of a swizzled tile
   static constexpr int kBlocks = W / kRowBytes;                  // tiles side by side
   static constexpr int kTile = kStepKeys * kRowBytes;
   static constexpr int kStageBytes = 2 * kBlocks * kTile;        // K, then V
-  static constexpr int kWarps = W == 256 ? 4 : 8;                // of the one CTA per SM
-  static constexpr int kStages = W == 64 ? 6 : 3;                // of each: 192 KB in all
+  // Warps of the one CTA per SM: what the register file holds at this instance's registers per thread (a quarter of the warps
+  // share a quarter of it), and stages of each: 180 to 192 KB in all.
+  static constexpr int kWarps = W == 64 && RB == 1 ? 16 : (W == 64 && RB == 2 ? 12 : 8);
+  static constexpr int kStages = kWarps == 16 ? 3 : (kWarps == 12 ? 4 : (W == 64 ? 6 : 3));
+  static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kChunks = W / 64;                         // 16-byte pieces of a K row per thread
   static constexpr int kSteps = W / 16;                          // k-steps of Q K^T
   static constexpr int kVWords = W == 64 ? 2 : 4;
   static constexpr int kTilesPerBlock = 2 * kVWords;
   static constexpr int kMTiles = W / 16;
   static constexpr int kRows = 8 * RB;
+  static constexpr int kORow = W + 4;                            // floats per row of a partial sum in shared memory
+  static constexpr int kPartBytes = kRows * (kORow + 2) * 4;
+  static_assert(kPartBytes <= kRingBytes, "a warp's partial sum lies in its ring");
+  static constexpr int kSmem = kWarps * kRingBytes + 1024;
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -74,8 +86,6 @@ __device__ __forceinline__ uint2 ld_shared8(uint32_t addr) {
   return v;
 }
 
-constexpr int kExpiredWait = 0xa77e;                   // code in the status words
-
 // By the whole warp: waits for the phase with the given parity, at most kLimitNs; whether it came, for all lanes alike.
 __device__ __forceinline__ bool wait_copies(uint32_t bar, uint32_t parity) {
   bool here = mbar_try_wait(bar, parity);
@@ -87,68 +97,53 @@ __device__ __forceinline__ bool wait_copies(uint32_t bar, uint32_t parity) {
 }
 
 // Steps of an item of sequence s, and its row blocks.  An item without keys has a step that finds none: its rows are zeros.
-__device__ __forceinline__ int item_steps(const KvSeq& s) { return max(1, (s.len + kStepKeys - 1) / kStepKeys); }
-__device__ __forceinline__ int64_t row_blocks(const KvSeq& s, int group, int rows) {
-  return (static_cast<int64_t>(s.n) * group + rows - 1) / rows;
-}
+__device__ __forceinline__ int item_steps(const KvSeq& s, int step_keys) { return max(1, (s.len + step_keys - 1) / step_keys); }
+__device__ __forceinline__ int row_blocks(const KvSeq& s, int group, int rows) { return (s.n * group + rows - 1) / rows; }
 
 // Share w of `total` steps among `workers`: [total * w / workers, total * (w + 1) / workers).
-__device__ __forceinline__ int64_t share_start(int64_t total, int64_t workers, int64_t w) { return total * w / workers; }
-__device__ __forceinline__ int64_t share_of(int64_t total, int64_t workers, int64_t x) {
-  return ((x + 1) * workers + total - 1) / total - 1;
-}
-__device__ __forceinline__ int64_t workers_of(int64_t total, int64_t workers) { return total < workers ? total : workers; }
+__device__ __forceinline__ int64_t share_start(int64_t total, int workers, int64_t w) { return total * w / workers; }
+__device__ __forceinline__ int64_t share_of(int64_t total, int workers, int64_t x) { return ((x + 1) * workers + total - 1) / total - 1; }
+__device__ __forceinline__ int workers_of(int64_t total, int workers) { return total < workers ? static_cast<int>(total) : workers; }
 
-// All threads of the CTA: the steps of the call, and in s_scan[8 + i] those of the sequences before the i-th thread's part of
-// the batch.  `bases` (one CTA only): the first step of every sequence, and the total.
-__device__ __forceinline__ void scan_sequences(const KvAttendArgs& a, int rows, int64_t* s_scan, int64_t* bases, int64_t* total) {
-  const int t = threadIdx.x, n = blockDim.x;
-  const int per = (a.c.batch + n - 1) / n;
-  const int b0 = min(t * per, a.c.batch), b1 = min(b0 + per, a.c.batch);
-  int64_t sum = 0;
-  for (int b = b0; b < b1; ++b) {
-    const KvSeq s = kv_seq(a.c, b);
-    if (s.bad && blockIdx.x == 0) report_bad_index(a.c);
-    sum += row_blocks(s, a.group, rows) * a.c.heads * item_steps(s);
-  }
-  int64_t x = sum;
+// What an item counts for when steps are dealt out: its steps, and kStartSteps for what a segment costs before its first step (a
+// chain of loads: page number, page, and the rows of Q).
+constexpr int kStartSteps = 2;
+__device__ __forceinline__ int64_t seq_units(const KvAttendArgs& a, const KvSeq& s, int rows, int step_keys) {
+  return static_cast<int64_t>(row_blocks(s, a.group, rows) * a.c.heads) * (item_steps(s, step_keys) + kStartSteps);
+}
+__device__ __forceinline__ int64_t warp_sum(int64_t x) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-    if ((t & 31) >= o) x += y;
-  }
-  if ((t & 31) == 31) s_scan[t >> 5] = x;
-  __syncthreads();
-  int64_t before = 0, all = 0;
-  for (int w = 0; w < (n >> 5); ++w) {
-    if (w < (t >> 5)) before += s_scan[w];
-    all += s_scan[w];
-  }
-  before += x - sum;
-  s_scan[8 + t] = before;
-  *total = all;
-  if (bases != nullptr) {
-    for (int b = b0; b < b1; ++b) {
-      bases[b] = before;
-      const KvSeq s = kv_seq(a.c, b);
-      before += row_blocks(s, a.group, rows) * a.c.heads * item_steps(s);
-    }
-    if (t == 0) bases[a.c.batch] = all;
-  }
-  __syncthreads();
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
 }
 
-template <int W, int RB, bool kE5M2>
+// Item of a warp's last segment.
+struct Segment {
+  int first, row0, n_rows, head;         // first new token of the sequence, rows of the block, K/V head
+  bool begins, ends;                     // the CTA's share has the item's first step, its last
+};
+
+// kLone: a cluster to an item, its CTAs and their warps sharing the item's steps; otherwise shares of all steps of the call.
+template <int W, int RB, bool kE5M2, bool kLone>
 __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                                                                   const KvAttendArgs a) {
+                                                                                const KvAttendArgs a) {
   using C = ACfg<W, RB>;
-  constexpr int kWarps = C::kWarps;
+  constexpr int kWarps = C::kWarps, kStepKeys = C::kStepKeys, kHalves = C::kHalves;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int64_t s_scan[8 + 32 * kWarps];
   __shared__ __align__(8) uint64_t s_bar[kWarps * C::kStages];
+  // scales of K of the step's halves (-1: no page), log2 of those of V
+  __shared__ __align__(16) float s_scale[kWarps * C::kStages][4];
+  // the first step of the item that a warp's last, and (where it had several) its first segment is of; -1: whole items only
+  __shared__ int64_t s_last[kWarps], s_head[kWarps];
+  __shared__ bool s_single[kWarps];
+  __shared__ Segment s_item[kLone ? 1 : kWarps];
+  __shared__ float s_m[C::kRows], s_l[C::kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + warp * C::kStages * C::kStageBytes;
+  const uint32_t ring0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t ring = ring0 + warp * C::kRingBytes;
   const uint32_t bars = smem_u32(s_bar) + 8u * warp * C::kStages;
+  // partial sums of warp w: [row][column], then the rows' references and sums
+  auto part_of = [&](int w) { return reinterpret_cast<float*>(smem_raw + (ring0 - smem_u32(smem_raw)) + w * C::kRingBytes); };
   if (lane == 0) {
     for (int i = 0; i < C::kStages; ++i) mbar_init(bars + 8 * i, 1);
     fence_mbar_init();
@@ -158,127 +153,240 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       prefetch_tensormap(&tv);
     }
   }
+  __syncwarp();
   start_after_predecessor();
   let_successor_start();
-  int64_t total;
-  scan_sequences(a, C::kRows, s_scan, blockIdx.x == 0 ? a.bases : nullptr, &total);
-  const int64_t workers = workers_of(total, static_cast<int64_t>(gridDim.x) * kWarps);
-  const int64_t me = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;         // neighbours on different SMs
-  if (me >= workers) return;
-  int64_t pos = share_start(total, workers, me);
-  const int64_t end = share_start(total, workers, me + 1);
-
-  // The sequence that pos is in: the last thread's part whose exclusive sum is not past it, then by steps of one.
-  int seq, per = (a.c.batch + 32 * kWarps - 1) / (32 * kWarps);
-  int64_t at;                                            // first step of `seq`
-  {
-    int part = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const int64_t v = s_scan[8 + 32 * i + lane];
-      part += __popc(__ballot_sync(0xffffffffu, v <= pos));
-    }
-    at = s_scan[8 + part - 1];
-    seq = (part - 1) * per;
-  }
-
   const int P = 1 << a.c.page_shift;
   const int boxes = P < kStepKeys ? 2 : 1;               // copies per step and tile
+  const int D = a.c.head_dim;
+  // Rows of 64 bytes come two to a swizzled line of 128 (D = 64; a copy moves a line at a time, whatever its length), rows of 32 padded to
+  // 64: in the first the halves of every other four lines are exchanged.
+  const uint32_t flip = W == 64 && D == 64 ? 64u : 0u;
+
+  // ---- what this warp has to do: steps [pos, end) of the call's (of the item's) ----
+  int64_t pos, end, at = 0, cta_lo = 0, cta_hi = 0, total = 0;
+  int ctas = 0;
+  int seq = 0, lone_row0 = 0, lone_head = 0;
+  KvSeq s;
+  int steps, items;
+  if constexpr (kLone) {
+    const int rank = static_cast<int>(blockIdx.x) % a.n_split, id = static_cast<int>(blockIdx.x) / a.n_split;
+    const int slot = id / a.c.heads;
+    lone_head = id - slot * a.c.heads;
+    int j;
+    kv_find_slot(a.c, slot, a.block_tokens, 1, &seq, &j);
+    s = kv_seq(a.c, seq);
+    if (s.bad && warp == 0 && lane == 0) report_bad_index(a.c);
+    // (a range that is out of range has n = 0 and so no items, but has slots: some CTA comes here for it)
+    const int64_t token0 = static_cast<int64_t>(j) * a.block_tokens;
+    if (token0 >= s.n) return;                           // the whole cluster
+    lone_row0 = static_cast<int>(token0) * a.group;
+    steps = item_steps(s, kStepKeys);
+    items = 1;
+    const int w = rank * kWarps + warp, n = a.n_split * kWarps;
+    pos = static_cast<int64_t>(steps) * w / n;
+    end = static_cast<int64_t>(steps) * (w + 1) / n;
+  } else {
+    // by every warp for itself: 32 sequences at a time, the first of which stay in registers
+    const KvSeq mine = lane < a.c.batch ? kv_seq(a.c, lane) : KvSeq{0, 0, 0, false};
+    const int64_t units = seq_units(a, mine, C::kRows, kStepKeys);
+    total = units;
+    bool bad = mine.bad;
+#pragma unroll 4
+    for (int b = 32 + lane; b < a.c.batch; b += 32) {
+      const KvSeq x = kv_seq(a.c, b);
+      bad = bad || x.bad;
+      total += seq_units(a, x, C::kRows, kStepKeys);
+    }
+    total = warp_sum(total);
+    if (bad && blockIdx.x == 0 && warp == 0) report_bad_index(a.c);
+    ctas = workers_of(total, gridDim.x);
+    if (threadIdx.x == 0) a.records[blockIdx.x].first_cta = -1;
+    if (static_cast<int>(blockIdx.x) >= ctas) return;
+    cta_lo = share_start(total, ctas, blockIdx.x);
+    cta_hi = share_start(total, ctas, blockIdx.x + 1);
+    pos = cta_lo + (cta_hi - cta_lo) * warp / kWarps;
+    end = cta_lo + (cta_hi - cta_lo) * (warp + 1) / kWarps;
+    // The sequence that pos is in.  (A warp without steps may stand behind the last one: it looks where the CTA begins.)
+    const int64_t from = pos < end ? pos : cta_lo;
+    for (int b0 = 0;; b0 += 32) {
+      KvSeq x = mine;
+      int64_t u = units;
+      if (b0 > 0) {
+        x = b0 + lane < a.c.batch ? kv_seq(a.c, b0 + lane) : KvSeq{0, 0, 0, false};
+        u = seq_units(a, x, C::kRows, kStepKeys);
+      }
+      int64_t sum = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, at + sum > from);
+      if (past != 0u) {
+        const int l = __ffs(past) - 1;
+        at += __shfl_sync(0xffffffffu, sum - u, l);
+        seq = b0 + l;
+        s.first = __shfl_sync(0xffffffffu, x.first, l);
+        s.n = __shfl_sync(0xffffffffu, x.n, l);
+        s.len = __shfl_sync(0xffffffffu, x.len, l);
+        break;
+      }
+      at += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    steps = item_steps(s, kStepKeys);
+    items = row_blocks(s, a.group, C::kRows) * a.c.heads;
+  }
+
+  // This CTA has the last part of an item that begins at `item_at`: what the combining kernel needs to know.
+  auto put_record = [&](int64_t item_at, int first, int row0, int n_rows, int h) {
+    a.records[blockIdx.x] = {static_cast<int>(share_of(total, ctas, item_at + kStartSteps)), first, row0, n_rows, h};
+  };
+
   int stage = 0;
   uint32_t phase = 0;
-
-  KvSeq s = kv_seq(a.c, seq);
-  int steps = item_steps(s);
-  int64_t items = row_blocks(s, a.group, C::kRows) * a.c.heads;
+  int64_t last_item = -1, head_item = -1;
+  bool single = false;
+  bool first = true;
   while (pos < end) {
-    while (pos >= at + items * steps) {                  // the next sequence that has items
-      at += items * steps;
-      s = kv_seq(a.c, ++seq);
-      steps = item_steps(s);
-      items = row_blocks(s, a.group, C::kRows) * a.c.heads;
+    int h, row0, n_rows, step0, step1;
+    int64_t item_at, item_end;
+    if constexpr (kLone) {
+      h = lone_head;
+      row0 = lone_row0;
+      n_rows = min(a.block_tokens * a.group, s.n * a.group - row0);
+      item_at = 0;
+      item_end = steps;
+      step0 = static_cast<int>(pos);
+      step1 = static_cast<int>(end);
+    } else {
+      const int units = steps + kStartSteps;
+      if (pos >= at + static_cast<int64_t>(items) * units) {             // the next sequence that has items
+        at += static_cast<int64_t>(items) * units;
+        s = kv_seq(a.c, ++seq);
+        steps = item_steps(s, kStepKeys);
+        items = row_blocks(s, a.group, C::kRows) * a.c.heads;
+        continue;
+      }
+      const int item = static_cast<int>((pos - at) / units);
+      item_at = at + static_cast<int64_t>(item) * units;
+      item_end = item_at + units;
+      // a share that ends before the item's first step leaves the item to the next
+      if (end - item_at <= kStartSteps) break;
+      step0 = max(0, static_cast<int>(pos - item_at) - kStartSteps);
+      step1 = static_cast<int>(min(item_end, end) - item_at) - kStartSteps;
+      const int rb = item / a.c.heads;
+      h = item - rb * a.c.heads;
+      row0 = rb * C::kRows;
+      n_rows = min(C::kRows, s.n * a.group - row0);
     }
-    const int64_t item = (pos - at) / steps;
-    const int64_t item_at = at + item * steps;
-    const int step0 = static_cast<int>(pos - item_at);
-    const int step1 = static_cast<int>(min(static_cast<int64_t>(steps), end - item_at));
-    const int rb = static_cast<int>(item / a.c.heads), h = static_cast<int>(item - static_cast<int64_t>(rb) * a.c.heads);
-    const int row0 = rb * C::kRows, n_rows = min(C::kRows, s.n * a.group - row0);
-    // keys that the block's last row sees; of the others, seen(row)
+    // keys that the block's last row sees, and its first
     auto seen = [&](int row) { return a.causal ? max(0, min(s.len, s.len - s.n + row / a.group + 1)) : s.len; };
     const int vis = seen(row0 + n_rows - 1);
     const int least = seen(row0);
     const int last = min(step1, (vis + kStepKeys - 1) / kStepKeys);     // steps past it see nothing
 
+    // The rows of Q: thread (g, t) takes columns 16 kChunks t ... of a block of 128 (64), the bytes of K that it reads below.  Asked
+    // for before the pages are: behind those they would wait for as long as a ring takes to fill.
+    uint4 q[RB][C::kChunks][2];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      const bool in = 8 * b + g < n_rows;
+      const int r = in ? row0 + 8 * b + g : row0, token = r / a.group;
+      const uint16_t* p = static_cast<const uint16_t*>(a.q.x) + (s.first + token) * a.q.token_stride + (h * a.group + (r - token * a.group)) * a.q.head_stride;
+#pragma unroll
+      for (int c = 0; c < C::kChunks; ++c) {
+        constexpr int kPer = C::kChunks < 2 ? C::kChunks : 2;            // chunks of a block
+        const int col = 128 * (c / 2) + 16 * (kPer * t + c % 2);
+        const bool read = in && col < D;
+        q[b][c][0] = read ? ld_global(reinterpret_cast<const uint4*>(p + col)) : make_uint4(0u, 0u, 0u, 0u);
+        q[b][c][1] = read ? ld_global(reinterpret_cast<const uint4*>(p + col + 8)) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+
     // ---- filling the ring ----
-    // Page of key `key` (of the two halves of a step, by lane & 1): loaded ahead, checked when it is used.
+    // Page numbers and scales of 32 pages at a time, a lane each: those of the batch of pages in use, the numbers and scales of the
+    // next, the numbers of the one after, so that no load is waited for once the segment has begun.
     const int* const table = a.c.table + static_cast<int64_t>(seq) * a.c.table_stride;
-    auto load_page = [&](int step) {
-      const int key = step * kStepKeys + (lane & 1) * 16;
-      return step < last && key < vis ? ld_int(table + (key >> a.c.page_shift)) : -2;
+    const int n_pages = (min(vis, last * kStepKeys) + P - 1) >> a.c.page_shift;     // of this segment's keys
+    auto load_page = [&](int p) { return p + lane < n_pages ? ld_int(table + p + lane) : -2; };
+    auto load_scale = [&](const float* d, int page) {
+      return static_cast<unsigned>(page) < static_cast<unsigned>(a.c.num_pages) ? ld_global(d + static_cast<int64_t>(page) * a.c.heads + h) : -1.f;
     };
-    // Copies of `step` into `st`; returns this lane's scale: of K (lanes 0, 1 mod 4) or V, of its half.
-    auto fill = [&](int step, int page, int st) {
-      const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.c.num_pages);
-      if (!ok && page != -2) report_bad_index(a.c);
-      float d = 0.f;
-      if (ok) d = ld_global(((lane & 2) ? a.c.v_descale : a.c.k_descale) + static_cast<int64_t>(page) * a.c.heads + h);
-      else d = -1.f;                                      // no such keys
-      const int p1 = __shfl_sync(0xffffffffu, ok ? page : -1, 1);
-      const int p0 = __shfl_sync(0xffffffffu, ok ? page : -1, 0);
+    int page0 = (step0 * kStepKeys) >> a.c.page_shift;   // the batch's first
+    int id = load_page(page0), id1 = load_page(page0 + 32), id2 = load_page(page0 + 64);
+    float kd_of = load_scale(a.c.k_descale, id), vd_of = load_scale(a.c.v_descale, id);
+    float kd1 = load_scale(a.c.k_descale, id1), vd1 = load_scale(a.c.v_descale, id1);
+    auto advance = [&](int step) {
+      if (((step * kStepKeys) >> a.c.page_shift) >= page0 + 32) {
+        page0 += 32;
+        id = id1;
+        kd_of = kd1;
+        vd_of = vd1;
+        id1 = id2;
+        kd1 = load_scale(a.c.k_descale, id1);
+        vd1 = load_scale(a.c.v_descale, id1);
+        id2 = load_page(page0 + 64);
+      }
+    };
+    // Copies of a step, by one lane.  (A batch of 32 pages begins with a step.)
+    auto copy = [&](int step, int st) {
+      const int key = step * kStepKeys, in_batch = (key >> a.c.page_shift) - page0;
+      const int p0 = __shfl_sync(0xffffffffu, id, in_batch);
+      const bool ok0 = static_cast<unsigned>(p0) < static_cast<unsigned>(a.c.num_pages);
+      int p1 = 0;
+      bool ok1 = false, bad = !ok0;
+      if (boxes == 2) {
+        p1 = __shfl_sync(0xffffffffu, id, in_batch + 1);
+        ok1 = static_cast<unsigned>(p1) < static_cast<unsigned>(a.c.num_pages);
+        bad = bad || (!ok1 && key + 16 < vis);
+      }
+      if (bad) report_bad_index(a.c);
       if (lane == 0) {
         const uint32_t bar = bars + 8 * st, dst = ring + st * C::kStageBytes;
-        const int in_page = (step * kStepKeys) & (P - 1);
-        const int loads = (p0 >= 0) + (boxes == 2 && p1 >= 0);
-        constexpr uint32_t kBoxRow = 2 * C::kBlocks * C::kRowBytes;
-        mbar_arrive_expect_tx(bar, loads * kBoxRow * (boxes == 2 ? 16 : kStepKeys));
-        for (int i = 0; i < boxes; ++i) {
-          const int p = i == 0 ? p0 : p1;
-          if (p < 0) continue;
-          const int slice = p * a.c.heads + h, row = i == 0 ? in_page : 0;
+        constexpr uint32_t kRow = 2 * C::kBlocks * C::kRowBytes;
+        mbar_arrive_expect_tx(bar, boxes == 2 ? (static_cast<int>(ok0) + ok1) * 16 * kRow : (ok0 ? kStepKeys * kRow : 0u));
+        if (ok0) {
+          const int slice = p0 * a.c.heads + h, row = (key & (P - 1)) >> (flip ? 1 : 0);
 #pragma unroll
           for (int c = 0; c < C::kBlocks; ++c) {
-            tma_load_3d(dst + c * C::kTile + i * 16 * C::kRowBytes, &tk, bar, c * 128, row, slice);
-            tma_load_3d(dst + (C::kBlocks + c) * C::kTile + i * 16 * C::kRowBytes, &tv, bar, c * 128, row, slice);
+            tma_load_3d(dst + c * C::kTile, &tk, bar, c * 128, row, slice);
+            tma_load_3d(dst + (C::kBlocks + c) * C::kTile, &tv, bar, c * 128, row, slice);
+          }
+        }
+        if (ok1) {
+          const int slice = p1 * a.c.heads + h;
+#pragma unroll
+          for (int c = 0; c < C::kBlocks; ++c) {
+            tma_load_3d(dst + c * C::kTile + 16 * C::kRowBytes, &tk, bar, c * 128, 0, slice);
+            tma_load_3d(dst + (C::kBlocks + c) * C::kTile + 16 * C::kRowBytes, &tv, bar, c * 128, 0, slice);
           }
         }
       }
-      return d;
+      __syncwarp();
     };
-    float scales[C::kStages];
-    int page_next = load_page(step0);
+    // Lane l looks after the step's half l & 1: the scale of K (l & 2 = 0), -1 where there is no page, or log2 of that of V.
+    auto put_scales = [&](int step, int st) {
+      const int key = step * kStepKeys + (lane & (kHalves - 1)) * 16;
+      const int src = ((key >> a.c.page_shift) - page0) & 31;
+      const float kd = __shfl_sync(0xffffffffu, kd_of, src), vd = __shfl_sync(0xffffffffu, vd_of, src);
+      if (lane < 4) s_scale[warp * C::kStages + st][lane] = (lane & 2) ? fmaxf(__log2f(vd), kLog2Least) : (key < vis ? kd : -1.f);
+    };
     {
       int st = stage;
 #pragma unroll
-      for (int i = 0; i < C::kStages; ++i) {
-        scales[i] = -1.f;
-        if (step0 + i < last) {
-          const int page = page_next;
-          page_next = load_page(step0 + i + 1);
-          scales[i] = fill(step0 + i, page, st);
-        }
+      for (int i = 0; i < C::kStages; ++i) {              // at most 32 pages: one batch
+        if (step0 + i < last) copy(step0 + i, st);
         if (++st == C::kStages) st = 0;
       }
     }
 
     // ---- the rows of Q as A operands ----
-    // Thread (g, t) takes columns 16 kChunks t ... of a block of 128 (64): the bytes of K that it reads below.
     uint32_t qa[C::kSteps][RB][2];
     float c_row[RB], m_row[RB], nm[RB], l_row[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
-      const int r = row0 + 8 * b + g;
-      const bool in = 8 * b + g < n_rows;
-      const int token = s.first + (in ? r / a.group : 0), head = h * a.group + (in ? r % a.group : 0);
-      const uint16_t* p = static_cast<const uint16_t*>(a.q.x) + token * a.q.token_stride + head * a.q.head_stride;
-      uint4 x[C::kChunks][2];
-#pragma unroll
-      for (int c = 0; c < C::kChunks; ++c) {
-        constexpr int kPer = C::kChunks < 2 ? C::kChunks : 2;            // chunks of a block
-        const int col = 128 * (c / 2) + 16 * (kPer * t + c % 2);
-        const bool read = in && col < a.c.head_dim;
-        x[c][0] = read ? ld_global(reinterpret_cast<const uint4*>(p + col)) : make_uint4(0u, 0u, 0u, 0u);
-        x[c][1] = read ? ld_global(reinterpret_cast<const uint4*>(p + col + 8)) : make_uint4(0u, 0u, 0u, 0u);
-      }
+      auto& x = q[b];
       float back = 1.f;
       if (a.bf16) {
         // into fp16: times the power of two that brings the row's largest to 2^14 ... 2^15
@@ -325,6 +433,15 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       nm[b] = 0.f;
       l_row[b] = 0.f;
     }
+    {
+      int st = stage;
+#pragma unroll
+      for (int i = 0; i < C::kStages; ++i) {
+        if (step0 + i < last) put_scales(step0 + i, st);
+        if (++st == C::kStages) st = 0;
+      }
+      __syncwarp();
+    }
 
     float o[C::kMTiles][RB][4];
 #pragma unroll
@@ -336,17 +453,9 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
 
     // ---- the steps ----
     for (int step = step0; step < last; ++step) {
-      const int page = page_next;
-      page_next = load_page(step + C::kStages + 1);
-      const float mine = scales[0];
-      float kd[2], vd[2];
-      kd[0] = __shfl_sync(0xffffffffu, mine, 0); kd[1] = __shfl_sync(0xffffffffu, mine, 1);
-      vd[0] = __shfl_sync(0xffffffffu, mine, 2); vd[1] = __shfl_sync(0xffffffffu, mine, 3);
-#pragma unroll
-      for (int i = 0; i + 1 < C::kStages; ++i) scales[i] = scales[i + 1];
-      scales[C::kStages - 1] = -1.f;
       if (!wait_copies(bars + 8 * stage, phase)) {
-        // Give up: report, wait (with a limit each) for the copies in flight, which write to this CTA's memory.
+        // Give up: report, wait (with a limit each) for the copies in flight, which write to this CTA's memory, and go where the
+        // others will be waiting.
         if (lane == 0) {
           if (a.c.status != nullptr) atomicCAS(a.c.status, 0, kExpiredWait);
           if (a.c.host_status != nullptr) *reinterpret_cast<volatile int*>(a.c.host_status) = kExpiredWait;
@@ -358,16 +467,19 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
             phase ^= 1u;
           }
         }
-        return;
+        end = pos;
+        break;
       }
       const uint32_t sk = ring + stage * C::kStageBytes, sv = sk + C::kBlocks * C::kTile;
+      const float4 scale = *reinterpret_cast<const float4*>(s_scale[warp * C::kStages + stage]);
+      const float kd[2] = {scale.x, scale.y}, lv[2] = {scale.z, scale.w};
       // a step that holds keys past some row's last, or of a page that is out of range
       const int key0 = step * kStepKeys;
-      const bool whole = key0 + kStepKeys <= least && kd[0] != -1.f && kd[1] != -1.f;
+      const bool whole = key0 + kStepKeys <= least && kd[0] != -1.f && (kHalves == 1 || kd[1] != -1.f);
 
-      float x[4][RB][2];                                  // score tile, row block, its two keys: x_j
+      float x[2 * kHalves][RB][2];                        // score tile, row block, its two keys: q . k8
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 2 * kHalves; ++j) {
         constexpr int kPairs = (RB + 1) / 2;
         float sc[kPairs][4];
 #pragma unroll
@@ -376,7 +488,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
 #pragma unroll
         for (int c = 0; c < C::kChunks; ++c) {
           uint32_t at_row;
-          if constexpr (W == 64) at_row = sk + row * 64 + ((t ^ ((row >> 1) & 3)) << 4);
+          if constexpr (W == 64) at_row = sk + ((row * 64 + ((t ^ ((row >> 1) & 3)) << 4)) ^ ((j & 1) ? flip : 0u));
           else at_row = sk + (c / 2) * C::kTile + row * 128 + (((2 * t + c % 2) ^ (row & 7)) << 4);
           const uint4 kr = ld_shared16(at_row);
           const uint32_t w[4] = {kr.x, kr.y, kr.z, kr.w};
@@ -392,9 +504,8 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
         }
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-          const float c = c_row[b] * kd[j >> 1];
-          x[j][b][0] = sc[b / 2][2 * (b & 1)] * c;
-          x[j][b][1] = sc[b / 2][2 * (b & 1) + 1] * c;
+          x[j][b][0] = sc[b / 2][2 * (b & 1)];
+          x[j][b][1] = sc[b / 2][2 * (b & 1) + 1];
         }
       }
       if (!whole) {
@@ -402,20 +513,22 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
         for (int b = 0; b < RB; ++b) {
           const int lim = seen(row0 + min(8 * b + g, n_rows - 1));
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < 2 * kHalves; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
               if (key0 + 8 * j + 2 * t + e >= lim || kd[j >> 1] == -1.f) x[j][b][e] = -INFINITY;
         }
       }
-      const float lv[2] = {fmaxf(__log2f(vd[0]), kLog2Least), fmaxf(__log2f(vd[1]), kLog2Least)};
       bool calm = true;
-      float top[RB];
+      float top[RB], c_of[RB][kHalves];
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        const float t0 = fmaxf(fmaxf(x[0][b][0], x[0][b][1]), fmaxf(x[1][b][0], x[1][b][1])) + lv[0];
-        const float t1 = fmaxf(fmaxf(x[2][b][0], x[2][b][1]), fmaxf(x[3][b][0], x[3][b][1])) + lv[1];
-        top[b] = fmaxf(t0, t1);
+        top[b] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kHalves; ++i) {
+          c_of[b][i] = fmaxf(c_row[b] * kd[i], 0x1p-126f);       // above zero: a masked -inf stays one
+          top[b] = fmaxf(top[b], fmaf(fmaxf(fmaxf(x[2 * i][b][0], x[2 * i][b][1]), fmaxf(x[2 * i + 1][b][0], x[2 * i + 1][b][1])), c_of[b][i], lv[i]));
+        }
         calm = calm && !(top[b] > m_row[b] + kRaiseBy);
       }
       if (!__all_sync(0xffffffffu, calm)) {
@@ -437,39 +550,36 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
           nm[b] = nm_new;
         }
       }
-      uint32_t pb[RB][4];
+      // P_j = 2^(x_j - m + log2 dv), and 2^(x_j - m) = P_j / dv for the denominators
+      uint32_t pb[RB][2 * kHalves];
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        float p[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int i = 0; i < kHalves; ++i) {
+          const float n = nm[b] + lv[i];
+          float p[4];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) p[2 * j + e] = ex2_approx(x[j][b][e] + nm[b]);
-        l_row[b] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) pb[b][j] = pack_half2(p[2 * j] * vd[j >> 1], p[2 * j + 1] * vd[j >> 1]);
-      }
-      if (!whole) {                                       // nothing of keys that do not count, not even a NaN times zero
-#pragma unroll
-        for (int b = 0; b < RB; ++b)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (kd[j >> 1] == -1.f) pb[b][j] = 0u;
+          for (int e = 0; e < 4; ++e) p[e] = ex2_approx(fmaf(x[2 * i + e / 2][b][e & 1], c_of[b][i], n));
+          l_row[b] = fmaf((p[0] + p[1]) + (p[2] + p[3]), ex2_approx(-lv[i]), l_row[b]);
+          pb[b][2 * i] = pack_half2(p[0], p[1]);
+          pb[b][2 * i + 1] = pack_half2(p[2], p[3]);
+        }
       }
 #pragma unroll
       for (int blk = 0; blk < C::kBlocks; ++blk) {
-        uint32_t vr[8][C::kVWords];
+        uint32_t vr[4 * kHalves][C::kVWords];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4 * kHalves; ++i) {
           const int row = 16 * (i >> 2) + 8 * ((i >> 1) & 1) + 2 * t + (i & 1);
           if constexpr (W == 64) {
-            const uint2 v = ld_shared8(sv + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1));
+            const uint2 v = ld_shared8(sv + ((row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1)) ^ ((i & 2) ? flip : 0u)));
             vr[i][0] = v.x; vr[i][1] = v.y;
           } else {
             const uint4 v = ld_shared16(sv + blk * C::kTile + row * 128 + ((g ^ (row & 7)) << 4));
             vr[i][0] = v.x; vr[i][1] = v.y; vr[i][C::kVWords - 2] = v.z; vr[i][C::kVWords - 1] = v.w;
           }
-          if (!whole && (key0 + row >= vis || kd[row >> 4] == -1.f)) {
+          // nothing of keys that do not count, not even a NaN times zero
+          if (!whole && (key0 + row >= vis || kd[i >> 2] == -1.f)) {
 #pragma unroll
             for (int w = 0; w < C::kVWords; ++w) vr[i][w] = 0u;
           }
@@ -477,7 +587,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
 #pragma unroll
         for (int w = 0; w < C::kVWords; ++w) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
+          for (int u = 0; u < kHalves; ++u) {
             const uint32_t* v = &vr[4 * u][w];
             constexpr int kKey = C::kVWords;
             uint32_t am[4][2];
@@ -494,23 +604,45 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
         }
       }
       __syncwarp();                                       // every lane has read the stage
-      if (step + C::kStages < last) scales[C::kStages - 1] = fill(step + C::kStages, page, stage);
+      if (step + C::kStages < last) {
+        advance(step + C::kStages);
+        copy(step + C::kStages, stage);
+        put_scales(step + C::kStages, stage);
+        __syncwarp();
+      }
       if (++stage == C::kStages) {
         stage = 0;
         phase ^= 1u;
       }
     }
+    if (pos >= end) break;
+
     // ---- what the segment gave ----
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
       l_row[b] += __shfl_xor_sync(0xffffffffu, l_row[b], 1);
       l_row[b] += __shfl_xor_sync(0xffffffffu, l_row[b], 2);
     }
-    const bool alone = step0 == 0 && step1 == steps;
-    const int D = a.c.head_dim;
-    // slot 2 w: the segment that share w begins with; 2 w + 1: one that begins an item and ends the share
-    const int64_t slot = 2 * me + (step0 == 0 ? 1 : 0);
-    float* const part = a.partial + slot * C::kRows * (D + 2);
+    const bool alone = !kLone && step0 == 0 && step1 == steps;           // the item is this warp's
+    // this is not its last segment
+    const bool more = !kLone && item_end < end && (end - item_end > kStartSteps);
+    // Where the sums go: to O; to the ring, which is idle once the last segment is through, to be put together with those of the
+    // CTA's other warps; or, of a first segment that others began, to the workspace.
+    float* part = nullptr;
+    int part_row = C::kORow;
+    if (!alone) {
+      if (more) {
+        part_row = D;
+        part = a.partial + (warp == 0 ? 2ll * blockIdx.x : 2ll * gridDim.x + static_cast<int64_t>(blockIdx.x) * kWarps + warp) * (C::kRows * (D + 2));
+        head_item = item_at;
+        if (warp == 0 && lane == 0) put_record(item_at, s.first, row0, n_rows, h);
+      } else {
+        part = part_of(warp);
+        last_item = item_at;
+        single = first;
+      }
+    }
+    float* const part_m = part + C::kRows * part_row;
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
       if (t == 0 && 8 * b + g < n_rows) {
@@ -520,8 +652,8 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
             a.lse[static_cast<int64_t>(s.first + r / a.group) * a.heads_q + h * a.group + r % a.group] =
                 l_row[b] == 0.f ? -INFINITY : (m_row[b] + __log2f(l_row[b])) * 0.6931471805599453f;
         } else {
-          part[C::kRows * D + 8 * b + g] = m_row[b];
-          part[C::kRows * (D + 1) + 8 * b + g] = l_row[b];
+          part_m[8 * b + g] = m_row[b];
+          part_m[C::kRows + 8 * b + g] = l_row[b];
         }
       }
       const float inv = l_row[b] == 0.f ? 0.f : 1.f / l_row[b];
@@ -554,84 +686,215 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
               st_global_v4(p + j, w[0], w[1], w[2], w[3]);
             }
           } else {
-            float4* const p = reinterpret_cast<float4*>(part + in * D + col);
+            float4* const p = reinterpret_cast<float4*>(part + in * part_row + col);
 #pragma unroll
             for (int j = 0; j < 2 * C::kTilesPerBlock; j += 4) p[j / 4] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
           }
         }
       }
     }
-    pos = item_at + step1;
+    if (!more) break;
+    pos = item_end;
+    first = false;
   }
-}
 
-// Rows (token and query head) whose item several warps shared: kParts warps to a row, of the CTA's eight.
-constexpr int kCombineWarps = 8;
-template <int kParts>
-__global__ void __launch_bounds__(32 * kCombineWarps) kv_combine_kernel(const KvAttendArgs a, int rows, int64_t workers_most) {
-  __shared__ float4 s_acc[kParts > 1 ? kCombineWarps : 1][64];
-  __shared__ float s_l[kCombineWarps];
-  start_after_predecessor();
-  let_successor_start();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kParts;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kCombineWarps / kParts) + warp / kParts;
-  const int token = static_cast<int>(row / a.heads_q), head = static_cast<int>(row - static_cast<int64_t>(token) * a.heads_q);
-  if (token >= a.c.tokens) return;                        // kParts > 1: the returns are the whole CTA's
-  int b, unused;
-  if (a.c.cu == nullptr) b = token / a.c.even;
-  else kv_find_slot(a.c, token, 1, 0, &b, &unused);
-  const KvSeq s = kv_seq(a.c, b);
-  if (token < s.first || token >= s.first + s.n) return;
-  const volatile int64_t* bases = a.bases;
-  const int64_t total = bases[a.c.batch], base = bases[b];
-  const int64_t workers = workers_of(total, workers_most);
-  const int h = head / a.group;
-  const int64_t r = static_cast<int64_t>(token - s.first) * a.group + head % a.group, rb = r / rows;
-  const int in = static_cast<int>(r - rb * rows);
-  const int steps = item_steps(s);
-  const int64_t first = base + (rb * a.c.heads + h) * steps;
-  const int64_t w0 = share_of(total, workers, first), w1 = share_of(total, workers, first + steps - 1);
-  if (w0 == w1) return;
-  const int D = a.c.head_dim;
-  // the item begins at the end of share w0 and goes on at the beginning of the next
-  auto part_of = [&](int64_t w) { return a.partial + (2 * w + (w == w0 ? 1 : 0)) * rows * (D + 2); };
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int64_t w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, ld_global(part_of(w) + rows * D + in));
+  if constexpr (kLone) {
+    // ---- the item's sum: of this CTA's warps, in the place of warp 0's, then of the cluster ----
+    if (lane == 0) s_single[warp] = last_item >= 0;
+    __syncthreads();
+    const int n_rows = min(a.block_tokens * a.group, s.n * a.group - lone_row0);
+    for (int i = threadIdx.x; i < n_rows * (W / 4); i += 32 * kWarps) {
+      const int r = i / (W / 4), col = 4 * (i % (W / 4));
+      if (col >= D) continue;
+      float m = -INFINITY, l = 0.f;
+      for (int w = 0; w < kWarps; ++w)
+        if (s_single[w]) m = fmaxf(m, part_of(w)[C::kRows * C::kORow + r]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 0; w < kWarps; ++w) {
+        if (!s_single[w]) continue;
+        const float* p = part_of(w);
+        const float mw = p[C::kRows * C::kORow + r];
+        const float f = mw == -INFINITY ? 0.f : ex2_approx(mw - m);
+        const float4 x = *reinterpret_cast<const float4*>(p + r * C::kORow + col);
+        acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+        l += p[C::kRows * C::kORow + C::kRows + r] * f;
+      }
+      *reinterpret_cast<float4*>(part_of(0) + r * C::kORow + col) = acc;
+      if (col == 0) {
+        s_m[r] = m;
+        s_l[r] = l;
+      }
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    const int n_split = a.n_split;
+    if (n_split > 1) cluster.sync();
+    else __syncthreads();
+    const int rank = static_cast<int>(blockIdx.x) % n_split;
+    for (int i = rank * 32 * kWarps + threadIdx.x; i < n_rows * (W / 4); i += n_split * 32 * kWarps) {
+      const int r = i / (W / 4), col = 4 * (i % (W / 4));
+      if (col >= D) continue;
+      float m = -INFINITY, l = 0.f;
+      for (int p = 0; p < n_split; ++p) m = fmaxf(m, n_split > 1 ? *cluster.map_shared_rank(s_m + r, p) : s_m[r]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int p = 0; p < n_split; ++p) {
+        const float *po = part_of(0) + r * C::kORow + col, *pm = s_m + r, *pl = s_l + r;
+        if (n_split > 1) {
+          po = cluster.map_shared_rank(po, p);
+          pm = cluster.map_shared_rank(pm, p);
+          pl = cluster.map_shared_rank(pl, p);
+        }
+        const float f = *pm == -INFINITY ? 0.f : ex2_approx(*pm - m);
+        const float4 x = *reinterpret_cast<const float4*>(po);
+        acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+        l += *pl * f;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int row = lone_row0 + r;
+      const int64_t at_row = static_cast<int64_t>(s.first + row / a.group) * a.heads_q + lone_head * a.group + row % a.group;
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at_row * D + col) =
+          a.bf16 ? make_uint2(pack_pair<true>(acc.x * inv, acc.y * inv), pack_pair<true>(acc.z * inv, acc.w * inv))
+                 : make_uint2(pack_pair<false>(acc.x * inv, acc.y * inv), pack_pair<false>(acc.z * inv, acc.w * inv));
+      if (a.lse != nullptr && col == 0) a.lse[at_row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+    }
+    if (n_split > 1) cluster.sync();                       // no CTA leaves while its shared memory is read
+    return;
+  }
+
+  // ---- items that several of the CTA's warps shared ----
+  // All threads go through them: the last segment of the warp that has an item's first part here, those of the warps after it while
+  // they had no other, and the first segment of a warp that had several.
+  if (lane == 0) {
+    s_last[warp] = last_item;
+    s_head[warp] = head_item;
+    s_single[warp] = single;
+    if (last_item >= 0) {                                  // `s` and `steps` are those of the last segment
+      const int units = steps + kStartSteps, item = static_cast<int>((last_item - at) / units), rb = item / a.c.heads;
+      s_item[warp] = {s.first, rb * C::kRows, min(C::kRows, s.n * a.group - rb * C::kRows), item - rb * a.c.heads,
+                      last_item + kStartSteps >= cta_lo, last_item + units <= cta_hi};
+    }
+  }
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) {
+    const int64_t item = s_last[w];
+    if (item < 0) continue;
+    if (s_single[w]) {                                     // begun by an earlier warp?
+      int x = w - 1;
+      while (x >= 0 && s_last[x] < 0 && s_head[x] < 0) --x;               // warps without steps, or with whole items only
+      if (x >= 0 && s_last[x] == item) continue;
+    }
+    int to = w + 1, heads_from = -1;
+    for (; to < kWarps; ++to) {
+      if (s_last[to] < 0 && s_head[to] < 0) continue;
+      if (s_single[to] && s_last[to] == item) continue;
+      if (s_head[to] == item) heads_from = to;
+      break;
+    }
+    const Segment it = s_item[w];
+    if (!it.begins && it.ends && threadIdx.x == 0) put_record(item, it.first, it.row0, it.n_rows, it.head);
+    float* const part = a.partial + (2ll * blockIdx.x + (it.begins ? 1 : 0)) * (C::kRows * (D + 2));
+    const float* const head = a.partial + (2ll * gridDim.x + static_cast<int64_t>(blockIdx.x) * kWarps + heads_from) * (C::kRows * (D + 2));
+    for (int i = threadIdx.x; i < C::kRows * (W / 4); i += 32 * kWarps) {
+      const int r = i / (W / 4), col = 4 * (i % (W / 4));
+      if (r >= it.n_rows || col >= D) continue;
+      float m = -INFINITY, mh = -INFINITY, l = 0.f, lh = 0.f, mw[kWarps];
+      uint4 u = make_uint4(0u, 0u, 0u, 0u);
+      if (heads_from >= 0) {
+        mh = ld_global(head + C::kRows * D + r);
+        lh = ld_global(head + C::kRows * (D + 1) + r);
+        u = ld_global(reinterpret_cast<const uint4*>(head + r * D + col));
+      }
 #pragma unroll
-  for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
-  float l = 0.f;
-  const int quads = D >> 2;                               // a lane has quads lane and lane + 32
-  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll 8
-  for (int64_t w = w0 + part; w <= w1; w += kParts) {
-    const float* p = part_of(w);
-    const float mw = ld_global(p + rows * D + in);
-    const float f = mw == -INFINITY ? 0.f : ex2_approx(mw - m);
-    l += ld_global(p + rows * (D + 1) + in) * f;
+      for (int x = 0; x < kWarps; ++x) mw[x] = x >= w && x < to && s_last[x] == item ? part_of(x)[C::kRows * C::kORow + r] : -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int q = lane + 32 * i;
-      if (q < quads) {
-        const uint4 u = ld_global(reinterpret_cast<const uint4*>(p + in * D) + q);
-        acc[i].x += __uint_as_float(u.x) * f; acc[i].y += __uint_as_float(u.y) * f;
-        acc[i].z += __uint_as_float(u.z) * f; acc[i].w += __uint_as_float(u.w) * f;
+      for (int x = 0; x < kWarps; ++x) m = fmaxf(m, mw[x]);
+      m = fmaxf(m, mh);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      auto add = [&](float mx, float lx, const float4& v) {
+        const float f = mx == -INFINITY ? 0.f : ex2_approx(mx - m);
+        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+        l += lx * f;
+      };
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        if (mw[x] == -INFINITY) continue;
+        const float* p = part_of(x);
+        add(mw[x], p[C::kRows * C::kORow + C::kRows + r], *reinterpret_cast<const float4*>(p + r * C::kORow + col));
+      }
+      if (heads_from >= 0)
+        add(mh, lh, make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w)));
+      if (it.begins && it.ends) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int row = it.row0 + r, token = row / a.group;
+        const int64_t at_row = static_cast<int64_t>(it.first + token) * a.heads_q + it.head * a.group + (row - token * a.group);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at_row * D + col) =
+            a.bf16 ? make_uint2(pack_pair<true>(acc.x * inv, acc.y * inv), pack_pair<true>(acc.z * inv, acc.w * inv))
+                   : make_uint2(pack_pair<false>(acc.x * inv, acc.y * inv), pack_pair<false>(acc.z * inv, acc.w * inv));
+        if (a.lse != nullptr && col == 0) a.lse[at_row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+      } else {
+        *reinterpret_cast<float4*>(part + r * D + col) = acc;
+        if (col == 0) {
+          part[C::kRows * D + r] = m;
+          part[C::kRows * (D + 1) + r] = l;
+        }
       }
     }
   }
-  if (kParts > 1) {
-    s_acc[warp][lane] = acc[0];
-    s_acc[warp][lane + 32] = acc[1];
-    if (lane == 0) s_l[warp] = l;
-    __syncthreads();
-    if (warp != 0) return;
+}
+
+// Items that several CTAs shared, by the record of the last of them: a warp to a row (token and query head).
+constexpr int kCombineWarps = 4;
+__global__ void __launch_bounds__(32 * kCombineWarps) kv_combine_kernel(const KvAttendArgs a, int rows) {
+  start_after_predecessor();
+  let_successor_start();
+  const int lane = threadIdx.x & 31, in = static_cast<int>(blockIdx.y) * kCombineWarps + (threadIdx.x >> 5);
+  const int* const rec = reinterpret_cast<const int*>(a.records + blockIdx.x);
+  const uint4 r4 = ld_global(reinterpret_cast<const uint4*>(rec));
+  const int h = ld_int(rec + 4), c0 = static_cast<int>(r4.x), c1 = blockIdx.x;
+  if (c0 < 0 || in >= static_cast<int>(r4.w)) return;
+  const int r = static_cast<int>(r4.z) + in, token = r / a.group;
+  const int64_t row = static_cast<int64_t>(r4.y + token) * a.heads_q + h * a.group + (r - token * a.group);
+  const int D = a.c.head_dim;
+  // the item begins at the end of share c0 and goes on at the beginning of the next
+  auto part_of = [&](int c) { return a.partial + (2ll * c + (c == c0 ? 1 : 0)) * (rows * (D + 2)); };
+  const int quads = D >> 2;                               // a lane has quads lane and lane + 32
+  float m = -INFINITY, l = 0.f;
+  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  constexpr int kAt = 8;                                  // parts at a time, all loads of which go out together
+  for (int c = c0; c <= c1; c += kAt) {
+    float mp[kAt], lp[kAt];
+    uint4 v[kAt][2];
 #pragma unroll
-    for (int w = 1; w < kParts; ++w) {
-      l += s_l[w];
+    for (int i = 0; i < kAt; ++i) {
+      mp[i] = -INFINITY;
+      lp[i] = 0.f;
+      v[i][0] = v[i][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (c + i <= c1) {
+        const float* p = part_of(c + i);
+        mp[i] = ld_global(p + rows * D + in);
+        lp[i] = ld_global(p + rows * (D + 1) + in);
+        if (lane < quads) v[i][0] = ld_global(reinterpret_cast<const uint4*>(p + in * D) + lane);
+        if (lane + 32 < quads) v[i][1] = ld_global(reinterpret_cast<const uint4*>(p + in * D) + lane + 32);
+      }
+    }
+    float top = m;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float4 v = s_acc[w][lane + 32 * i];
-        acc[i].x += v.x; acc[i].y += v.y; acc[i].z += v.z; acc[i].w += v.w;
+    for (int i = 0; i < kAt; ++i) top = fmaxf(top, mp[i]);
+    if (top == -INFINITY) continue;
+    const float back = m == -INFINITY ? 0.f : ex2_approx(m - top);
+    m = top;
+    l *= back;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      acc[k].x *= back; acc[k].y *= back; acc[k].z *= back; acc[k].w *= back;
+    }
+#pragma unroll
+    for (int i = 0; i < kAt; ++i) {
+      const float f = mp[i] == -INFINITY ? 0.f : ex2_approx(mp[i] - m);
+      l += lp[i] * f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        acc[k].x += __uint_as_float(v[i][k].x) * f; acc[k].y += __uint_as_float(v[i][k].y) * f;
+        acc[k].z += __uint_as_float(v[i][k].z) * f; acc[k].w += __uint_as_float(v[i][k].w) * f;
       }
     }
   }
@@ -656,73 +919,102 @@ int block_rows(const KvAttendSizes& z) {
   if (mean <= 8) return 8;
   return mean <= 16 || width_of(z.head_dim) == 256 ? 16 : 32;
 }
+int warps_of(const KvAttendSizes& z) {
+  const int rows = block_rows(z);
+  switch (width_of(z.head_dim)) {
+    case 64: return rows == 8 ? ACfg<64, 1>::kWarps : (rows == 16 ? ACfg<64, 2>::kWarps : ACfg<64, 4>::kWarps);
+    case 128: return rows == 8 ? ACfg<128, 1>::kWarps : (rows == 16 ? ACfg<128, 2>::kWarps : ACfg<128, 4>::kWarps);
+    default: return rows == 8 ? ACfg<256, 1>::kWarps : ACfg<256, 2>::kWarps;
+  }
+}
 
-template <int W, int RB, bool kE5M2>
-cudaError_t launch_attend(const CUtensorMap& tk, const CUtensorMap& tv, const KvAttendArgs& a, int sms, cudaStream_t stream) {
+// A cluster to an item (no second kernel, no workspace) where that leaves no CTA more than kLoneKeys keys, going by what the page
+// table can hold; CTAs of the cluster, or 0.
+constexpr int64_t kLoneKeys = 1024;
+int lone_split(const KvAttendSizes& z, int sms) {
+  const int group = z.heads_q / z.heads, rows = block_rows(z);
+  if (group > rows) return 0;
+  const int64_t items = kv_slots(z.batch, z.tokens, z.tokens / z.batch, z.ragged, rows / group, 1) * z.heads;
+  int split = 1;
+  const int64_t steps = (z.keys_most + kv_step_keys(width_of(z.head_dim)) - 1) / kv_step_keys(width_of(z.head_dim));
+  while (split < 8 && 2 * split * items <= sms && split * warps_of(z) < steps) split *= 2;
+  return z.keys_most <= kLoneKeys * split && items <= 2 * sms ? split : 0;
+}
+
+template <int W, int RB, bool kE5M2, bool kLone>
+cudaError_t launch_attend(const CUtensorMap& tk, const CUtensorMap& tv, const KvAttendArgs& a, const KvAttendSizes& z, int sms, cudaStream_t stream) {
   using C = ACfg<W, RB>;
-  auto kernel = &kv_attend_kernel<W, RB, kE5M2>;
-  constexpr int smem = C::kWarps * C::kStages * C::kStageBytes + 1024;
+  auto kernel = &kv_attend_kernel<W, RB, kE5M2, kLone>;
   static std::atomic<bool> ready[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const bool cached = dev >= 0 && dev < 64;
   if (!cached || !ready[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return e;
     if (cached) ready[dev].store(true, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(sms), 1, 1);
   cfg.blockDim = dim3(32 * C::kWarps, 1, 1);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1] = {overlap_attribute()};
+  cudaLaunchAttribute attr[2] = {overlap_attribute()};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (kLone) {
+    const int64_t items = kv_slots(z.batch, z.tokens, z.tokens / z.batch, z.ragged, a.block_tokens, 1) * z.heads;
+    cfg.gridDim = dim3(static_cast<unsigned>(items * a.n_split), 1, 1);
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(a.n_split);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = a.n_split > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, tk, tv, a);
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(sms), 1, 1);
   e = cudaLaunchKernelEx(&cfg, kernel, tk, tv, a);
   if (e != cudaSuccess) return e;
-  // Up to kWideRows rows a CTA takes one: an item of a long sequence has a part from every warp that shared it.
-  constexpr int64_t kWideRows = 8192;
-  const int64_t n = static_cast<int64_t>(a.c.tokens) * a.heads_q;
-  const int64_t ctas = n <= kWideRows ? n : (n + kCombineWarps - 1) / kCombineWarps;
-  if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(sms), C::kRows / kCombineWarps, 1);
   cfg.blockDim = dim3(32 * kCombineWarps, 1, 1);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, n <= kWideRows ? &kv_combine_kernel<kCombineWarps> : &kv_combine_kernel<1>, a, C::kRows,
-                            static_cast<int64_t>(sms) * C::kWarps);
+  return cudaLaunchKernelEx(&cfg, &kv_combine_kernel, a, C::kRows);
 }
 
-template <bool kE5M2>
-cudaError_t launch_fmt(const CUtensorMap& tk, const CUtensorMap& tv, const KvAttendArgs& a, int sms, int rows, cudaStream_t stream) {
-  switch (width_of(a.c.head_dim)) {
-    case 64:
-      return rows == 8 ? launch_attend<64, 1, kE5M2>(tk, tv, a, sms, stream)
-                       : (rows == 16 ? launch_attend<64, 2, kE5M2>(tk, tv, a, sms, stream) : launch_attend<64, 4, kE5M2>(tk, tv, a, sms, stream));
-    case 128:
-      return rows == 8 ? launch_attend<128, 1, kE5M2>(tk, tv, a, sms, stream)
-                       : (rows == 16 ? launch_attend<128, 2, kE5M2>(tk, tv, a, sms, stream) : launch_attend<128, 4, kE5M2>(tk, tv, a, sms, stream));
-    default:
-      return rows == 8 ? launch_attend<256, 1, kE5M2>(tk, tv, a, sms, stream) : launch_attend<256, 2, kE5M2>(tk, tv, a, sms, stream);
-  }
+template <int W, int RB>
+cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const KvAttendArgs& a, const KvAttendSizes& z, bool e5m2, int sms, cudaStream_t stream) {
+  if (a.n_split > 0)
+    return e5m2 ? launch_attend<W, RB, true, true>(tk, tv, a, z, sms, stream) : launch_attend<W, RB, false, true>(tk, tv, a, z, sms, stream);
+  return e5m2 ? launch_attend<W, RB, true, false>(tk, tv, a, z, sms, stream) : launch_attend<W, RB, false, false>(tk, tv, a, z, sms, stream);
 }
 
-int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+int64_t records_bytes(int sms) { return (static_cast<int64_t>(sms) * sizeof(KvRecord) + 255) / 256 * 256; }
 
 }  // namespace
 
 int64_t kv_attend_workspace(const KvAttendSizes& z, int sms) {
-  const int64_t slots = 2ll * sms * (width_of(z.head_dim) == 256 ? ACfg<256, 1>::kWarps : ACfg<128, 1>::kWarps);
-  return round256((static_cast<int64_t>(z.batch) + 1) * 8) + slots * block_rows(z) * (z.head_dim + 2) * 4;
+  if (lone_split(z, sms) > 0) return 0;
+  const int64_t slots = static_cast<int64_t>(sms) * (2 + warps_of(z));
+  return records_bytes(sms) + slots * block_rows(z) * (z.head_dim + 2) * 4;
 }
 
 cudaError_t launch_kv_attend(const CUtensorMap& tk, const CUtensorMap& tv, KvAttendArgs a, const KvAttendSizes& z, void* workspace, bool e5m2, int sms,
                              cudaStream_t stream) {
-  a.bases = static_cast<int64_t*>(workspace);
-  a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256((static_cast<int64_t>(a.c.batch) + 1) * 8));
+  a.records = static_cast<KvRecord*>(workspace);
+  a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + records_bytes(sms));
   const int rows = block_rows(z);
-  return e5m2 ? launch_fmt<true>(tk, tv, a, sms, rows, stream) : launch_fmt<false>(tk, tv, a, sms, rows, stream);
+  a.n_split = lone_split(z, sms);
+  a.block_tokens = rows / a.group;
+  switch (width_of(a.c.head_dim)) {
+    case 64:
+      return rows == 8 ? launch_rows<64, 1>(tk, tv, a, z, e5m2, sms, stream)
+                       : (rows == 16 ? launch_rows<64, 2>(tk, tv, a, z, e5m2, sms, stream) : launch_rows<64, 4>(tk, tv, a, z, e5m2, sms, stream));
+    case 128:
+      return rows == 8 ? launch_rows<128, 1>(tk, tv, a, z, e5m2, sms, stream)
+                       : (rows == 16 ? launch_rows<128, 2>(tk, tv, a, z, e5m2, sms, stream) : launch_rows<128, 4>(tk, tv, a, z, e5m2, sms, stream));
+    default:
+      return rows == 8 ? launch_rows<256, 1>(tk, tv, a, z, e5m2, sms, stream) : launch_rows<256, 2>(tk, tv, a, z, e5m2, sms, stream);
+  }
 }
 
 }  // namespace fa8

@@ -164,9 +164,11 @@ int fa8_kv_attention(const fa8_kv_attention_params* p, void* cuda_stream) {
   const int64_t slices = static_cast<int64_t>(c.num_pages) * c.heads_kv;
   if (!(m.valid && m.k == c.k && m.v == c.v && m.slices == slices && m.page_size == c.page_size && m.head_dim == c.head_dim)) {
     m.valid = false;
-    const uint32_t inner = static_cast<uint32_t>(fa8::kv_box_bytes(c.head_dim)), rows = c.page_size < 32 ? 16u : 32u;
-    if (!fa8::make_byte_map(&m.tk, c.k, c.head_dim, c.page_size, slices, inner, rows)) return FA8_ERR_CUDA;
-    if (!fa8::make_byte_map(&m.tv, c.v, c.head_dim, c.page_size, slices, inner, rows)) return FA8_ERR_CUDA;
+    const uint32_t inner = static_cast<uint32_t>(fa8::kv_box_bytes(c.head_dim)), rows = static_cast<uint32_t>(fa8::kv_box_rows(c.head_dim, c.page_size));
+    const uint64_t row = static_cast<uint64_t>(fa8::kv_map_bytes(c.head_dim));
+    const uint64_t n_rows = static_cast<uint64_t>(c.page_size) * c.head_dim / row;
+    if (!fa8::make_byte_map(&m.tk, c.k, row, n_rows, slices, inner, rows)) return FA8_ERR_CUDA;
+    if (!fa8::make_byte_map(&m.tv, c.v, row, n_rows, slices, inner, rows)) return FA8_ERR_CUDA;
     m.k = c.k;
     m.v = c.v;
     m.slices = slices;

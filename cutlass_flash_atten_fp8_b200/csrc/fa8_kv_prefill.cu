@@ -287,6 +287,8 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
   start_after_predecessor();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
 
+  // rows of 64 bytes lie two to a swizzled line of 128: the halves of every other four lines are exchanged
+  const uint32_t flip = W == 64 && a.c.head_dim == 64 ? 64u : 0u;
   const int group = a.group, tile_tokens = kTileM / group;       // a token's rows lie in one tile
   // Consumers of the item ring: the next item (false: no more, or a wait ran out).
   int n_items = 0;
@@ -398,9 +400,9 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.blk_full[n]));
         ++blocks;
-        // one copy per page part of the block (box_rows keys) and 128 columns
-        const int box_rows = min(1 << a.c.page_shift, 32);
-        const bool issues = here && (16 * lane) % box_rows == 0;
+        // one copy per page part of the block (box_keys keys) and 128 columns
+        const int box_keys = kv_box_keys(W, 1 << a.c.page_shift);
+        const bool issues = here && (16 * lane) % box_keys == 0;
         const int boxes = __popc(__ballot_sync(0xffffffffu, issues));
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
@@ -411,10 +413,10 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           if (lane == 0) sh.valid[st] = max(0, min(C::kN, it.vis - blk * C::kN));
           __syncwarp();
           const uint32_t bar = smem_u32(&sh.raw_full[st]);
-          if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_rows * C::kRawRow * C::kRawBlocks);
+          if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_keys * C::kRawRow * C::kRawBlocks);
           __syncwarp();
           if (issues) {
-            const int row = (blk * C::kN + 16 * lane) & ((1 << a.c.page_shift) - 1);
+            const int row = ((blk * C::kN + 16 * lane) & ((1 << a.c.page_shift) - 1)) >> (flip ? 1 : 0);
 #pragma unroll
             for (int b = 0; b < C::kRawBlocks; ++b)
               tma_load_3d(s_raw + st * C::kRawBytes + b * C::kRawBlockBytes + 16 * lane * C::kRawRow, kv ? &tv : &tk, bar, 128 * b, row,
@@ -578,7 +580,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         for (int p = w; p < kParts; p += 4) {
           const int cb = p % C::kCols, r = (p / C::kCols) * 8 + (lane & 7), q = lane >> 3;
           uint32_t from;
-          if constexpr (W == 64) from = src + r * 64 + ((q ^ ((r >> 1) & 3)) << 4);
+          if constexpr (W == 64) from = src + ((r * 64 + ((q ^ ((r >> 1) & 3)) << 4)) ^ ((r & 8) ? flip : 0u));
           else from = src + (cb >> 1) * C::kRawBlockBytes + r * 128 + (((4 * (cb & 1) + q) ^ (r & 7)) << 4);
           uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
           const uint32_t f = sh.factor[st][r >> 4];
