@@ -64,6 +64,7 @@ struct KvAttendArgs {
   // of an item; in the workspace the rest.
   int n_split;
   int block_tokens;
+  int unit_shift;                 // log2 of the steps that work is dealt out by
   struct KvRecord* records;       // one per CTA
   float* partial;
 };

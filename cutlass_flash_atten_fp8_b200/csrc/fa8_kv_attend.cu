@@ -100,21 +100,12 @@ __device__ __forceinline__ bool wait_copies(uint32_t bar, uint32_t parity) {
 __device__ __forceinline__ int item_steps(const KvSeq& s, int step_keys) { return max(1, (s.len + step_keys - 1) / step_keys); }
 __device__ __forceinline__ int row_blocks(const KvSeq& s, int group, int rows) { return (s.n * group + rows - 1) / rows; }
 
-// Share w of `total` steps among `workers`: [total * w / workers, total * (w + 1) / workers).
-__device__ __forceinline__ int64_t share_start(int64_t total, int workers, int64_t w) { return total * w / workers; }
-__device__ __forceinline__ int64_t share_of(int64_t total, int workers, int64_t x) { return ((x + 1) * workers + total - 1) / total - 1; }
-__device__ __forceinline__ int workers_of(int64_t total, int workers) { return total < workers ? static_cast<int>(total) : workers; }
-
-// What an item counts for when steps are dealt out: its steps, and kStartSteps for what a segment costs before its first step (a
-// chain of loads: page number, page, and the rows of Q).
-constexpr int kStartSteps = 2;
-__device__ __forceinline__ int64_t seq_units(const KvAttendArgs& a, const KvSeq& s, int rows, int step_keys) {
-  return static_cast<int64_t>(row_blocks(s, a.group, rows) * a.c.heads) * (item_steps(s, step_keys) + kStartSteps);
-}
-__device__ __forceinline__ int64_t warp_sum(int64_t x) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
+// What an item counts for when work is dealt out, in units of 2^unit_shift steps: its steps, and kStartUnits for what a segment costs
+// before its first step (a chain of loads: page number, page).
+constexpr int kStartUnits = 2;
+__device__ __forceinline__ int item_units(const KvAttendArgs& a, int steps) { return ((steps - 1) >> a.unit_shift) + 1 + kStartUnits; }
+__device__ __forceinline__ int seq_units(const KvAttendArgs& a, const KvSeq& s, int rows, int step_keys) {
+  return row_blocks(s, a.group, rows) * a.c.heads * item_units(a, item_steps(s, step_keys));
 }
 
 // Item of a warp's last segment.
@@ -133,8 +124,8 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
   __shared__ __align__(8) uint64_t s_bar[kWarps * C::kStages];
   // scales of K of the step's halves (-1: no page), log2 of those of V
   __shared__ __align__(16) float s_scale[kWarps * C::kStages][4];
-  // the first step of the item that a warp's last, and (where it had several) its first segment is of; -1: whole items only
-  __shared__ int64_t s_last[kWarps], s_head[kWarps];
+  // the first unit of the item that a warp's last, and (where it had several) its first segment is of; -1: whole items only
+  __shared__ int s_last[kWarps], s_head[kWarps];
   __shared__ bool s_single[kWarps];
   __shared__ Segment s_item[kLone ? 1 : kWarps];
   __shared__ float s_m[C::kRows], s_l[C::kRows];
@@ -163,9 +154,8 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
   // 64: in the first the halves of every other four lines are exchanged.
   const uint32_t flip = W == 64 && D == 64 ? 64u : 0u;
 
-  // ---- what this warp has to do: steps [pos, end) of the call's (of the item's) ----
-  int64_t pos, end, at = 0, cta_lo = 0, cta_hi = 0, total = 0;
-  int ctas = 0;
+  // ---- what this warp has to do: units [pos, end) of the call's (kLone: steps of the item's) ----
+  int pos, end, at = 0, cta_lo = 0, cta_hi = 0, share = 1;
   int seq = 0, lone_row0 = 0, lone_head = 0;
   KvSeq s;
   int steps, items;
@@ -183,14 +173,14 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
     lone_row0 = static_cast<int>(token0) * a.group;
     steps = item_steps(s, kStepKeys);
     items = 1;
-    const int w = rank * kWarps + warp, n = a.n_split * kWarps;
-    pos = static_cast<int64_t>(steps) * w / n;
-    end = static_cast<int64_t>(steps) * (w + 1) / n;
+    const int w = rank * kWarps + warp, n = a.n_split * kWarps, each = steps / n, rest = steps - each * n;
+    pos = each * w + min(w, rest);
+    end = pos + each + (w < rest ? 1 : 0);
   } else {
     // by every warp for itself: 32 sequences at a time, the first of which stay in registers
     const KvSeq mine = lane < a.c.batch ? kv_seq(a.c, lane) : KvSeq{0, 0, 0, false};
-    const int64_t units = seq_units(a, mine, C::kRows, kStepKeys);
-    total = units;
+    const int units = seq_units(a, mine, C::kRows, kStepKeys);
+    int total = units;
     bool bad = mine.bad;
 #pragma unroll 4
     for (int b = 32 + lane; b < a.c.batch; b += 32) {
@@ -198,28 +188,29 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       bad = bad || x.bad;
       total += seq_units(a, x, C::kRows, kStepKeys);
     }
-    total = warp_sum(total);
+    total = __reduce_add_sync(0xffffffffu, total);
     if (bad && blockIdx.x == 0 && warp == 0) report_bad_index(a.c);
-    ctas = workers_of(total, gridDim.x);
     if (threadIdx.x == 0) a.records[blockIdx.x].first_cta = -1;
-    if (static_cast<int>(blockIdx.x) >= ctas) return;
-    cta_lo = share_start(total, ctas, blockIdx.x);
-    cta_hi = share_start(total, ctas, blockIdx.x + 1);
-    pos = cta_lo + (cta_hi - cta_lo) * warp / kWarps;
-    end = cta_lo + (cta_hi - cta_lo) * (warp + 1) / kWarps;
+    share = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+    if (static_cast<int>(blockIdx.x) * static_cast<int64_t>(share) >= total) return;
+    cta_lo = blockIdx.x * share;
+    cta_hi = min(cta_lo + share, total);
+    const int each = (cta_hi - cta_lo) / kWarps, rest = (cta_hi - cta_lo) % kWarps;
+    pos = cta_lo + each * warp + min(warp, rest);
+    end = pos + each + (warp < rest ? 1 : 0);
     // The sequence that pos is in.  (A warp without steps may stand behind the last one: it looks where the CTA begins.)
-    const int64_t from = pos < end ? pos : cta_lo;
+    const int from = pos < end ? pos : cta_lo;
     for (int b0 = 0;; b0 += 32) {
       KvSeq x = mine;
-      int64_t u = units;
+      int u = units;
       if (b0 > 0) {
         x = b0 + lane < a.c.batch ? kv_seq(a.c, b0 + lane) : KvSeq{0, 0, 0, false};
         u = seq_units(a, x, C::kRows, kStepKeys);
       }
-      int64_t sum = u;
+      int sum = u;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+        const int y = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += y;
       }
       const uint32_t past = __ballot_sync(0xffffffffu, at + sum > from);
@@ -239,42 +230,42 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
   }
 
   // This CTA has the last part of an item that begins at `item_at`: what the combining kernel needs to know.
-  auto put_record = [&](int64_t item_at, int first, int row0, int n_rows, int h) {
-    a.records[blockIdx.x] = {static_cast<int>(share_of(total, ctas, item_at + kStartSteps)), first, row0, n_rows, h};
+  auto put_record = [&](int item_at, int first, int row0, int n_rows, int h) {
+    a.records[blockIdx.x] = {(item_at + kStartUnits) / share, first, row0, n_rows, h};
   };
 
   int stage = 0;
   uint32_t phase = 0;
-  int64_t last_item = -1, head_item = -1;
+  int last_item = -1, head_item = -1;
   bool single = false;
   bool first = true;
   while (pos < end) {
     int h, row0, n_rows, step0, step1;
-    int64_t item_at, item_end;
+    int item_at, item_end;
     if constexpr (kLone) {
       h = lone_head;
       row0 = lone_row0;
       n_rows = min(a.block_tokens * a.group, s.n * a.group - row0);
       item_at = 0;
       item_end = steps;
-      step0 = static_cast<int>(pos);
-      step1 = static_cast<int>(end);
+      step0 = pos;
+      step1 = end;
     } else {
-      const int units = steps + kStartSteps;
-      if (pos >= at + static_cast<int64_t>(items) * units) {             // the next sequence that has items
-        at += static_cast<int64_t>(items) * units;
+      const int units = item_units(a, steps);
+      if (pos >= at + items * units) {                     // the next sequence that has items
+        at += items * units;
         s = kv_seq(a.c, ++seq);
         steps = item_steps(s, kStepKeys);
         items = row_blocks(s, a.group, C::kRows) * a.c.heads;
         continue;
       }
-      const int item = static_cast<int>((pos - at) / units);
-      item_at = at + static_cast<int64_t>(item) * units;
+      const int item = (pos - at) / units;
+      item_at = at + item * units;
       item_end = item_at + units;
       // a share that ends before the item's first step leaves the item to the next
-      if (end - item_at <= kStartSteps) break;
-      step0 = max(0, static_cast<int>(pos - item_at) - kStartSteps);
-      step1 = static_cast<int>(min(item_end, end) - item_at) - kStartSteps;
+      if (end - item_at <= kStartUnits) break;
+      step0 = max(0, pos - item_at - kStartUnits) << a.unit_shift;
+      step1 = min(steps, (min(item_end, end) - item_at - kStartUnits) << a.unit_shift);
       const int rb = item / a.c.heads;
       h = item - rb * a.c.heads;
       row0 = rb * C::kRows;
@@ -372,11 +363,12 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       const float kd = __shfl_sync(0xffffffffu, kd_of, src), vd = __shfl_sync(0xffffffffu, vd_of, src);
       if (lane < 4) s_scale[warp * C::kStages + st][lane] = (lane & 2) ? fmaxf(__log2f(vd), kLog2Least) : (key < vis ? kd : -1.f);
     };
+    // (Code that runs once a launch is kept short: its instructions have to be fetched past the pages that are being read.)
     {
       int st = stage;
-#pragma unroll
-      for (int i = 0; i < C::kStages; ++i) {              // at most 32 pages: one batch
-        if (step0 + i < last) copy(step0 + i, st);
+#pragma unroll 1
+      for (int i = step0; i < min(step0 + C::kStages, last); ++i) {      // at most 32 pages: one batch
+        copy(i, st);
         if (++st == C::kStages) st = 0;
       }
     }
@@ -435,9 +427,9 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
     }
     {
       int st = stage;
-#pragma unroll
-      for (int i = 0; i < C::kStages; ++i) {
-        if (step0 + i < last) put_scales(step0 + i, st);
+#pragma unroll 1
+      for (int i = step0; i < min(step0 + C::kStages, last); ++i) {
+        put_scales(i, st);
         if (++st == C::kStages) st = 0;
       }
       __syncwarp();
@@ -625,7 +617,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
     }
     const bool alone = !kLone && step0 == 0 && step1 == steps;           // the item is this warp's
     // this is not its last segment
-    const bool more = !kLone && item_end < end && (end - item_end > kStartSteps);
+    const bool more = !kLone && item_end < end && end - item_end > kStartUnits;
     // Where the sums go: to O; to the ring, which is idle once the last segment is through, to be put together with those of the
     // CTA's other warps; or, of a first segment that others began, to the workspace.
     float* part = nullptr;
@@ -768,43 +760,38 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
     s_head[warp] = head_item;
     s_single[warp] = single;
     if (last_item >= 0) {                                  // `s` and `steps` are those of the last segment
-      const int units = steps + kStartSteps, item = static_cast<int>((last_item - at) / units), rb = item / a.c.heads;
+      const int units = item_units(a, steps), item = (last_item - at) / units, rb = item / a.c.heads;
       s_item[warp] = {s.first, rb * C::kRows, min(C::kRows, s.n * a.group - rb * C::kRows), item - rb * a.c.heads,
-                      last_item + kStartSteps >= cta_lo, last_item + units <= cta_hi};
+                      last_item + kStartUnits >= cta_lo, last_item + units <= cta_hi};
     }
   }
   __syncthreads();
-  for (int w = 0; w < kWarps; ++w) {
-    const int64_t item = s_last[w];
-    if (item < 0) continue;
-    if (s_single[w]) {                                     // begun by an earlier warp?
-      int x = w - 1;
-      while (x >= 0 && s_last[x] < 0 && s_head[x] < 0) --x;               // warps without steps, or with whole items only
-      if (x >= 0 && s_last[x] == item) continue;
-    }
-    int to = w + 1, heads_from = -1;
-    for (; to < kWarps; ++to) {
-      if (s_last[to] < 0 && s_head[to] < 0) continue;
-      if (s_single[to] && s_last[to] == item) continue;
-      if (s_head[to] == item) heads_from = to;
-      break;
-    }
+  // lane x holds what warp x has
+  const int last_of = lane < kWarps ? s_last[lane] : -1, head_of = lane < kWarps ? s_head[lane] : -1;
+  const bool single_of = lane < kWarps && s_single[lane];
+  const uint32_t with_parts = __ballot_sync(0xffffffffu, last_of >= 0 || head_of >= 0), before = with_parts & ((1u << lane) - 1u);
+  const int previous = __shfl_sync(0xffffffffu, last_of, before != 0u ? 31 - __clz(before) : lane);
+  uint32_t starts = __ballot_sync(0xffffffffu, last_of >= 0 && !(single_of && before != 0u && previous == last_of));
+  for (; starts != 0u; starts &= starts - 1u) {
+    const int w = __ffs(starts) - 1, item = __shfl_sync(0xffffffffu, last_of, w);
+    const uint32_t members = __ballot_sync(0xffffffffu, last_of == item && lane >= w && (lane == w || single_of));
+    const uint32_t heads = __ballot_sync(0xffffffffu, head_of == item && lane > w);
     const Segment it = s_item[w];
     if (!it.begins && it.ends && threadIdx.x == 0) put_record(item, it.first, it.row0, it.n_rows, it.head);
     float* const part = a.partial + (2ll * blockIdx.x + (it.begins ? 1 : 0)) * (C::kRows * (D + 2));
-    const float* const head = a.partial + (2ll * gridDim.x + static_cast<int64_t>(blockIdx.x) * kWarps + heads_from) * (C::kRows * (D + 2));
-    for (int i = threadIdx.x; i < C::kRows * (W / 4); i += 32 * kWarps) {
+    const float* const head = a.partial + (2ll * gridDim.x + static_cast<int64_t>(blockIdx.x) * kWarps + (__ffs(heads) - 1)) * (C::kRows * (D + 2));
+    for (int i = threadIdx.x; i < it.n_rows * (W / 4); i += 32 * kWarps) {
       const int r = i / (W / 4), col = 4 * (i % (W / 4));
-      if (r >= it.n_rows || col >= D) continue;
-      float m = -INFINITY, mh = -INFINITY, l = 0.f, lh = 0.f, mw[kWarps];
+      if (col >= D) continue;
+      float mw[kWarps], mh = -INFINITY, lh = 0.f, m = -INFINITY, l = 0.f;
       uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (heads_from >= 0) {
+      if (heads != 0u) {
         mh = ld_global(head + C::kRows * D + r);
         lh = ld_global(head + C::kRows * (D + 1) + r);
         u = ld_global(reinterpret_cast<const uint4*>(head + r * D + col));
       }
 #pragma unroll
-      for (int x = 0; x < kWarps; ++x) mw[x] = x >= w && x < to && s_last[x] == item ? part_of(x)[C::kRows * C::kORow + r] : -INFINITY;
+      for (int x = 0; x < kWarps; ++x) mw[x] = members >> x & 1u ? part_of(x)[C::kRows * C::kORow + r] : -INFINITY;
 #pragma unroll
       for (int x = 0; x < kWarps; ++x) m = fmaxf(m, mw[x]);
       m = fmaxf(m, mh);
@@ -816,12 +803,11 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       };
 #pragma unroll
       for (int x = 0; x < kWarps; ++x) {
-        if (mw[x] == -INFINITY) continue;
+        if (!(members >> x & 1u)) continue;
         const float* p = part_of(x);
         add(mw[x], p[C::kRows * C::kORow + C::kRows + r], *reinterpret_cast<const float4*>(p + r * C::kORow + col));
       }
-      if (heads_from >= 0)
-        add(mh, lh, make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w)));
+      add(mh, lh, make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w)));
       if (it.begins && it.ends) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int row = it.row0 + r, token = row / a.group;
@@ -1004,6 +990,11 @@ cudaError_t launch_kv_attend(const CUtensorMap& tk, const CUtensorMap& tv, KvAtt
   a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + records_bytes(sms));
   const int rows = block_rows(z);
   a.n_split = lone_split(z, sms);
+  // units of all items together are a 31-bit number
+  const int step_keys = kv_step_keys(width_of(a.c.head_dim));
+  const double items = (static_cast<double>(z.tokens) * a.group / rows + z.batch) * z.heads;
+  a.unit_shift = 0;
+  while (items * ((static_cast<double>(z.keys_most) / step_keys) / (1 << a.unit_shift) + 2 + kStartUnits) > 1e9 && a.unit_shift < 30) ++a.unit_shift;
   a.block_tokens = rows / a.group;
   switch (width_of(a.c.head_dim)) {
     case 64:
