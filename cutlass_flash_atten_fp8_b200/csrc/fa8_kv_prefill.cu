@@ -87,6 +87,7 @@ struct Shared {
   Item item[kItemSlots];                 // seq < 0: no more
   uint32_t factor[C::kRaw][C::kGroups];  // fp16 pair to multiply a group of 16 keys by
   int valid[C::kRaw];                    // rows of the tile that are keys
+  int complete[C::kRaw];                 // all are, and of pages that exist
   float residual[kBlockSlots][2][C::kGroups];   // of K and V; K's is -1 for a group without a page
   float ref[kBlockSlots][2];             // reference scales of the item that the block is of
   int flagged[kBlockSlots];              // some residual is not 1
@@ -223,6 +224,7 @@ __device__ __forceinline__ float exponentials(uint32_t t_s, float c, float nm, i
 }
 
 // Largest c s + log2(scale of V) over 64 keys.
+template <bool kGeneral>
 __device__ __noinline__ float half_max(uint32_t t_s, float c, int lim, const float* rk, const float* rv) {
   float m = -INFINITY;
 #pragma unroll 1
@@ -231,11 +233,21 @@ __device__ __noinline__ float half_max(uint32_t t_s, float c, int lim, const flo
     tmem_ld_32x32b_x32(t_s + 32 * q, s);
     tmem_wait_ld();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int grp = (32 * q + i) >> 4;
-      const float k = rk[grp];
-      const float x = fmaf(__uint_as_float(s[i]), c * k, fmaxf(__log2f(rv[grp]), kLog2Least));
-      if (32 * q + i < lim && k != -1.f) m = fmaxf(m, x);
+    for (int h = 0; h < 2; ++h) {
+      float x = -INFINITY;
+      if (kGeneral) {
+        const float k = rk[2 * q + h];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float y = __uint_as_float(s[16 * h + i]) * (c * k);
+          if (32 * q + 16 * h + i < lim && k != -1.f) x = fmaxf(x, y);
+        }
+        m = fmaxf(m, x + fmaxf(__log2f(rv[2 * q + h]), kLog2Least));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x = fmaxf(x, __uint_as_float(s[16 * h + i]));
+        m = fmaxf(m, x * c);
+      }
     }
   }
   return m;
@@ -290,6 +302,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
   // rows of 64 bytes lie two to a swizzled line of 128: the halves of every other four lines are exchanged
   const uint32_t flip = W == 64 && a.c.head_dim == 64 ? 64u : 0u;
   const int group = a.group, tile_tokens = kTileM / group;       // a token's rows lie in one tile
+  const int over_group = (65536 + group - 1) / group;            // r / group = (r * over_group) >> 16 for r < 128
   // Consumers of the item ring: the next item (false: no more, or a wait ran out).
   int n_items = 0;
   auto next_item = [&](Item& it) {
@@ -404,13 +417,17 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         const int box_keys = kv_box_keys(W, 1 << a.c.page_shift);
         const bool issues = here && (16 * lane) % box_keys == 0;
         const int boxes = __popc(__ballot_sync(0xffffffffu, issues));
+        const bool all_here = __all_sync(0xffffffffu, here || lane >= C::kGroups);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const int st = tiles % C::kRaw;
           ok = __all_sync(0xffffffffu, wait_bounded(wctx, &sh.raw_empty[st], ((tiles / C::kRaw) & 1) ^ 1, 0xb300 + st));
           if (!ok) break;
           if (lane < C::kGroups) sh.factor[st][lane] = here ? (kv ? fv : fk) : 0u;
-          if (lane == 0) sh.valid[st] = max(0, min(C::kN, it.vis - blk * C::kN));
+          if (lane == 0) {
+            sh.valid[st] = max(0, min(C::kN, it.vis - blk * C::kN));
+            sh.complete[st] = all_here && it.vis >= (blk + 1) * C::kN;
+          }
           __syncwarp();
           const uint32_t bar = smem_u32(&sh.raw_full[st]);
           if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_keys * C::kRawRow * C::kRawBlocks);
@@ -573,21 +590,28 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         if (!ok) break;
         const int valid = sh.valid[st];
         const uint32_t src = s_raw + st * C::kRawBytes, dst = s_ring + rg * C::kRingBytes;
-        // a warp takes eight rows and 64 columns at a time: eight lanes side by side read and write eight rows of one
-        // 16-byte column, which the swizzles spread over all banks
-        constexpr int kParts = (C::kN / 8) * C::kCols;
-#pragma unroll 4
-        for (int p = w; p < kParts; p += 4) {
-          const int cb = p % C::kCols, r = (p / C::kCols) * 8 + (lane & 7), q = lane >> 3;
-          uint32_t from;
-          if constexpr (W == 64) from = src + ((r * 64 + ((q ^ ((r >> 1) & 3)) << 4)) ^ ((r & 8) ? flip : 0u));
-          else from = src + (cb >> 1) * C::kRawBlockBytes + r * 128 + (((4 * (cb & 1) + q) ^ (r & 7)) << 4);
-          uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
-          const uint32_t f = sh.factor[st][r >> 4];
-          if (r < valid && f != 0u) widen16<kE5M2>(ld_shared16(from), f, lo, hi);
+        // A warp takes eight rows and 64 columns at a time: eight lanes side by side read and write eight rows of one 16-byte
+        // column, which the swizzles spread over all banks.  All its loads go out before the first is used.
+        constexpr int kParts = (C::kN / 8) * C::kCols, kMine = kParts / 4;
+        const int q = lane >> 3, r8 = lane & 7;
+        uint4 x[kMine];
+        uint32_t f[kMine];
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+          const int p = w + 4 * k, cb = p % C::kCols, r = (p / C::kCols) * 8 + r8;
+          if constexpr (W == 64) x[k] = ld_shared16(src + ((r * 64 + ((q ^ ((r >> 1) & 3)) << 4)) ^ ((r & 8) ? flip : 0u)));
+          else x[k] = ld_shared16(src + (cb >> 1) * C::kRawBlockBytes + r * 128 + (((4 * (cb & 1) + q) ^ r8) << 4));
+          f[k] = sh.factor[st][r >> 4];
+        }
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+          const int p = w + 4 * k, cb = p % C::kCols, r = (p / C::kCols) * 8 + r8;
+          uint4 lo, hi;
+          widen16<kE5M2>(x[k], f[k], lo, hi);
+          if (!sh.complete[st] && (r >= valid || f[k] == 0u)) lo = hi = make_uint4(0u, 0u, 0u, 0u);
           const uint32_t to = dst + cb * (C::kN * 128) + r * 128;
-          st_shared16(to + (((2 * q) ^ (r & 7)) << 4), lo);
-          st_shared16(to + (((2 * q + 1) ^ (r & 7)) << 4), hi);
+          st_shared16(to + (((2 * q) ^ r8) << 4), lo);
+          st_shared16(to + (((2 * q + 1) ^ r8) << 4), hi);
         }
         fence_proxy_async_smem();                                // what was written is for the products to read
         __syncwarp();
@@ -621,22 +645,26 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       }
       const int D = a.c.head_dim;
       // ---- Q: this warp's 32 rows into shared memory, fp16 ----
+      constexpr int kLanes = W / 8, kRowsAt = 32 / kLanes;       // lanes of a row (8 columns each), rows at a time
+      const int my_col = lane % kLanes, my_row = 32 * sub + lane / kLanes;
       float back = 1.f;
       {
-        constexpr int kLanes = W / 8, kRowsAt = 32 / kLanes;     // lanes of a row (8 columns each), rows at a time
-        const int col = 8 * (lane % kLanes);
-#pragma unroll 4
-        for (int r0 = 0; r0 < 32; r0 += kRowsAt) {
-          const int r = 32 * sub + r0 + lane / kLanes;
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (r < n_rows && col < D) {
-            const int64_t token = it.first + tok0 + r / group;
-            const int head = it.head * group + r % group;
-            x = ld_global(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q.x) + token * a.q.token_stride + head * a.q.head_stride + col));
-          }
+        uint4 x[32 / kRowsAt];                                   // all of them under way at once
+        const uint16_t* const q0 = static_cast<const uint16_t*>(a.q.x) + (static_cast<int64_t>(it.first) + tok0) * a.q.token_stride +
+                                   static_cast<int64_t>(it.head) * group * a.q.head_stride + 8 * my_col;
+#pragma unroll
+        for (int k = 0; k < 32 / kRowsAt; ++k) {
+          const int r = my_row + k * kRowsAt, token = (r * over_group) >> 16;
+          x[k] = make_uint4(0u, 0u, 0u, 0u);
+          if (r < n_rows && 8 * my_col < D)
+            x[k] = ld_global(reinterpret_cast<const uint4*>(q0 + token * a.q.token_stride + (r - token * group) * a.q.head_stride));
+        }
+#pragma unroll
+        for (int k = 0; k < 32 / kRowsAt; ++k) {
+          const int r = my_row + k * kRowsAt;
           if (a.bf16) {
             float big = 0.f;
-            uint32_t v[4] = {x.x, x.y, x.z, x.w};
+            uint32_t v[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float2 f = half_pair<true>(v[e] & 0x7fff7fffu);
@@ -648,19 +676,18 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
             const float f = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
             const float g = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 y = half_pair<true>(v[k]);
-              v[k] = pack_half2(y.x * f, y.y * f);
+            for (int i = 0; i < 4; ++i) {
+              const float2 y = half_pair<true>(v[i]);
+              v[i] = pack_half2(y.x * f, y.y * f);
             }
-            x = make_uint4(v[0], v[1], v[2], v[3]);
+            x[k] = make_uint4(v[0], v[1], v[2], v[3]);
 #pragma unroll
-            for (int k = 0; k < kRowsAt; ++k) {
-              const float y = __shfl_sync(0xffffffffu, g, k * kLanes);
-              if (lane == r0 + k) back = y;
+            for (int i = 0; i < kRowsAt; ++i) {
+              const float y = __shfl_sync(0xffffffffu, g, i * kLanes);
+              if (lane == k * kRowsAt + i) back = y;
             }
           }
-          const int c = lane % kLanes;
-          st_shared16(s_q + tile * C::kQBytes + (c >> 3) * (kTileM * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), x);
+          st_shared16(s_q + tile * C::kQBytes + (my_col >> 3) * (kTileM * 128) + r * 128 + (((my_col & 7) ^ (r & 7)) << 4), x[k]);
         }
       }
       fence_proxy_async_smem();
@@ -670,7 +697,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       const int r = 32 * sub + lane;
       Row row{};
       row.m = -INFINITY;
-      const int my_token = tok0 + min(r, n_rows - 1) / group;
+      const int my_token = tok0 + ((min(r, n_rows - 1) * over_group) >> 16);
       row.lim = a.causal ? max(0, min(it.len, it.len - it.n + my_token + 1)) : it.len;
       const int least = a.causal ? max(0, min(it.len, it.len - it.n + tok0 + 1)) : it.len;       // of the tile's first row
       float vref = 1.f;
@@ -693,7 +720,8 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           // the exact maximum of the first block
           float m = -INFINITY;
           for (int half = 0; half < C::kHalves; ++half)
-            m = fmaxf(m, half_max(t_s + 64 * half, row.c, row.lim - key0 - 64 * half, &sh.residual[n][0][4 * half], &sh.residual[n][1][4 * half]));
+            m = fmaxf(m, general ? half_max<true>(t_s + 64 * half, row.c, row.lim - key0 - 64 * half, &sh.residual[n][0][4 * half], &sh.residual[n][1][4 * half])
+                                 : half_max<false>(t_s + 64 * half, row.c, 0, nullptr, nullptr));
           row.m = m - kHeadroom;
           row.nm = m == -INFINITY ? 0.f : -row.m;
           row.most = m == -INFINITY ? 0.f : kRaiseAbove;
@@ -710,7 +738,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           if (__any_sync(0xffffffffu, !(sum <= row.most))) {
             // Some row has outgrown its reference (or holds a NaN): take this half's maximum in, and rescale O, for which the
             // products before have to be done: those before this block's scores are, where the scores came after them.
-            const float top = half_max(ts, row.c, lim, rk, rv);
+            const float top = half_max<true>(ts, row.c, lim, rk, rv);
             const float m = sum <= row.most ? row.m : fmaxf(row.m, top - kHeadroom);
             const float nm = m == -INFINITY ? 0.f : -m;
             const float alpha = row.m == -INFINITY ? 0.f : ex2_approx(nm - row.nm);
@@ -756,7 +784,9 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       tc_fence_after();
       const bool whole = plan.parts == 1;
       const float inv = (row.l == 0.f ? 0.f : (whole ? 1.f / row.l : 1.f)) * vref;
-      const int64_t out_row = (static_cast<int64_t>(it.first) + tok0 + r / group) * a.heads_q + it.head * group + r % group;
+      const int token = (r * over_group) >> 16;
+      const int64_t row0 = (static_cast<int64_t>(it.first) + tok0) * a.heads_q + it.head * group;
+      const int64_t out_row = row0 + token * a.heads_q + (r - token * group);
       if (r < n_rows) {
         if (whole) {
           if (a.lse != nullptr) a.lse[out_row] = row.l == 0.f ? -INFINITY : (row.m + __log2f(row.l)) * 0.6931471805599453f;
@@ -800,15 +830,12 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       tc_fence_before();
       if (whole) {
         __syncwarp();
-        constexpr int kLanes = W / 8, kRowsAt = 32 / kLanes;
-        const int ch = lane % kLanes;
-#pragma unroll 4
-        for (int r0 = 0; r0 < 32; r0 += kRowsAt) {
-          const int q = 32 * sub + r0 + lane / kLanes;
-          if (q < n_rows && 8 * ch < D) {
-            const uint4 v = ld_shared16(stage + (ch >> 3) * (kTileM * 128) + q * 128 + (((ch & 7) ^ (q & 7)) << 4));
-            const int64_t orow = (static_cast<int64_t>(it.first) + tok0 + q / group) * a.heads_q + it.head * group + q % group;
-            st_global_v4(static_cast<uint16_t*>(a.o) + orow * D + 8 * ch, v.x, v.y, v.z, v.w);
+#pragma unroll 8
+        for (int k = 0; k < 32 / kRowsAt; ++k) {
+          const int q = my_row + k * kRowsAt, t = (q * over_group) >> 16;
+          if (q < n_rows && 8 * my_col < D) {
+            const uint4 v = ld_shared16(stage + (my_col >> 3) * (kTileM * 128) + q * 128 + (((my_col & 7) ^ (q & 7)) << 4));
+            st_global_v4(static_cast<uint16_t*>(a.o) + (row0 + t * a.heads_q + (q - t * group)) * D + 8 * my_col, v.x, v.y, v.z, v.w);
           }
         }
         __syncwarp();
