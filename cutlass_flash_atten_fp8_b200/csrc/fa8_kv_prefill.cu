@@ -43,7 +43,7 @@ template <int W>
 struct PCfg {
   static constexpr int kTiles = W == 256 ? 1 : 2;
   static constexpr int kN = W == 256 ? 64 : 128;               // keys of a block
-  static constexpr int kHalves = kN / 64;
+  static constexpr int kSub = kN / 64;                         // sub-blocks of 64 keys, which scores and P come in
   static constexpr int kGroups = kN / 16;                      // of keys that share a page
   static constexpr int kCols = W / 64;                         // column blocks of 64 fp16 (128 bytes)
   static constexpr int kRawRow = W < 128 ? W : 128;            // bytes of a row of a raw (fp8) tile
@@ -54,7 +54,8 @@ struct PCfg {
   static constexpr int kRing = 4;                              // widened tiles
   static constexpr int kRingBytes = kN * W * 2;
   static constexpr int kQBytes = kTileM * W * 2;               // of a tile
-  static constexpr int kOCol = W == 256 ? 128 : 256;           // O of tile i at kOCol + W i; S at 128 i, or 64 b
+  // Columns of tensor memory: a tile's two score buffers of 64 (P over them), then its O.
+  static constexpr int kTileCols = 128 + W;
   static constexpr int kSoftWarps = 4 * kTiles;
   static constexpr int kWideWarp0 = kSoftWarps;
   static constexpr int kLoadWarp = kWideWarp0 + 4;
@@ -63,7 +64,7 @@ struct PCfg {
   static constexpr int kRawOffset = kTiles * kQBytes;
   static constexpr int kRingOffset = kRawOffset + kRaw * kRawBytes;
   static constexpr int kSharedOffset = kRingOffset + kRing * kRingBytes;
-  static_assert(kOCol + W * kTiles <= 512, "tensor memory");
+  static_assert(kTileCols * kTiles <= 512, "tensor memory");
 };
 
 struct Item {
@@ -81,7 +82,7 @@ struct Shared {
   uint64_t item_full[kItemSlots], item_empty[kItemSlots];
   uint64_t raw_full[C::kRaw], raw_empty[C::kRaw];
   uint64_t ring_full[C::kRing], ring_empty[C::kRing];
-  uint64_t q_full[2], s_full[2], p_full[2][2], o_half[2], o_final[2];
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2], o_final[2];     // by tile, and score buffer
   uint64_t blk_full[kBlockSlots];
   uint64_t drain;
   Item item[kItemSlots];                 // seq < 0: no more
@@ -175,47 +176,39 @@ struct Row {
   int lim;                               // keys that the row sees
 };
 
-// P of 64 keys (tensor-memory columns t_s ... t_s + 63) into pk, fp16 pairs; returns the sum of P and adds that of the
-// denominators to *l.  General: keys from `lim` on (counted from the first of these) are masked, residual scales are multiplied in.
+// P of 32 keys from their scores s, into pk as fp16 pairs; returns the sum of P and adds that of the denominators to *l.  General:
+// keys from `lim` on are masked, the residual scales of the two groups of sixteen keys are multiplied in.
 template <bool kGeneral>
-__device__ __forceinline__ float exponentials(uint32_t t_s, float c, float nm, int lim, const float* rk, const float* rv, uint32_t (&pk)[32],
-                                              float* l) {
-  f32x2_t sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-  float sum_p = 0.f, sum_l = 0.f;
-  const f32x2_t c2 = pack2(c, c), nm2 = pack2(nm, nm);
+__device__ __forceinline__ float exponentials(const uint32_t (&s)[32], float c, float nm, int lim, const float* rk, const float* rv,
+                                              uint32_t* pk, float* l) {
+  if (kGeneral) {
+    float sum = 0.f, sum_l = 0.f;
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    uint32_t s[32];
-    tmem_ld_32x32b_x32(t_s + 32 * q, s);
-    tmem_wait_ld();
-    if (kGeneral) {
+    for (int h = 0; h < 2; ++h) {
+      const float k = rk[h], v = rv[h], ck = c * k;
 #pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        const int grp = (32 * q + i) >> 4;
-        const float k = rk[grp], v = rv[grp], ck = c * k;
+      for (int i = 16 * h; i < 16 * h + 16; i += 2) {
         float x0 = fmaf(__uint_as_float(s[i]), ck, nm), x1 = fmaf(__uint_as_float(s[i + 1]), ck, nm);
-        if (32 * q + i >= lim || k == -1.f) x0 = -INFINITY;
-        if (32 * q + i + 1 >= lim || k == -1.f) x1 = -INFINITY;
-        const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
+        if (i >= lim || k == -1.f) x0 = -INFINITY;
+        if (i + 1 >= lim || k == -1.f) x1 = -INFINITY;
+        const float e0 = ex2_approx(x0), e1 = ex2_approx(x1), p0 = e0 * v, p1 = e1 * v;
         sum_l += e0 + e1;
-        const float p0 = e0 * v, p1 = e1 * v;
-        sum_p += p0 + p1;
-        pk[16 * q + i / 2] = pack_half2(p0, p1);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        float x0, x1;
-        unpack2(fma2(pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, nm2), x0, x1);
-        const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
-        sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pack2(e0, e1));
-        pk[16 * q + i / 2] = pack_half2(e0, e1);
+        sum += p0 + p1;
+        pk[i / 2] = pack_half2(p0, p1);
       }
     }
-  }
-  if (kGeneral) {
     *l += sum_l;
-    return sum_p;
+    return sum;
+  }
+  f32x2_t sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+  const f32x2_t c2 = pack2(c, c), nm2 = pack2(nm, nm);
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    float x0, x1;
+    unpack2(fma2(pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, nm2), x0, x1);
+    const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
+    sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pack2(e0, e1));
+    pk[i / 2] = pack_half2(e0, e1);
   }
   float a, b;
   unpack2(add2(sum[0], sum[1]), a, b);
@@ -223,34 +216,40 @@ __device__ __forceinline__ float exponentials(uint32_t t_s, float c, float nm, i
   return a + b;
 }
 
-// Largest c s + log2(scale of V) over 64 keys.
+// Largest c s + log2(scale of V) of 32 keys.
 template <bool kGeneral>
-__device__ __noinline__ float half_max(uint32_t t_s, float c, int lim, const float* rk, const float* rv) {
+__device__ __forceinline__ float largest(const uint32_t (&s)[32], float c, int lim, const float* rk, const float* rv) {
   float m = -INFINITY;
-#pragma unroll 1
-  for (int q = 0; q < 2; ++q) {
-    uint32_t s[32];
-    tmem_ld_32x32b_x32(t_s + 32 * q, s);
-    tmem_wait_ld();
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float x = -INFINITY;
-      if (kGeneral) {
-        const float k = rk[2 * q + h];
+  for (int h = 0; h < 2; ++h) {
+    float x = -INFINITY;
+    if (kGeneral) {
+      const float k = rk[h];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float y = __uint_as_float(s[16 * h + i]) * (c * k);
-          if (32 * q + 16 * h + i < lim && k != -1.f) x = fmaxf(x, y);
-        }
-        m = fmaxf(m, x + fmaxf(__log2f(rv[2 * q + h]), kLog2Least));
-      } else {
+      for (int i = 16 * h; i < 16 * h + 16; ++i)
+        if (i < lim && k != -1.f) x = fmaxf(x, __uint_as_float(s[i]) * (c * k));
+      m = fmaxf(m, x + fmaxf(__log2f(rv[h]), kLog2Least));
+    } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x = fmaxf(x, __uint_as_float(s[16 * h + i]));
-        m = fmaxf(m, x * c);
-      }
+      for (int i = 16 * h; i < 16 * h + 16; ++i) x = fmaxf(x, __uint_as_float(s[i]));
+      m = fmaxf(m, x * c);
     }
   }
   return m;
+}
+
+// Columns of tensor memory times alpha.
+__device__ __noinline__ void rescale(uint32_t t, int columns, float alpha) {
+#pragma unroll 1
+  for (int c = 0; c < columns; c += 16) {
+    uint32_t x[16];
+    tmem_ld_32x32b_x16(t + c, x);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
+    tmem_st_32x32b_x16(t + c, x);
+  }
+  tmem_wait_st();
 }
 
 template <int W, bool kE5M2>
@@ -275,9 +274,9 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     init(sh.ring_full, C::kRing, 4);
     init(sh.ring_empty, C::kRing, 1);
     init(sh.q_full, 2, 4);
-    init(sh.s_full, 2, 1);
+    init(&sh.s_full[0][0], 4, 1);
     init(&sh.p_full[0][0], 4, 4);
-    init(sh.o_half, 2, 1);
+    init(sh.o_done, 2, 1);
     init(sh.o_final, 2, 1);
     init(sh.blk_full, kBlockSlots, 1);
     init(&sh.drain, 1, 1);
@@ -462,105 +461,68 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
   } else if (warp == C::kMmaWarp) {
     // ---------------------------------------------------------------- issuer
     if (elect_one()) {
-      constexpr uint32_t kIdescQK = idesc(C::kN, false), kIdescPV = idesc(W, true);
+      constexpr uint32_t kIdescQK = idesc(64, false), kIdescPV = idesc(W, true);
       constexpr uint32_t kColQ = kTileM * 128 / 16, kColK = C::kN * 128 / 16;     // column blocks of Q and K in 16 bytes
+      constexpr uint32_t kSubRows = 64 * 128 / 16;                                // 64 rows of a column block
       const uint32_t q_lo = desc_lo(s_q, 16), k_lo = desc_lo(s_ring, 16), v_lo = desc_lo(s_ring, C::kN * 128);
       bool ok = true;
       uint32_t ld = 0;                                           // widened tiles used so far: K, V, K, V ...
       uint32_t qn[2] = {0, 0};                                   // q_full phases by tile
-      uint32_t pn[2] = {0, 0};                                   // p_full phases by tile (or score buffer)
+      uint32_t pn[2] = {0, 0};                                   // sub-blocks by tile
       auto ring_wait = [&](uint32_t i) { return wait_bounded(wctx, &sh.ring_full[i % C::kRing], (i / C::kRing) & 1, 0xb400); };
       auto ring_release = [&](uint32_t i) { tc_commit(smem_u32(&sh.ring_empty[i % C::kRing])); };
-      auto issue_qk = [&](int tile, uint32_t col, uint32_t i) {
-        const uint32_t kk = k_lo + (i % C::kRing) * (C::kRingBytes / 16), qq = q_lo + tile * (C::kQBytes / 16);
+      // S of sub-block sb (of widened tile i) into score buffer b.
+      auto issue_qk = [&](int tile, uint32_t b, uint32_t i, int sb) {
+        const uint32_t kk = k_lo + (i % C::kRing) * (C::kRingBytes / 16) + (C::kSub > 1 ? (sb & 1) * kSubRows : 0u), qq = q_lo + tile * (C::kQBytes / 16);
 #pragma unroll
         for (int k = 0; k < W / 16; ++k)
-          mma_f16_ss(tmem + col, desc(qq + (k >> 2) * kColQ + 2 * (k & 3)), desc(kk + (k >> 2) * kColK + 2 * (k & 3)), kIdescQK, k > 0);
+          mma_f16_ss(tmem + C::kTileCols * tile + 64 * b, desc(qq + (k >> 2) * kColQ + 2 * (k & 3)), desc(kk + (k >> 2) * kColK + 2 * (k & 3)), kIdescQK,
+                     k > 0);
+        tc_commit(smem_u32(&sh.s_full[tile][b]));
       };
-      auto issue_pv = [&](int tile, uint32_t col, uint32_t i, int half, bool first) {
-        const uint32_t vv = v_lo + (i % C::kRing) * (C::kRingBytes / 16);
+      auto issue_pv = [&](int tile, uint32_t b, uint32_t i, int sb) {
+        const uint32_t vv = v_lo + (i % C::kRing) * (C::kRingBytes / 16) + (C::kSub > 1 ? (sb & 1) * kSubRows : 0u);
 #pragma unroll
-        for (int k = 4 * half; k < 4 * half + 4; ++k)
-          mma_f16_ts(tmem + C::kOCol + tile * W, tmem + col + 8 * k, desc(vv + k * 128), kIdescPV, !(first && k == 0));
+        for (int k = 0; k < 4; ++k)
+          mma_f16_ts(tmem + C::kTileCols * tile + 128, tmem + C::kTileCols * tile + 64 * b + 8 * k, desc(vv + k * 128), kIdescPV, sb > 0 || k > 0);
+        tc_commit(smem_u32(&sh.o_done[tile]));
       };
       Item it;
       while (ok && (ok = next_item(it))) {
         item_read();
         if (it.seq < 0) break;
-        const int nb = it.blk1 - it.blk0;
+        const int n = (it.blk1 - it.blk0) * C::kSub;
         const int nt = C::kTiles == 2 && it.n_tokens > tile_tokens ? 2 : 1;
-        if constexpr (C::kTiles == 2) {
-          ok = ring_wait(ld);
+        // The scores run two sub-blocks ahead: S(sb + 2) goes into the buffer that P V (sb) has read.
+        for (int sb = -2; sb < n && ok; ++sb) {
+          const uint32_t lv = ld + 2 * (max(sb, 0) / C::kSub) + 1, lk = ld + 2 * ((sb + 2) / C::kSub);
+          const bool qk = sb + 2 < n;
+          if (sb >= 0 && sb % C::kSub == 0) ok = ring_wait(lv);
           for (int i = 0; i < nt && ok; ++i) {
-            ok = wait_bounded(wctx, &sh.q_full[i], qn[i]++ & 1, 0xb500 + i);
-            if (!ok) break;
-            tc_fence_after();
-            issue_qk(i, 128 * i, ld);
-            tc_commit(smem_u32(&sh.s_full[i]));
-          }
-          if (!ok) break;
-          ring_release(ld);
-          for (int j = 0; j < nb && ok; ++j) {
-            const uint32_t lv = ld + 2 * j + 1, lk = lv + 1;
-            const bool more = j + 1 < nb;
-            ok = ring_wait(lv);
-            for (int i = 0; i < nt && ok; ++i) {
-#pragma unroll
-              for (int half = 0; half < C::kHalves; ++half) {
-                if (ok) ok = wait_bounded(wctx, &sh.p_full[i][half], pn[i] & 1, 0xb600 + 2 * i + half);
-                if (!ok) break;
-                tc_fence_after();
-                issue_pv(i, 128 * i, lv, half, j == 0);
-                if (half == 0) tc_commit(smem_u32(&sh.o_half[i]));
-              }
-              if (!ok) break;
-              ++pn[i];
-              if (!more) tc_commit(smem_u32(&sh.o_final[i]));
-              if (more) {
-                if (i == 0) ok = ring_wait(lk);
-                if (!ok) break;
-                tc_fence_after();
-                issue_qk(i, 128 * i, lk);
-                tc_commit(smem_u32(&sh.s_full[i]));
-              }
-            }
-            if (!ok) break;
-            ring_release(lv);
-            if (more) ring_release(lk);
-          }
-        } else {
-          // one tile, score buffers in turn: S(j + 2) follows P V (j) into the buffer that it read
-          ok = wait_bounded(wctx, &sh.q_full[0], qn[0]++ & 1, 0xb500);
-          for (int j = 0; j < 2 && j < nb && ok; ++j) {
-            ok = ring_wait(ld + 2 * j);
-            if (!ok) break;
-            tc_fence_after();
-            issue_qk(0, 64 * ((pn[0] + j) & 1), ld + 2 * j);
-            tc_commit(smem_u32(&sh.s_full[(pn[0] + j) & 1]));
-            ring_release(ld + 2 * j);
-          }
-          for (int j = 0; j < nb && ok; ++j) {
-            const uint32_t lv = ld + 2 * j + 1, b = pn[0] & 1;
-            ok = ring_wait(lv);
-            if (ok) ok = wait_bounded(wctx, &sh.p_full[b][0], (pn[0] >> 1) & 1, 0xb600 + b);
-            if (!ok) break;
-            ++pn[0];
-            tc_fence_after();
-            issue_pv(0, 64 * b, lv, 0, j == 0);
-            tc_commit(smem_u32(&sh.o_half[0]));
-            if (j + 1 == nb) tc_commit(smem_u32(&sh.o_final[0]));
-            ring_release(lv);
-            if (j + 2 < nb) {
-              ok = ring_wait(ld + 2 * j + 4);
+            const uint32_t b = (pn[i] + sb) & 1;
+            if (sb >= 0) {
+              ok = wait_bounded(wctx, &sh.p_full[i][b], ((pn[i] + sb) >> 1) & 1, 0xb600 + 2 * i + b);
               if (!ok) break;
               tc_fence_after();
-              issue_qk(0, 64 * b, ld + 2 * j + 4);
-              tc_commit(smem_u32(&sh.s_full[b]));
-              ring_release(ld + 2 * j + 4);
+              issue_pv(i, b, lv, sb);
+              if (sb + 1 == n) tc_commit(smem_u32(&sh.o_final[i]));
+            } else if (sb == -2) {
+              ok = wait_bounded(wctx, &sh.q_full[i], qn[i]++ & 1, 0xb500 + i);
+              if (!ok) break;
+            }
+            if (qk) {
+              if (i == 0 && (sb + 2) % C::kSub == 0) ok = ring_wait(lk);
+              if (!ok) break;
+              tc_fence_after();
+              issue_qk(i, b, lk, sb + 2);
             }
           }
+          if (!ok) break;
+          if (sb >= 0 && (sb + 1) % C::kSub == 0) ring_release(lv);
+          if (qk && (sb + 3) % C::kSub == 0) ring_release(lk);
         }
-        ld += 2 * nb;
+        for (int i = 0; i < nt; ++i) pn[i] += n;
+        ld += 2 * (it.blk1 - it.blk0);
       }
       {
         // products in flight, and their arrivals, end before tensor and shared memory are freed (with a limit)
@@ -625,9 +587,9 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     // ---------------------------------------------------------------- softmax
     const int tile = warp / 4, sub = warp % 4;                   // rows 32 sub ... of the tile = lanes of tensor memory
     const uint32_t lanes = static_cast<uint32_t>(32 * sub) << 16;
-    const uint32_t t_o = tmem + lanes + C::kOCol + tile * W;
+    const uint32_t t_tile = tmem + lanes + C::kTileCols * tile, t_o = t_tile + 128;
     uint32_t blocks = 0;                                         // of all items (the residual ring), also those this tile sits out
-    uint32_t mine = 0;                                           // blocks this tile took part in
+    uint32_t mine = 0;                                           // sub-blocks this tile took part in
     uint32_t taken = 0;                                          // items this tile took part in
     Item it;
     bool ok = true;
@@ -701,80 +663,77 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       row.lim = a.causal ? max(0, min(it.len, it.len - it.n + my_token + 1)) : it.len;
       const int least = a.causal ? max(0, min(it.len, it.len - it.n + tok0 + 1)) : it.len;       // of the tile's first row
       float vref = 1.f;
-      for (int j = 0; j < nb && ok; ++j, ++blocks, ++mine) {
-        const uint32_t n = blocks % kBlockSlots;
-        const int buf = C::kTiles == 2 ? tile : static_cast<int>(mine & 1);
-        const uint32_t t_s = tmem + lanes + (C::kTiles == 2 ? 128 * tile : 64 * buf);
-        ok = wait_bounded(wctx, &sh.blk_full[n], (blocks / kBlockSlots) & 1, 0xb900);
-        if (ok) ok = wait_bounded(wctx, &sh.s_full[buf], (C::kTiles == 2 ? mine : mine >> 1) & 1, 0xba00 + buf);
+      for (int sb = 0; sb < nb * C::kSub && ok; ++sb, ++mine) {
+        const int j = sb / C::kSub, buf = mine & 1;
+        const uint32_t n = (blocks + j) % kBlockSlots;
+        const uint32_t t_s = t_tile + 64 * buf;
+        if (sb % C::kSub == 0) ok = wait_bounded(wctx, &sh.blk_full[n], ((blocks + j) / kBlockSlots) & 1, 0xb900);
+        if (ok) ok = wait_bounded(wctx, &sh.s_full[tile][buf], (mine >> 1) & 1, 0xba00 + buf);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        if (j == 0) {
+        if (sb == 0) {
           row.c = a.scale_log2 * back * sh.ref[n][0];
           vref = sh.ref[n][1];
         }
-        const int key0 = (it.blk0 + j) * C::kN;
-        const bool general = sh.flagged[n] != 0 || key0 + C::kN > least;
-        if (j == 0) {
-          // the exact maximum of the first block
-          float m = -INFINITY;
-          for (int half = 0; half < C::kHalves; ++half)
-            m = fmaxf(m, general ? half_max<true>(t_s + 64 * half, row.c, row.lim - key0 - 64 * half, &sh.residual[n][0][4 * half], &sh.residual[n][1][4 * half])
-                                 : half_max<false>(t_s + 64 * half, row.c, 0, nullptr, nullptr));
+        const int key0 = it.blk0 * C::kN + 64 * sb, lim = row.lim - key0;
+        const bool general = sh.flagged[n] != 0 || key0 + 64 > least;
+        const float *rk = sh.residual[n][0] + 4 * (sb % C::kSub), *rv = sh.residual[n][1] + 4 * (sb % C::kSub);
+        uint32_t x[2][32], pk[32];
+        auto load = [&] {
+          tmem_ld_32x32b_x32(t_s, x[0]);
+          tmem_ld_32x32b_x32(t_s + 32, x[1]);
+          tmem_wait_ld();
+        };
+        auto top_of = [&](bool g) {
+          return g ? fmaxf(largest<true>(x[0], row.c, lim, rk, rv), largest<true>(x[1], row.c, lim - 32, rk + 2, rv + 2))
+                   : fmaxf(largest<false>(x[0], row.c, 0, nullptr, nullptr), largest<false>(x[1], row.c, 0, nullptr, nullptr));
+        };
+        load();
+        if (sb == 0) {                                           // the exact maximum of the first 64 keys
+          const float m = top_of(general);
           row.m = m - kHeadroom;
           row.nm = m == -INFINITY ? 0.f : -row.m;
           row.most = m == -INFINITY ? 0.f : kRaiseAbove;
         }
-#pragma unroll
-        for (int half = 0; half < C::kHalves; ++half) {
-          uint32_t pk[32];
-          const float* rk = &sh.residual[n][0][4 * half];
-          const float* rv = &sh.residual[n][1][4 * half];
-          const int lim = row.lim - key0 - 64 * half;
-          const uint32_t ts = t_s + 64 * half;
-          float l = 0.f;
-          float sum = general ? exponentials<true>(ts, row.c, row.nm, lim, rk, rv, pk, &l) : exponentials<false>(ts, row.c, row.nm, 0, rk, rv, pk, &l);
-          if (__any_sync(0xffffffffu, !(sum <= row.most))) {
-            // Some row has outgrown its reference (or holds a NaN): take this half's maximum in, and rescale O, for which the
-            // products before have to be done: those before this block's scores are, where the scores came after them.
-            const float top = half_max<true>(ts, row.c, lim, rk, rv);
-            const float m = sum <= row.most ? row.m : fmaxf(row.m, top - kHeadroom);
-            const float nm = m == -INFINITY ? 0.f : -m;
-            const float alpha = row.m == -INFINITY ? 0.f : ex2_approx(nm - row.nm);
-            row.m = m;
-            row.nm = nm;
-            row.most = m == -INFINITY ? 0.f : kRaiseAbove;
-            row.l *= alpha;
-            const bool summed = C::kTiles == 2 ? (j > 0 || half > 0) : j > 0;
-            if (summed) {
-              if (C::kTiles == 2 && half > 0) ok = wait_bounded(wctx, &sh.o_half[tile], mine & 1, 0xbb00);
-              if (C::kTiles == 1) ok = wait_bounded(wctx, &sh.o_half[0], (mine - 1) & 1, 0xbb00);
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              tc_fence_after();
-#pragma unroll 1
-              for (int c = 0; c < W; c += 32) {
-                uint32_t o[32];
-                tmem_ld_32x32b_x32(t_o + c, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                tmem_st_32x32b_x32(t_o + c, o);
-              }
-              tmem_wait_st();
-            }
-            l = 0.f;
-            exponentials<true>(ts, row.c, row.nm, lim, rk, rv, pk, &l);
-          }
-          row.l += l;
-          tmem_st_32x32b_x32(t_s + 32 * half, pk);               // over the scores, two to a column
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[buf][half]));
+        float l = 0.f, sum;
+        if (general) {
+          sum = exponentials<true>(x[0], row.c, row.nm, lim, rk, rv, pk, &l);
+          sum += exponentials<true>(x[1], row.c, row.nm, lim - 32, rk + 2, rv + 2, pk + 16, &l);
+        } else {
+          sum = exponentials<false>(x[0], row.c, row.nm, 0, nullptr, nullptr, pk, &l);
+          sum += exponentials<false>(x[1], row.c, row.nm, 0, nullptr, nullptr, pk + 16, &l);
         }
+        if (__any_sync(0xffffffffu, !(sum <= row.most))) {
+          // Some row has outgrown its reference (or holds a NaN): take these keys' maximum in, and rescale O, for which the products
+          // before have to be done.
+          load();
+          const float top = top_of(general) - kHeadroom;
+          const float m = sum <= row.most ? row.m : fmaxf(row.m, top);
+          const float nm = m == -INFINITY ? 0.f : -m;
+          const float alpha = row.m == -INFINITY ? 0.f : ex2_approx(nm - row.nm);
+          row.m = m;
+          row.nm = nm;
+          row.most = m == -INFINITY ? 0.f : kRaiseAbove;
+          row.l *= alpha;
+          if (sb > 0) {
+            ok = __all_sync(0xffffffffu, wait_bounded(wctx, &sh.o_done[tile], (mine - 1) & 1, 0xbb00));
+            if (!ok) break;
+            tc_fence_after();
+            rescale(t_o, W, alpha);
+          }
+          l = 0.f;
+          exponentials<true>(x[0], row.c, row.nm, general ? lim : 64, rk, rv, pk, &l);
+          exponentials<true>(x[1], row.c, row.nm, general ? lim - 32 : 64, rk + 2, rv + 2, pk + 16, &l);
+        }
+        row.l += l;
+        tmem_st_32x32b_x32(t_s, pk);                             // over the scores, two to a column
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[tile][buf]));
       }
+      blocks += nb;
       if (!ok) break;
 
       // ---- O ----
