@@ -43,7 +43,10 @@ template <int W>
 struct PCfg {
   static constexpr int kTiles = W == 256 ? 1 : 2;
   static constexpr int kN = W == 256 ? 64 : 128;               // keys of a block
-  static constexpr int kSub = kN / 64;                         // sub-blocks of 64 keys, which scores and P come in
+  // Score buffers of a tile: one where two tiles take turns.  (Two of 64 keys each for the tiles of head dim 128 would keep a
+  // tile's scores ahead of its softmax, but a product of N = 64 is bound by reading Q: 80 cycles a step of 16 against 64 for N = 128,
+  // 327 us against 26x for 1024 tokens and 16384 keys.)
+  static constexpr int kBufs = kTiles == 2 ? 1 : 2;
   static constexpr int kGroups = kN / 16;                      // of keys that share a page
   static constexpr int kCols = W / 64;                         // column blocks of 64 fp16 (128 bytes)
   static constexpr int kRawRow = W < 128 ? W : 128;            // bytes of a row of a raw (fp8) tile
@@ -54,13 +57,17 @@ struct PCfg {
   static constexpr int kRing = 4;                              // widened tiles
   static constexpr int kRingBytes = kN * W * 2;
   static constexpr int kQBytes = kTileM * W * 2;               // of a tile
-  // Columns of tensor memory: a tile's two score buffers of 64 (P over them), then its O.
-  static constexpr int kTileCols = 128 + W;
-  static constexpr int kSoftWarps = 4 * kTiles;
+  // Columns of tensor memory: a tile's score buffers (P over them), then its O.
+  static constexpr int kOCol = kN * kBufs, kTileCols = kOCol + W;
+  static constexpr int kSoftWarps = 8 * kTiles;
   static constexpr int kWideWarp0 = kSoftWarps;
   static constexpr int kLoadWarp = kWideWarp0 + 4;
   static constexpr int kMmaWarp = kLoadWarp + 1;
-  static constexpr int kThreads = 32 * (kMmaWarp + 1);
+  // Whole warpgroups (two warps stand by), so that registers can be dealt out anew: 512 * 88 + 128 * 72 + 128 * 56 = 768 * 80.
+  static constexpr bool kDeal = kTiles == 2;
+  static constexpr int kThreads = 32 * (kLoadWarp + 4);
+  static constexpr uint32_t kSoftRegs = 88, kWideRegs = 72, kOtherRegs = 56;
+  static_assert(!kDeal || 32 * kSoftWarps * kSoftRegs + 128 * (kWideRegs + kOtherRegs) <= kThreads * 80, "registers of the launch");
   static constexpr int kRawOffset = kTiles * kQBytes;
   static constexpr int kRingOffset = kRawOffset + kRaw * kRawBytes;
   static constexpr int kSharedOffset = kRingOffset + kRing * kRingBytes;
@@ -82,7 +89,7 @@ struct Shared {
   uint64_t item_full[kItemSlots], item_empty[kItemSlots];
   uint64_t raw_full[C::kRaw], raw_empty[C::kRaw];
   uint64_t ring_full[C::kRing], ring_empty[C::kRing];
-  uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2], o_final[2];     // by tile, and score buffer
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], o_final[2], o_done;        // by tile, and score buffer
   uint64_t blk_full[kBlockSlots];
   uint64_t drain;
   Item item[kItemSlots];                 // seq < 0: no more
@@ -92,6 +99,7 @@ struct Shared {
   float residual[kBlockSlots][2][C::kGroups];   // of K and V; K's is -1 for a group without a page
   float ref[kBlockSlots][2];             // reference scales of the item that the block is of
   int flagged[kBlockSlots];              // some residual is not 1
+  float row[2][kTileM];                  // by tile and row, between the two warps that have it: what Q was divided by, maxima, sums
   uint32_t tmem;
   int abort;
 };
@@ -256,10 +264,10 @@ template <int W, bool kE5M2>
 __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                                                                           const KvAttendArgs a, const KvPrefillPlan plan) {
   using C = PCfg<W>;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* const gen = smem_raw + (base - smem_u32(smem_raw));
-  Shared<W>& sh = *reinterpret_cast<Shared<W>*>(gen + C::kSharedOffset);
+  // (No static shared memory, so this lies at a multiple of 1024 bytes, which the swizzled tiles need.)
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = smem_u32(smem_raw);
+  Shared<W>& sh = *reinterpret_cast<Shared<W>*>(smem_raw + C::kSharedOffset);
   const uint32_t s_q = base, s_raw = base + C::kRawOffset, s_ring = base + C::kRingOffset;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Wait wctx{&sh.abort, a.c.status, a.c.host_status};
@@ -273,10 +281,10 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     init(sh.raw_empty, C::kRaw, 4);
     init(sh.ring_full, C::kRing, 4);
     init(sh.ring_empty, C::kRing, 1);
-    init(sh.q_full, 2, 4);
+    init(sh.q_full, 2, 8);
     init(&sh.s_full[0][0], 4, 1);
-    init(&sh.p_full[0][0], 4, 4);
-    init(sh.o_done, 2, 1);
+    init(&sh.p_full[0][0], 4, 8);
+    init(&sh.o_done, 1, 1);
     init(sh.o_final, 2, 1);
     init(sh.blk_full, kBlockSlots, 1);
     init(&sh.drain, 1, 1);
@@ -297,6 +305,11 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
   tc_fence_after();
   start_after_predecessor();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
+  if (threadIdx.x == 0 && (base & 1023u) != 0u) {            // never seen; the tiles would be garbage, and it is reported
+    sh.abort = 1;
+    if (wctx.status) atomicCAS(wctx.status, 0, 0xb000);
+    if (wctx.host_status) *wctx.host_status = 0xb000;
+  }
 
   // rows of 64 bytes lie two to a swizzled line of 128: the halves of every other four lines are exchanged
   const uint32_t flip = W == 64 && a.c.head_dim == 64 ? 64u : 0u;
@@ -312,6 +325,9 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
   };
   auto item_read = [&] { mbar_arrive(smem_u32(&sh.item_empty[n_items++ % kItemSlots])); };
 
+  __syncwarp();
+  if (warp >= C::kLoadWarp) {
+  if constexpr (C::kDeal) setmaxnreg_dec<C::kOtherRegs>();
   if (warp == C::kLoadWarp) {
     // ---------------------------------------------------------------- producer
     bool ok = true;
@@ -461,68 +477,66 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
   } else if (warp == C::kMmaWarp) {
     // ---------------------------------------------------------------- issuer
     if (elect_one()) {
-      constexpr uint32_t kIdescQK = idesc(64, false), kIdescPV = idesc(W, true);
+      constexpr uint32_t kIdescQK = idesc(C::kN, false), kIdescPV = idesc(W, true);
       constexpr uint32_t kColQ = kTileM * 128 / 16, kColK = C::kN * 128 / 16;     // column blocks of Q and K in 16 bytes
-      constexpr uint32_t kSubRows = 64 * 128 / 16;                                // 64 rows of a column block
       const uint32_t q_lo = desc_lo(s_q, 16), k_lo = desc_lo(s_ring, 16), v_lo = desc_lo(s_ring, C::kN * 128);
       bool ok = true;
       uint32_t ld = 0;                                           // widened tiles used so far: K, V, K, V ...
       uint32_t qn[2] = {0, 0};                                   // q_full phases by tile
-      uint32_t pn[2] = {0, 0};                                   // sub-blocks by tile
+      uint32_t pn[2] = {0, 0};                                   // blocks by tile
       auto ring_wait = [&](uint32_t i) { return wait_bounded(wctx, &sh.ring_full[i % C::kRing], (i / C::kRing) & 1, 0xb400); };
       auto ring_release = [&](uint32_t i) { tc_commit(smem_u32(&sh.ring_empty[i % C::kRing])); };
-      // S of sub-block sb (of widened tile i) into score buffer b.
-      auto issue_qk = [&](int tile, uint32_t b, uint32_t i, int sb) {
-        const uint32_t kk = k_lo + (i % C::kRing) * (C::kRingBytes / 16) + (C::kSub > 1 ? (sb & 1) * kSubRows : 0u), qq = q_lo + tile * (C::kQBytes / 16);
+      auto issue_qk = [&](int tile, uint32_t b, uint32_t i) {
+        const uint32_t kk = k_lo + (i % C::kRing) * (C::kRingBytes / 16), qq = q_lo + tile * (C::kQBytes / 16);
 #pragma unroll
         for (int k = 0; k < W / 16; ++k)
-          mma_f16_ss(tmem + C::kTileCols * tile + 64 * b, desc(qq + (k >> 2) * kColQ + 2 * (k & 3)), desc(kk + (k >> 2) * kColK + 2 * (k & 3)), kIdescQK,
-                     k > 0);
+          mma_f16_ss(tmem + C::kTileCols * tile + C::kN * b, desc(qq + (k >> 2) * kColQ + 2 * (k & 3)), desc(kk + (k >> 2) * kColK + 2 * (k & 3)),
+                     kIdescQK, k > 0);
         tc_commit(smem_u32(&sh.s_full[tile][b]));
       };
-      auto issue_pv = [&](int tile, uint32_t b, uint32_t i, int sb) {
-        const uint32_t vv = v_lo + (i % C::kRing) * (C::kRingBytes / 16) + (C::kSub > 1 ? (sb & 1) * kSubRows : 0u);
+      auto issue_pv = [&](int tile, uint32_t b, uint32_t i, bool more) {
+        const uint32_t vv = v_lo + (i % C::kRing) * (C::kRingBytes / 16);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mma_f16_ts(tmem + C::kTileCols * tile + 128, tmem + C::kTileCols * tile + 64 * b + 8 * k, desc(vv + k * 128), kIdescPV, sb > 0 || k > 0);
-        tc_commit(smem_u32(&sh.o_done[tile]));
+        for (int k = 0; k < C::kN / 16; ++k)
+          mma_f16_ts(tmem + C::kTileCols * tile + C::kOCol, tmem + C::kTileCols * tile + C::kN * b + 8 * k, desc(vv + k * 128), kIdescPV, more || k > 0);
+        if (C::kBufs > 1) tc_commit(smem_u32(&sh.o_done));
       };
       Item it;
       while (ok && (ok = next_item(it))) {
         item_read();
         if (it.seq < 0) break;
-        const int n = (it.blk1 - it.blk0) * C::kSub;
+        const int n = it.blk1 - it.blk0;
         const int nt = C::kTiles == 2 && it.n_tokens > tile_tokens ? 2 : 1;
-        // The scores run two sub-blocks ahead: S(sb + 2) goes into the buffer that P V (sb) has read.
-        for (int sb = -2; sb < n && ok; ++sb) {
-          const uint32_t lv = ld + 2 * (max(sb, 0) / C::kSub) + 1, lk = ld + 2 * ((sb + 2) / C::kSub);
-          const bool qk = sb + 2 < n;
-          if (sb >= 0 && sb % C::kSub == 0) ok = ring_wait(lv);
+        // The scores run kBufs blocks ahead: S(j + kBufs) goes into the buffer that P V (j) has read.
+        for (int j = -C::kBufs; j < n && ok; ++j) {
+          const uint32_t lv = ld + 2 * j + 1, lk = ld + 2 * (j + C::kBufs);
+          const bool qk = j + C::kBufs < n;
+          if (j >= 0) ok = ring_wait(lv);
           for (int i = 0; i < nt && ok; ++i) {
-            const uint32_t b = (pn[i] + sb) & 1;
-            if (sb >= 0) {
-              ok = wait_bounded(wctx, &sh.p_full[i][b], ((pn[i] + sb) >> 1) & 1, 0xb600 + 2 * i + b);
+            const uint32_t b = (pn[i] + j) % C::kBufs;
+            if (j >= 0) {
+              ok = wait_bounded(wctx, &sh.p_full[i][b], ((pn[i] + j) / C::kBufs) & 1, 0xb600 + 2 * i + b);
               if (!ok) break;
               tc_fence_after();
-              issue_pv(i, b, lv, sb);
-              if (sb + 1 == n) tc_commit(smem_u32(&sh.o_final[i]));
-            } else if (sb == -2) {
+              issue_pv(i, b, lv, j > 0);
+              if (j + 1 == n) tc_commit(smem_u32(&sh.o_final[i]));
+            } else if (j == -C::kBufs) {
               ok = wait_bounded(wctx, &sh.q_full[i], qn[i]++ & 1, 0xb500 + i);
               if (!ok) break;
             }
             if (qk) {
-              if (i == 0 && (sb + 2) % C::kSub == 0) ok = ring_wait(lk);
+              if (i == 0) ok = ring_wait(lk);
               if (!ok) break;
               tc_fence_after();
-              issue_qk(i, b, lk, sb + 2);
+              issue_qk(i, b, lk);
             }
           }
           if (!ok) break;
-          if (sb >= 0 && (sb + 1) % C::kSub == 0) ring_release(lv);
-          if (qk && (sb + 3) % C::kSub == 0) ring_release(lk);
+          if (j >= 0) ring_release(lv);
+          if (qk) ring_release(lk);
         }
         for (int i = 0; i < nt; ++i) pn[i] += n;
-        ld += 2 * (it.blk1 - it.blk0);
+        ld += 2 * n;
       }
       {
         // products in flight, and their arrivals, end before tensor and shared memory are freed (with a limit)
@@ -532,8 +546,10 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       }
     }
     __syncwarp();
+  }
   } else if (warp >= C::kWideWarp0) {
     // ---------------------------------------------------------------- widening
+    if constexpr (C::kDeal) setmaxnreg_dec<C::kWideRegs>();
     const int w = warp - C::kWideWarp0;
     uint32_t tiles = 0;
     Item it;
@@ -553,27 +569,31 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         const int valid = sh.valid[st];
         const uint32_t src = s_raw + st * C::kRawBytes, dst = s_ring + rg * C::kRingBytes;
         // A warp takes eight rows and 64 columns at a time: eight lanes side by side read and write eight rows of one 16-byte
-        // column, which the swizzles spread over all banks.  All its loads go out before the first is used.
+        // column, which the swizzles spread over all banks.  Four loads go out before the first is used.
         constexpr int kParts = (C::kN / 8) * C::kCols, kMine = kParts / 4;
         const int q = lane >> 3, r8 = lane & 7;
-        uint4 x[kMine];
-        uint32_t f[kMine];
+        constexpr int kAt = kMine < 4 ? kMine : 4;
+#pragma unroll 1
+        for (int k0 = 0; k0 < kMine; k0 += kAt) {
+        uint4 x[kAt];
+        uint32_t f[kAt];
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) {
-          const int p = w + 4 * k, cb = p % C::kCols, r = (p / C::kCols) * 8 + r8;
+        for (int k = 0; k < kAt; ++k) {
+          const int p = w + 4 * (k0 + k), cb = p % C::kCols, r = (p / C::kCols) * 8 + r8;
           if constexpr (W == 64) x[k] = ld_shared16(src + ((r * 64 + ((q ^ ((r >> 1) & 3)) << 4)) ^ ((r & 8) ? flip : 0u)));
           else x[k] = ld_shared16(src + (cb >> 1) * C::kRawBlockBytes + r * 128 + (((4 * (cb & 1) + q) ^ r8) << 4));
           f[k] = sh.factor[st][r >> 4];
         }
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) {
-          const int p = w + 4 * k, cb = p % C::kCols, r = (p / C::kCols) * 8 + r8;
+        for (int k = 0; k < kAt; ++k) {
+          const int p = w + 4 * (k0 + k), cb = p % C::kCols, r = (p / C::kCols) * 8 + r8;
           uint4 lo, hi;
           widen16<kE5M2>(x[k], f[k], lo, hi);
           if (!sh.complete[st] && (r >= valid || f[k] == 0u)) lo = hi = make_uint4(0u, 0u, 0u, 0u);
           const uint32_t to = dst + cb * (C::kN * 128) + r * 128;
           st_shared16(to + (((2 * q) ^ r8) << 4), lo);
           st_shared16(to + (((2 * q + 1) ^ r8) << 4), hi);
+        }
         }
         fence_proxy_async_smem();                                // what was written is for the products to read
         __syncwarp();
@@ -585,16 +605,48 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    const int tile = warp / 4, sub = warp % 4;                   // rows 32 sub ... of the tile = lanes of tensor memory
+    if constexpr (C::kDeal) setmaxnreg_inc<C::kSoftRegs>();
+    // Two warps to 32 rows (lanes of tensor memory): each takes half of a block's keys, of O's columns and of the rows of Q.
+    const int tile = warp / 8, sub = warp % 4, part = warp / 4 % 2;
     const uint32_t lanes = static_cast<uint32_t>(32 * sub) << 16;
-    const uint32_t t_tile = tmem + lanes + C::kTileCols * tile, t_o = t_tile + 128;
+    const uint32_t t_tile = tmem + lanes + C::kTileCols * tile, t_o = t_tile + C::kOCol + part * (W / 2);
+    constexpr int kMyKeys = C::kN / 2, kMyCols = W / 2;
+    const int r = 32 * sub + lane;                               // this thread's row
+    const int pair_bar = 1 + tile * 4 + sub;
+    // (Tensor-memory instructions and barriers want whole warps: lanes that left a wait at different times meet before each.)
+    auto pair_sync = [&] {
+      __syncwarp();
+      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+    };
+    auto pair_any = [&](bool x) {
+      __syncwarp();
+      uint32_t y;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+                   : "=r"(y) : "r"(static_cast<uint32_t>(x)), "r"(pair_bar) : "memory");
+      return y != 0u;
+    };
+    // The other warp's value for this row.
+    auto exchange = [&](float x) {
+      float* const p = &sh.row[tile][r];
+      if (part == 0) *p = x;
+      pair_sync();
+      float y = 0.f;
+      if (part == 1) {
+        y = *p;
+        *p = x;
+      }
+      pair_sync();
+      return part == 1 ? y : *p;
+    };
     uint32_t blocks = 0;                                         // of all items (the residual ring), also those this tile sits out
-    uint32_t mine = 0;                                           // sub-blocks this tile took part in
+    uint32_t mine = 0;                                           // blocks this tile took part in
     uint32_t taken = 0;                                          // items this tile took part in
     Item it;
     bool ok = true;
-    while (ok && (ok = next_item(it))) {
-      __syncwarp();
+    while (true) {
+      // A warp whose wait ran out takes the other of its pair along: neither waits for one that has left.
+      ok = !pair_any(!next_item(it));
+      if (!ok) break;
       if (lane == 0) item_read();
       else ++n_items;
       if (it.seq < 0) break;
@@ -606,24 +658,24 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         continue;
       }
       const int D = a.c.head_dim;
-      // ---- Q: this warp's 32 rows into shared memory, fp16 ----
-      constexpr int kLanes = W / 8, kRowsAt = 32 / kLanes;       // lanes of a row (8 columns each), rows at a time
-      const int my_col = lane % kLanes, my_row = 32 * sub + lane / kLanes;
-      float back = 1.f;
+      // ---- Q: sixteen rows into shared memory, fp16 ----
       {
-        uint4 x[32 / kRowsAt];                                   // all of them under way at once
+        constexpr int kLanes = W / 8, kRowsAt = 32 / kLanes, kTimes = 16 / kRowsAt;     // lanes of a row (8 columns each), rows at a time
+        const int col = lane % kLanes, row0 = 32 * sub + 16 * part + lane / kLanes;
+        uint4 x[kTimes];                                         // all of them under way at once
         const uint16_t* const q0 = static_cast<const uint16_t*>(a.q.x) + (static_cast<int64_t>(it.first) + tok0) * a.q.token_stride +
-                                   static_cast<int64_t>(it.head) * group * a.q.head_stride + 8 * my_col;
+                                   static_cast<int64_t>(it.head) * group * a.q.head_stride + 8 * col;
 #pragma unroll
-        for (int k = 0; k < 32 / kRowsAt; ++k) {
-          const int r = my_row + k * kRowsAt, token = (r * over_group) >> 16;
+        for (int k = 0; k < kTimes; ++k) {
+          const int q = row0 + k * kRowsAt, token = (q * over_group) >> 16;
           x[k] = make_uint4(0u, 0u, 0u, 0u);
-          if (r < n_rows && 8 * my_col < D)
-            x[k] = ld_global(reinterpret_cast<const uint4*>(q0 + token * a.q.token_stride + (r - token * group) * a.q.head_stride));
+          if (q < n_rows && 8 * col < D)
+            x[k] = ld_global(reinterpret_cast<const uint4*>(q0 + token * a.q.token_stride + (q - token * group) * a.q.head_stride));
         }
 #pragma unroll
-        for (int k = 0; k < 32 / kRowsAt; ++k) {
-          const int r = my_row + k * kRowsAt;
+        for (int k = 0; k < kTimes; ++k) {
+          const int q = row0 + k * kRowsAt;
+          float back = 1.f;
           if (a.bf16) {
             float big = 0.f;
             uint32_t v[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
@@ -636,98 +688,108 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
             for (int o = kLanes / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
             const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 126);
             const float f = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
-            const float g = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
+            back = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float2 y = half_pair<true>(v[i]);
               v[i] = pack_half2(y.x * f, y.y * f);
             }
             x[k] = make_uint4(v[0], v[1], v[2], v[3]);
-#pragma unroll
-            for (int i = 0; i < kRowsAt; ++i) {
-              const float y = __shfl_sync(0xffffffffu, g, i * kLanes);
-              if (lane == k * kRowsAt + i) back = y;
-            }
           }
-          st_shared16(s_q + tile * C::kQBytes + (my_col >> 3) * (kTileM * 128) + r * 128 + (((my_col & 7) ^ (r & 7)) << 4), x[k]);
+          if (col == 0) sh.row[tile][q] = back;
+          st_shared16(s_q + tile * C::kQBytes + (col >> 3) * (kTileM * 128) + q * 128 + (((col & 7) ^ (q & 7)) << 4), x[k]);
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[tile]));
+      pair_sync();                                               // the other warp's rows of sh.row
+      const float back = sh.row[tile][r];
+      pair_sync();
 
-      const int r = 32 * sub + lane;
       Row row{};
       row.m = -INFINITY;
       const int my_token = tok0 + ((min(r, n_rows - 1) * over_group) >> 16);
       row.lim = a.causal ? max(0, min(it.len, it.len - it.n + my_token + 1)) : it.len;
       const int least = a.causal ? max(0, min(it.len, it.len - it.n + tok0 + 1)) : it.len;       // of the tile's first row
       float vref = 1.f;
-      for (int sb = 0; sb < nb * C::kSub && ok; ++sb, ++mine) {
-        const int j = sb / C::kSub, buf = mine & 1;
+      for (int j = 0; j < nb && ok; ++j, ++mine) {
+        const int buf = mine % C::kBufs;
         const uint32_t n = (blocks + j) % kBlockSlots;
-        const uint32_t t_s = t_tile + 64 * buf;
-        if (sb % C::kSub == 0) ok = wait_bounded(wctx, &sh.blk_full[n], ((blocks + j) / kBlockSlots) & 1, 0xb900);
-        if (ok) ok = wait_bounded(wctx, &sh.s_full[tile][buf], (mine >> 1) & 1, 0xba00 + buf);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        const uint32_t t_s = t_tile + C::kN * buf + part * kMyKeys;
+        ok = wait_bounded(wctx, &sh.blk_full[n], ((blocks + j) / kBlockSlots) & 1, 0xb900);
+        if (ok) ok = wait_bounded(wctx, &sh.s_full[tile][buf], (mine / C::kBufs) & 1, 0xba00 + buf);
+        __syncwarp();
         tc_fence_after();
-        if (sb == 0) {
+        const int key0 = (it.blk0 + j) * C::kN, lim = row.lim - key0 - part * kMyKeys;
+        const bool general = sh.flagged[n] != 0 || key0 + C::kN > least;
+        const float *rk = sh.residual[n][0] + part * (kMyKeys / 16), *rv = sh.residual[n][1] + part * (kMyKeys / 16);
+        // the largest score of this warp's keys
+        auto top_of = [&] {
+          float m = -INFINITY;
+#pragma unroll 1
+          for (int k = 0; k < kMyKeys; k += 32) {
+            uint32_t x[32];
+            tmem_ld_32x32b_x32(t_s + k, x);
+            tmem_wait_ld();
+            m = fmaxf(m, general ? largest<true>(x, row.c, lim - k, rk + k / 16, rv + k / 16) : largest<false>(x, row.c, 0, nullptr, nullptr));
+          }
+          return m;
+        };
+        if (j == 0) {
           row.c = a.scale_log2 * back * sh.ref[n][0];
           vref = sh.ref[n][1];
-        }
-        const int key0 = it.blk0 * C::kN + 64 * sb, lim = row.lim - key0;
-        const bool general = sh.flagged[n] != 0 || key0 + 64 > least;
-        const float *rk = sh.residual[n][0] + 4 * (sb % C::kSub), *rv = sh.residual[n][1] + 4 * (sb % C::kSub);
-        uint32_t x[2][32], pk[32];
-        auto load = [&] {
-          tmem_ld_32x32b_x32(t_s, x[0]);
-          tmem_ld_32x32b_x32(t_s + 32, x[1]);
-          tmem_wait_ld();
-        };
-        auto top_of = [&](bool g) {
-          return g ? fmaxf(largest<true>(x[0], row.c, lim, rk, rv), largest<true>(x[1], row.c, lim - 32, rk + 2, rv + 2))
-                   : fmaxf(largest<false>(x[0], row.c, 0, nullptr, nullptr), largest<false>(x[1], row.c, 0, nullptr, nullptr));
-        };
-        load();
-        if (sb == 0) {                                           // the exact maximum of the first 64 keys
-          const float m = top_of(general);
+          float m = top_of();                                    // exact for the first block
+          m = fmaxf(m, exchange(m));
           row.m = m - kHeadroom;
           row.nm = m == -INFINITY ? 0.f : -row.m;
           row.most = m == -INFINITY ? 0.f : kRaiseAbove;
         }
-        float l = 0.f, sum;
-        if (general) {
-          sum = exponentials<true>(x[0], row.c, row.nm, lim, rk, rv, pk, &l);
-          sum += exponentials<true>(x[1], row.c, row.nm, lim - 32, rk + 2, rv + 2, pk + 16, &l);
-        } else {
-          sum = exponentials<false>(x[0], row.c, row.nm, 0, nullptr, nullptr, pk, &l);
-          sum += exponentials<false>(x[1], row.c, row.nm, 0, nullptr, nullptr, pk + 16, &l);
-        }
-        if (__any_sync(0xffffffffu, !(sum <= row.most))) {
-          // Some row has outgrown its reference (or holds a NaN): take these keys' maximum in, and rescale O, for which the products
-          // before have to be done.
-          load();
-          const float top = top_of(general) - kHeadroom;
-          const float m = sum <= row.most ? row.m : fmaxf(row.m, top);
+        // P of the block; the scores are left as they are until no reference has to be raised for them.
+        uint32_t pk[kMyKeys / 2];
+        float l = 0.f;
+        bool raised = false;
+        while (true) {
+          float sum = 0.f;
+          l = 0.f;
+#pragma unroll
+          for (int q = 0; q < kMyKeys / 32; ++q) {
+            uint32_t x[32];
+            tmem_ld_32x32b_x32(t_s + 32 * q, x);
+            tmem_wait_ld();
+            sum += general ? exponentials<true>(x, row.c, row.nm, lim - 32 * q, rk + 2 * q, rv + 2 * q, pk + 16 * q, &l)
+                           : exponentials<false>(x, row.c, row.nm, 0, nullptr, nullptr, pk + 16 * q, &l);
+          }
+          // (also: the other warp has read what P is about to be written over)
+          const bool over = !(sum <= row.most);
+          const bool any = pair_any(over || !ok);
+          if (any && pair_any(!ok)) {
+            ok = false;
+            break;
+          }
+          if (!any || raised) break;
+          // Some row has outgrown its reference (or holds a NaN): take this block's maximum in and rescale O, for which the products
+          // before have to be done (with one buffer they are: this block's scores came after them).
+          raised = true;
+          const float mine_top = top_of() - kHeadroom, top = over ? mine_top : -INFINITY;
+          const float m = fmaxf(fmaxf(row.m, top), exchange(top));
           const float nm = m == -INFINITY ? 0.f : -m;
           const float alpha = row.m == -INFINITY ? 0.f : ex2_approx(nm - row.nm);
           row.m = m;
           row.nm = nm;
           row.most = m == -INFINITY ? 0.f : kRaiseAbove;
           row.l *= alpha;
-          if (sb > 0) {
-            ok = __all_sync(0xffffffffu, wait_bounded(wctx, &sh.o_done[tile], (mine - 1) & 1, 0xbb00));
-            if (!ok) break;
+          if (j > 0) {
+            if (C::kBufs > 1) ok = wait_bounded(wctx, &sh.o_done, (mine - 1) & 1, 0xbb00) && ok;
+            __syncwarp();
             tc_fence_after();
-            rescale(t_o, W, alpha);
+            rescale(t_o, kMyCols, alpha);
           }
-          l = 0.f;
-          exponentials<true>(x[0], row.c, row.nm, general ? lim : 64, rk, rv, pk, &l);
-          exponentials<true>(x[1], row.c, row.nm, general ? lim - 32 : 64, rk + 2, rv + 2, pk + 16, &l);
         }
+        if (!ok) break;
         row.l += l;
-        tmem_st_32x32b_x32(t_s, pk);                             // over the scores, two to a column
+        if constexpr (kMyKeys == 64) tmem_st_32x32b_x32(t_tile + C::kN * buf + part * 32, pk);       // over the scores
+        else tmem_st_32x32b_x16(t_tile + C::kN * buf + part * 16, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -737,16 +799,17 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       if (!ok) break;
 
       // ---- O ----
-      ok = __all_sync(0xffffffffu, wait_bounded(wctx, &sh.o_final[tile], taken & 1, 0xbc00 + tile));
+      const bool whole = plan.parts == 1;
+      row.l += exchange(row.l);
+      ok = !pair_any(!wait_bounded(wctx, &sh.o_final[tile], taken & 1, 0xbc00 + tile));
       if (!ok) break;
       ++taken;
       tc_fence_after();
-      const bool whole = plan.parts == 1;
       const float inv = (row.l == 0.f ? 0.f : (whole ? 1.f / row.l : 1.f)) * vref;
       const int token = (r * over_group) >> 16;
       const int64_t row0 = (static_cast<int64_t>(it.first) + tok0) * a.heads_q + it.head * group;
       const int64_t out_row = row0 + token * a.heads_q + (r - token * group);
-      if (r < n_rows) {
+      if (r < n_rows && part == 0) {
         if (whole) {
           if (a.lse != nullptr) a.lse[out_row] = row.l == 0.f ? -INFINITY : (row.m + __log2f(row.l)) * 0.6931471805599453f;
         } else {
@@ -756,14 +819,16 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         }
       }
       float* const po = whole ? nullptr : plan.partial_o + (static_cast<int64_t>(it.part) * a.c.tokens * a.heads_q + out_row) * D;
-      // through this warp's rows of Q's shared memory, which the last scores have been made from: 16 bytes a lane side by side
+      // through these rows and columns of Q's shared memory, which the last scores have been made from: 16 bytes a lane side by side
       const uint32_t stage = s_q + tile * C::kQBytes;
 #pragma unroll 1
-      for (int c = 0; c < W; c += 32) {
+      for (int c = 0; c < kMyCols; c += 32) {
+        __syncwarp();
         uint32_t o[32];
         tmem_ld_32x32b_x32(t_o + c, o);
         tmem_wait_ld();
-        if (c >= D) continue;
+        const int col = part * kMyCols + c;
+        if (col >= D) continue;
         if (whole) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
@@ -773,7 +838,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
               const float x = __uint_as_float(o[i + 2 * k]) * inv, y = __uint_as_float(o[i + 2 * k + 1]) * inv;
               v[k] = a.bf16 ? pack_pair<true>(x, y) : pack_pair<false>(x, y);
             }
-            const int ch = (c + i) >> 3;
+            const int ch = (col + i) >> 3;
             st_shared_v4(stage + (ch >> 3) * (kTileM * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), v[0], v[1], v[2], v[3]);
           }
         } else if (r < n_rows) {
@@ -782,23 +847,25 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
             float4 v;
             v.x = __uint_as_float(o[i]) * inv; v.y = __uint_as_float(o[i + 1]) * inv;
             v.z = __uint_as_float(o[i + 2]) * inv; v.w = __uint_as_float(o[i + 3]) * inv;
-            *reinterpret_cast<float4*>(po + c + i) = v;
+            *reinterpret_cast<float4*>(po + col + i) = v;
           }
         }
       }
       tc_fence_before();
       if (whole) {
         __syncwarp();
-#pragma unroll 8
-        for (int k = 0; k < 32 / kRowsAt; ++k) {
-          const int q = my_row + k * kRowsAt, t = (q * over_group) >> 16;
-          if (q < n_rows && 8 * my_col < D) {
-            const uint4 v = ld_shared16(stage + (my_col >> 3) * (kTileM * 128) + q * 128 + (((my_col & 7) ^ (q & 7)) << 4));
-            st_global_v4(static_cast<uint16_t*>(a.o) + (row0 + t * a.heads_q + (q - t * group)) * D + 8 * my_col, v.x, v.y, v.z, v.w);
+        constexpr int kLanes = kMyCols / 8, kRowsAt = 32 / kLanes;       // lanes of half a row, rows at a time
+        const int ch = part * kLanes + lane % kLanes;
+#pragma unroll 4
+        for (int q = 32 * sub + lane / kLanes; q < 32 * sub + 32; q += kRowsAt) {
+          const int t = (q * over_group) >> 16;
+          if (q < n_rows && 8 * ch < D) {
+            const uint4 v = ld_shared16(stage + (ch >> 3) * (kTileM * 128) + q * 128 + (((ch & 7) ^ (q & 7)) << 4));
+            st_global_v4(static_cast<uint16_t*>(a.o) + (row0 + t * a.heads_q + (q - t * group)) * D + 8 * ch, v.x, v.y, v.z, v.w);
           }
         }
-        __syncwarp();
       }
+      pair_sync();                                               // both warps are through with these rows of Q's memory
     }
   }
   let_successor_start();
@@ -869,7 +936,7 @@ template <int W, bool kE5M2>
 cudaError_t launch_one(const CUtensorMap& tk, const CUtensorMap& tv, const KvAttendArgs& a, const KvPrefillPlan& plan, int sms, cudaStream_t stream) {
   using C = PCfg<W>;
   auto kernel = &kv_prefill_kernel<W, kE5M2>;
-  constexpr int smem = C::kSharedOffset + static_cast<int>(sizeof(Shared<W>)) + 1024;
+  constexpr int smem = C::kSharedOffset + static_cast<int>(sizeof(Shared<W>));
   static_assert(smem <= 227 * 1024, "shared memory");
   static std::atomic<bool> ready[64];
   int dev = 0;
