@@ -569,31 +569,42 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         const int valid = sh.valid[st];
         const uint32_t src = s_raw + st * C::kRawBytes, dst = s_ring + rg * C::kRingBytes;
         // A warp takes eight rows and 64 columns at a time: eight lanes side by side read and write eight rows of one 16-byte
-        // column, which the swizzles spread over all banks.  Four loads go out before the first is used.
+        // column, which the swizzles spread over all banks.
         constexpr int kParts = (C::kN / 8) * C::kCols, kMine = kParts / 4;
         const int q = lane >> 3, r8 = lane & 7;
-        constexpr int kAt = kMine < 4 ? kMine : 4;
-#pragma unroll 1
-        for (int k0 = 0; k0 < kMine; k0 += kAt) {
-        uint4 x[kAt];
-        uint32_t f[kAt];
-#pragma unroll
-        for (int k = 0; k < kAt; ++k) {
-          const int p = w + 4 * (k0 + k), cb = p % C::kCols, r = (p / C::kCols) * 8 + r8;
-          if constexpr (W == 64) x[k] = ld_shared16(src + ((r * 64 + ((q ^ ((r >> 1) & 3)) << 4)) ^ ((r & 8) ? flip : 0u)));
-          else x[k] = ld_shared16(src + (cb >> 1) * C::kRawBlockBytes + r * 128 + (((4 * (cb & 1) + q) ^ r8) << 4));
-          f[k] = sh.factor[st][r >> 4];
-        }
-#pragma unroll
-        for (int k = 0; k < kAt; ++k) {
-          const int p = w + 4 * (k0 + k), cb = p % C::kCols, r = (p / C::kCols) * 8 + r8;
-          uint4 lo, hi;
-          widen16<kE5M2>(x[k], f[k], lo, hi);
-          if (!sh.complete[st] && (r >= valid || f[k] == 0u)) lo = hi = make_uint4(0u, 0u, 0u, 0u);
-          const uint32_t to = dst + cb * (C::kN * 128) + r * 128;
+        auto from = [&](int p) {
+          const int cb = p % C::kCols, r = (p / C::kCols) * 8 + r8;
+          if constexpr (W == 64) return src + ((r * 64 + ((q ^ ((r >> 1) & 3)) << 4)) ^ ((r & 8) ? flip : 0u));
+          else return src + (cb >> 1) * C::kRawBlockBytes + r * 128 + (((4 * (cb & 1) + q) ^ r8) << 4);
+        };
+        auto put = [&](int p, const uint4& lo, const uint4& hi) {
+          const uint32_t to = dst + (p % C::kCols) * (C::kN * 128) + ((p / C::kCols) * 8 + r8) * 128;
           st_shared16(to + (((2 * q) ^ r8) << 4), lo);
           st_shared16(to + (((2 * q + 1) ^ r8) << 4), hi);
-        }
+        };
+        if (sh.complete[st]) {
+          // all loads go out before the first is used
+          uint4 x[kMine];
+          uint32_t f[kMine];
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) {
+            x[k] = ld_shared16(from(w + 4 * k));
+            f[k] = sh.factor[st][(w + 4 * k) / C::kCols / 2];
+          }
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) {
+            uint4 lo, hi;
+            widen16<kE5M2>(x[k], f[k], lo, hi);
+            put(w + 4 * k, lo, hi);
+          }
+        } else {
+#pragma unroll 1
+          for (int p = w; p < kParts; p += 4) {
+            const uint32_t f = sh.factor[st][p / C::kCols / 2];
+            uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+            if (f != 0u && (p / C::kCols) * 8 + r8 < valid) widen16<kE5M2>(ld_shared16(from(p)), f, lo, hi);
+            put(p, lo, hi);
+          }
         }
         fence_proxy_async_smem();                                // what was written is for the products to read
         __syncwarp();
