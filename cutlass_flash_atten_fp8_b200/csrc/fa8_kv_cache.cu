@@ -18,8 +18,9 @@ namespace fa8 {
 
 namespace {
 
-constexpr int kHold = 4;               // chunks of sixteen elements that a thread keeps in registers
-constexpr int kWarpWork = 32 * kHold * 16;
+constexpr int kVec = 8;                 // elements of a vector: 16 bytes of half precision, 8 of fp8
+constexpr int kHold = 8;                // vectors that a thread keeps in registers (1 where units have no more)
+constexpr int kWarpWork = 32 * kHold * kVec;
 constexpr int kMaxThreads = 512;
 constexpr int kWarpsPerCta = 4;        // units of a CTA where a warp takes one
 
@@ -27,8 +28,8 @@ constexpr int kWarpsPerCta = 4;        // units of a CTA where a warp takes one
 struct Unit {
   int head;
   bool of_v;
-  int page;                            // -1: nothing to do, or (read) zeros are due
-  int off, rows;                       // slots off .. off + rows - 1
+  int page;                            // as the table has it; -1: nothing to do, or (read) zeros are due
+  int off, rows;                       // slots off .. off + rows - 1; off -1: of a sequence that is out of range
   int row0;                            // first row of the token-major tensors
 };
 
@@ -48,6 +49,7 @@ __device__ __forceinline__ Unit find_unit(const KvArgs& a, int64_t u) {
     if (i == 0 && j == 0) report_bad_index(a);
     const int64_t lo = static_cast<int64_t>(j) * P;
     if (kRead && lo < s.n) {
+      r.off = -1;
       r.rows = min(P, s.n - static_cast<int>(lo));
       r.row0 = s.first + static_cast<int>(lo);
     }
@@ -60,12 +62,19 @@ __device__ __forceinline__ Unit find_unit(const KvArgs& a, int64_t u) {
   r.off = static_cast<int>(lo) & (P - 1);
   r.rows = static_cast<int>(hi - lo);
   r.row0 = s.first + static_cast<int>(lo - start);
-  r.page = kv_page(a, b, static_cast<int>(pi));
+  r.page = ld_int(a.table + static_cast<int64_t>(b) * a.table_stride + pi);      // looked at once the rows are on their way
   return r;
 }
 
-// Row of chunk i where a row has `per_row` <= 16 chunks, i < 2048: magic = 65536 / per_row + 1.
-__device__ __forceinline__ int row_of(int i, uint32_t magic) { return static_cast<int>((static_cast<uint32_t>(i) * magic) >> 16); }
+// Row of vector i where a row has `per_row` <= 32 vectors, i <= 4096: magic = 2^20 / per_row + 1.
+__device__ __forceinline__ int row_of(int i, uint32_t magic) { return static_cast<int>((static_cast<uint32_t>(i) * magic) >> 20); }
+
+// A page number from the table, -1 (reported) if it is out of range.
+__device__ __forceinline__ int checked(const KvArgs& a, int page) {
+  if (static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages)) return page;
+  report_bad_index(a);
+  return -1;
+}
 
 template <bool kE5M2>
 __device__ __forceinline__ float scale_for(float amax) {
@@ -114,7 +123,7 @@ __device__ __forceinline__ uint2 to_fp8x8(const uint4& x, float inv) {
 }
 
 // kWarp: a unit to a warp, several a CTA; otherwise a unit to a CTA.
-template <bool kBf16, bool kE5M2, bool kWarp>
+template <bool kBf16, bool kE5M2, bool kWarp, int kHold>
 __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_append_kernel(const KvArgs a, const KvRows kin, const KvRows vin,
                                                                                             int64_t units, uint32_t magic) {
   __shared__ float part[kMaxThreads / 32];
@@ -124,36 +133,32 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_ap
   const int64_t u = kWarp ? static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5) : blockIdx.x;
   if (u >= units) return;
   const Unit w = find_unit<false>(a, u);
-  if (w.page < 0) return;                                 // the same for all threads of the unit
-  const int D = a.head_dim, per_row = D >> 4, chunks = w.rows * per_row;
+  if (w.rows == 0) return;                                // the same for all threads of the unit, as below
+  const int D = a.head_dim, per_row = D / kVec, n = w.rows * per_row;
   const KvRows& in = w.of_v ? vin : kin;
   const uint16_t* x = static_cast<const uint16_t*>(in.x) + w.row0 * in.token_stride + w.head * in.head_stride;
-  const int64_t page_head = static_cast<int64_t>(w.page) * a.heads + w.head;
-  uint8_t* const y = (w.of_v ? a.v : a.k) + (page_head << a.page_shift) * D;
-  float* const descale = (w.of_v ? a.v_descale : a.k_descale) + page_head;
-  const float old = w.off > 0 ? ld_global(descale) : 0.f;
   auto src = [&](int i) {
     const int r = row_of(i, magic);
-    return reinterpret_cast<const uint4*>(x + r * in.token_stride + 16 * (i - r * per_row));
+    return reinterpret_cast<const uint4*>(x + r * in.token_stride + kVec * (i - r * per_row));
   };
-  uint4 hold[kHold][2];
-  float amax = 0.f;
+  uint4 hold[kHold];
 #pragma unroll
   for (int h = 0; h < kHold; ++h) {
     const int i = tid + h * n_threads;
-    hold[h][0] = hold[h][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (i < chunks) {
-      const uint4* p = src(i);
-      hold[h][0] = ld_global(p);
-      hold[h][1] = ld_global(p + 1);
-    }
+    hold[h] = make_uint4(0u, 0u, 0u, 0u);
+    if (i < n) hold[h] = ld_global(src(i));
   }
+  const int page = checked(a, w.page);
+  if (page < 0) return;
+  const int64_t page_head = static_cast<int64_t>(page) * a.heads + w.head;
+  uint8_t* const y = (w.of_v ? a.v : a.k) + (page_head << a.page_shift) * D;
+  float* const descale = (w.of_v ? a.v_descale : a.k_descale) + page_head;
+  const float old = w.off > 0 ? ld_global(descale) : 0.f;
+  float amax = 0.f;
 #pragma unroll
-  for (int h = 0; h < kHold; ++h) amax = fmaxf(amax, fmaxf(abs_max<kBf16>(hold[h][0]), abs_max<kBf16>(hold[h][1])));
-  for (int i = tid + kHold * n_threads; i < chunks; i += n_threads) {
-    const uint4* p = src(i);
-    amax = fmaxf(amax, fmaxf(abs_max<kBf16>(ld_global(p)), abs_max<kBf16>(ld_global(p + 1))));
-  }
+  for (int h = 0; h < kHold; ++h)
+    amax = fmaxf(amax, abs_max<kBf16>(hold[h]));
+  for (int i = tid + kHold * n_threads; i < n; i += n_threads) amax = fmaxf(amax, abs_max<kBf16>(ld_global(src(i))));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if (!kWarp) {
@@ -167,7 +172,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_ap
     if (d > old) {
       const float f = old / d;
       uint4* const older = reinterpret_cast<uint4*>(y);
-      for (int i = tid; i < w.off * per_row; i += n_threads) {
+      for (int i = tid; i < w.off * (D / 16); i += n_threads) {
         const uint4 c = ld_global(older + i);
         const uint32_t in4[4] = {c.x, c.y, c.z, c.w};
         uint32_t out4[4];
@@ -184,23 +189,16 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_ap
   }
   if (tid == 0) *descale = d;                             // every thread has read the old one: the reduction lies between
   const float inv = 1.f / d;
-  uint4* const dst = reinterpret_cast<uint4*>(y + w.off * D);
+  uint2* const dst = reinterpret_cast<uint2*>(y + w.off * D);
 #pragma unroll
   for (int h = 0; h < kHold; ++h) {
     const int i = tid + h * n_threads;
-    if (i < chunks) {
-      const uint2 lo = to_fp8x8<kBf16, kE5M2>(hold[h][0], inv), hi = to_fp8x8<kBf16, kE5M2>(hold[h][1], inv);
-      dst[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-    }
+    if (i < n) dst[i] = to_fp8x8<kBf16, kE5M2>(hold[h], inv);
   }
-  for (int i = tid + kHold * n_threads; i < chunks; i += n_threads) {
-    const uint4* p = src(i);
-    const uint2 lo = to_fp8x8<kBf16, kE5M2>(ld_global(p), inv), hi = to_fp8x8<kBf16, kE5M2>(ld_global(p + 1), inv);
-    dst[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-  }
+  for (int i = tid + kHold * n_threads; i < n; i += n_threads) dst[i] = to_fp8x8<kBf16, kE5M2>(ld_global(src(i)), inv);
 }
 
-template <bool kBf16, bool kE5M2, bool kWarp>
+template <bool kBf16, bool kE5M2, bool kWarp, int kHold>
 __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_read_kernel(const KvArgs a, uint16_t* k_out, uint16_t* v_out,
                                                                                           int64_t units, uint32_t magic) {
   start_after_predecessor();
@@ -209,39 +207,37 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_re
   const int64_t u = kWarp ? static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5) : blockIdx.x;
   if (u >= units) return;
   const Unit w = find_unit<true>(a, u);
-  const int D = a.head_dim, per_row = D >> 4, chunks = w.rows * per_row;
-  if (chunks == 0) return;
-  const int64_t page_head = static_cast<int64_t>(w.page < 0 ? 0 : w.page) * a.heads + w.head;
-  const uint8_t* x = (w.of_v ? a.v : a.k) + ((page_head << a.page_shift) + w.off) * D;
-  const float d = w.page < 0 ? 0.f : ld_global((w.of_v ? a.v_descale : a.k_descale) + page_head);
+  if (w.rows == 0) return;
+  const int D = a.head_dim, per_row = D / kVec, n = w.rows * per_row;
+  const int page = w.page == -1 && w.off < 0 ? -1 : checked(a, w.page);
+  const int64_t page_head = static_cast<int64_t>(max(page, 0)) * a.heads + w.head;
+  const uint8_t* x = (w.of_v ? a.v : a.k) + ((page_head << a.page_shift) + max(w.off, 0)) * D;
+  const float d = page < 0 ? 0.f : ld_global((w.of_v ? a.v_descale : a.k_descale) + page_head);
   const int64_t row = static_cast<int64_t>(a.heads) * D;
   uint16_t* const y = (w.of_v ? v_out : k_out) + w.row0 * row + w.head * D;
-  for (int i0 = tid; i0 < chunks; i0 += kHold * n_threads) {
-    uint4 c[kHold];
+  for (int i0 = tid; i0 < n; i0 += kHold * n_threads) {
+    uint2 c[kHold];
 #pragma unroll
     for (int h = 0; h < kHold; ++h) {
       const int i = i0 + h * n_threads;
-      c[h] = make_uint4(0u, 0u, 0u, 0u);
-      if (i < chunks && w.page >= 0) c[h] = ld_stream16(x + 16 * static_cast<int64_t>(i));
+      c[h] = i < n && page >= 0 ? ld_stream8(x + kVec * static_cast<int64_t>(i)) : make_uint2(0u, 0u);
     }
 #pragma unroll
     for (int h = 0; h < kHold; ++h) {
       const int i = i0 + h * n_threads;
-      if (i >= chunks) continue;
-      const uint32_t in4[4] = {c[h].x, c[h].y, c[h].z, c[h].w};
-      uint32_t out8[8];
+      if (i >= n) continue;
+      const uint32_t in2[2] = {c[h].x, c[h].y};
+      uint32_t out4[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 2; ++k) {
         uint32_t lo, hi;
-        fp8_to_half4<kE5M2>(in4[k], lo, hi);
+        fp8_to_half4<kE5M2>(in2[k], lo, hi);
         const float2 p = half_pair<false>(lo), q = half_pair<false>(hi);
-        out8[2 * k] = pack_pair<kBf16>(p.x * d, p.y * d);
-        out8[2 * k + 1] = pack_pair<kBf16>(q.x * d, q.y * d);
+        out4[2 * k] = pack_pair<kBf16>(p.x * d, p.y * d);
+        out4[2 * k + 1] = pack_pair<kBf16>(q.x * d, q.y * d);
       }
       const int r = row_of(i, magic);
-      uint16_t* const p = y + r * row + 16 * (i - r * per_row);
-      st_global_v4(p, out8[0], out8[1], out8[2], out8[3]);
-      st_global_v4(p + 8, out8[4], out8[5], out8[6], out8[7]);
+      st_global_v4(y + r * row + kVec * (i - r * per_row), out4[0], out4[1], out4[2], out4[3]);
     }
   }
 }
@@ -250,7 +246,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_re
 struct UnitPlan {
   int64_t units;
   int threads;                       // of a CTA; a warp's unit below that
-  bool warp;
+  bool warp, one;                    // a unit to a warp; no more than a vector a thread
   uint32_t magic;
   cudaLaunchConfig_t cfg;
 };
@@ -260,9 +256,10 @@ bool plan_units(const KvArgs& a, cudaStream_t stream, cudaLaunchAttribute* attr,
   const int mean = a.cu != nullptr ? (a.tokens + a.batch - 1) / a.batch : a.even;
   const int work = (mean < P ? mean : P) * a.head_dim;
   p->warp = work <= kWarpWork;
-  p->threads = p->warp ? 32 * kWarpsPerCta : (work / (kHold * 16) + 31) / 32 * 32;
+  p->one = work <= 32 * kVec;
+  p->threads = p->warp ? 32 * kWarpsPerCta : (work / (kHold * kVec) + 31) / 32 * 32;
   if (p->threads > kMaxThreads) p->threads = kMaxThreads;
-  p->magic = 65536u / static_cast<uint32_t>(a.head_dim / 16) + 1u;
+  p->magic = (1u << 20) / static_cast<uint32_t>(a.head_dim / kVec) + 1u;
   const int64_t ctas = p->warp ? (p->units + kWarpsPerCta - 1) / kWarpsPerCta : p->units;
   if (ctas > 0x7fffffff) return false;
   p->cfg = cudaLaunchConfig_t{};
@@ -280,7 +277,8 @@ cudaError_t append(const KvArgs& a, const KvRows& k, const KvRows& v, cudaStream
   cudaLaunchAttribute attr[1];
   UnitPlan p;
   if (!plan_units(a, stream, attr, &p)) return cudaErrorInvalidConfiguration;
-  return cudaLaunchKernelEx(&p.cfg, p.warp ? &kv_append_kernel<kBf16, kE5M2, true> : &kv_append_kernel<kBf16, kE5M2, false>, a, k, v,
+  return cudaLaunchKernelEx(&p.cfg, p.one ? &kv_append_kernel<kBf16, kE5M2, true, 1>
+                                         : (p.warp ? &kv_append_kernel<kBf16, kE5M2, true, kHold> : &kv_append_kernel<kBf16, kE5M2, false, kHold>), a, k, v,
                             p.units, p.magic);
 }
 
@@ -289,7 +287,7 @@ cudaError_t read(const KvArgs& a, void* k_out, void* v_out, cudaStream_t stream)
   cudaLaunchAttribute attr[1];
   UnitPlan p;
   if (!plan_units(a, stream, attr, &p)) return cudaErrorInvalidConfiguration;
-  return cudaLaunchKernelEx(&p.cfg, p.warp ? &kv_read_kernel<kBf16, kE5M2, true> : &kv_read_kernel<kBf16, kE5M2, false>, a,
+  return cudaLaunchKernelEx(&p.cfg, p.warp ? &kv_read_kernel<kBf16, kE5M2, true, kHold> : &kv_read_kernel<kBf16, kE5M2, false, kHold>, a,
                             static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out), p.units, p.magic);
 }
 
