@@ -74,7 +74,7 @@ struct KvAttendSizes {
   int64_t keys_most;              // that a sequence can have: table_width * page_size
 };
 // tk, tv: the pools as 3-D byte tensors {kv_map_bytes, page_size * head_dim / kv_map_bytes, num_pages * heads} with a box of
-// kv_box_bytes x kv_box_rows x 1, swizzled over the box's row.
+// kv_box_bytes x min(page_size, the kernel's keys) x 1, swizzled over the box's row.
 cudaError_t launch_kv_attend(const CUtensorMap& tk, const CUtensorMap& tv, KvAttendArgs a, const KvAttendSizes& z, void* workspace,
                              bool e5m2, int sms, cudaStream_t stream);
 int64_t kv_attend_workspace(const KvAttendSizes& z, int sms);
@@ -93,20 +93,19 @@ cudaError_t launch_kv_prefill(const CUtensorMap& tk, const CUtensorMap& tv, cons
                               bool e5m2, int sms, cudaStream_t stream);
 // Whether a call is one for launch_kv_prefill.
 bool kv_prefill_takes(const KvAttendSizes& z);
-// Keys of a step of the kernel built for head dims up to `width`; the bytes of a row of the pools' maps (rows of 64 bytes are taken
-// two at a time) and of a box, and a box's rows: a step's keys, or a page's.
+// Bytes of a row of the pools' maps (rows of 64 bytes are taken two at a time) and of a box; keys of a box: those that a kernel copies at a
+// time (a step of the kernel for few rows, 32 or, at head dims above 128, 16 in the other), or a page's.
 #ifdef __CUDACC__
 #define FA8_HD __host__ __device__
 #else
 #define FA8_HD
 #endif
-FA8_HD constexpr int kv_step_keys(int width) { return width == 256 ? 16 : 32; }
 FA8_HD constexpr int kv_map_bytes(int head_dim) { return head_dim == 64 ? 128 : head_dim; }
 FA8_HD constexpr int kv_box_bytes(int head_dim) { return head_dim < 64 ? 64 : 128; }
-FA8_HD constexpr int kv_box_keys(int head_dim, int page_size) {
-  return page_size < kv_step_keys(head_dim <= 128 ? 128 : 256) ? page_size : kv_step_keys(head_dim <= 128 ? 128 : 256);
-}
-FA8_HD constexpr int kv_box_rows(int head_dim, int page_size) { return kv_box_keys(head_dim, page_size) * head_dim / kv_map_bytes(head_dim); }
+// Keys of a step of the kernel for few rows, built for head dims up to `width` and blocks of `rows` rows: what the registers hold.
+FA8_HD constexpr int kv_step_keys(int width, int rows) { return width == 256 || (width == 128 && rows == 32) ? 16 : 32; }
+FA8_HD constexpr int kv_prefill_copy_keys(int width) { return width == 256 ? 16 : 32; }
+int kv_attend_step_keys(const KvAttendSizes& z);
 
 // fa8_capi.cu: a 3-D byte tensor {inner, mid, outer} with a {box_inner, box_mid, 1} tile, swizzled over
 // box_inner bytes (64 or 128).  False, with the detail string set, on failure.

@@ -47,7 +47,7 @@ constexpr int kExpiredWait = 0xa77e;                   // code in the status wor
 // Head dims up to W run in the instance built for W (the copies fill what is missing with zeros); RB blocks of eight rows.
 template <int W, int RB>
 struct ACfg {
-  static constexpr int kStepKeys = kv_step_keys(W);              // of a step: 4, 8 and 8 KB of K and V
+  static constexpr int kStepKeys = kv_step_keys(W, 8 * RB);      // of a step: 4 or 8 KB of K and V
   static constexpr int kHalves = kStepKeys / 16;                 // of a step: sixteen keys lie in one page
   static constexpr int kRowBytes = W < 128 ? W : 128;            // of a swizzled tile
   static constexpr int kBlocks = W / kRowBytes;                  // tiles side by side
@@ -56,7 +56,7 @@ struct ACfg {
   // Warps of the one CTA per SM: what the register file holds at this instance's registers per thread (a quarter of the warps
   // share a quarter of it), and stages of each: 180 to 192 KB in all.
   static constexpr int kWarps = W == 64 && RB == 1 ? 16 : (W == 64 && RB == 2 ? 12 : 8);
-  static constexpr int kStages = kWarps == 16 ? 3 : (kWarps == 12 ? 4 : (W == 64 ? 6 : 3));
+  static constexpr int kStages = kWarps == 16 ? 3 : (kWarps == 12 ? 4 : (kStageBytes == 4096 ? 6 : 3));
   static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kChunks = W / 64;                         // 16-byte pieces of a K row per thread
   static constexpr int kSteps = W / 16;                          // k-steps of Q K^T
@@ -914,16 +914,21 @@ int warps_of(const KvAttendSizes& z) {
   }
 }
 
+int step_keys_of(const KvAttendSizes& z) { return kv_step_keys(width_of(z.head_dim), block_rows(z)); }
+
 // A cluster to an item (no second kernel, no workspace) where that leaves no CTA more than kLoneKeys keys, going by what the page
-// table can hold; CTAs of the cluster, or 0.
+// table can hold; CTAs of the cluster, or 0.  Clusters of a launch are to run at once: as a cluster lies within a part of the GPU of
+// 16 to 20 SMs, and a CTA takes an SM, no more than one of eight per sixteen SMs is counted on (sixteen of them: 27 us, where eight
+// take 14 and 32 of four 15: B1 H32 Hk8 D128, 1000 keys), and of four as many as fill seven eighths of the SMs.
 constexpr int64_t kLoneKeys = 1024;
 int lone_split(const KvAttendSizes& z, int sms) {
   const int group = z.heads_q / z.heads, rows = block_rows(z);
   if (group > rows) return 0;
   const int64_t items = kv_slots(z.batch, z.tokens, z.tokens / z.batch, z.ragged, rows / group, 1) * z.heads;
+  const int64_t steps = (z.keys_most + step_keys_of(z) - 1) / step_keys_of(z);
   int split = 1;
-  const int64_t steps = (z.keys_most + kv_step_keys(width_of(z.head_dim)) - 1) / kv_step_keys(width_of(z.head_dim));
-  while (split < 8 && 2 * split * items <= sms && split * warps_of(z) < steps) split *= 2;
+  for (const int n : {2, 4, 8})
+    if (n * items <= (n == 8 ? sms / 2 : (n == 4 ? sms * 7 / 8 : sms)) && n / 2 * warps_of(z) < steps) split = n;
   return z.keys_most <= kLoneKeys * split && items <= 2 * sms ? split : 0;
 }
 
@@ -978,6 +983,8 @@ int64_t records_bytes(int sms) { return (static_cast<int64_t>(sms) * sizeof(KvRe
 
 }  // namespace
 
+int kv_attend_step_keys(const KvAttendSizes& z) { return step_keys_of(z); }
+
 int64_t kv_attend_workspace(const KvAttendSizes& z, int sms) {
   if (lone_split(z, sms) > 0) return 0;
   const int64_t slots = static_cast<int64_t>(sms) * (2 + warps_of(z));
@@ -991,7 +998,7 @@ cudaError_t launch_kv_attend(const CUtensorMap& tk, const CUtensorMap& tv, KvAtt
   const int rows = block_rows(z);
   a.n_split = lone_split(z, sms);
   // units of all items together are a 31-bit number
-  const int step_keys = kv_step_keys(width_of(a.c.head_dim));
+  const int step_keys = step_keys_of(z);
   const double items = (static_cast<double>(z.tokens) * a.group / rows + z.batch) * z.heads;
   a.unit_shift = 0;
   while (items * ((static_cast<double>(z.keys_most) / step_keys) / (1 << a.unit_shift) + 2 + kStartUnits) > 1e9 && a.unit_shift < 30) ++a.unit_shift;

@@ -151,36 +151,38 @@ int fa8_kv_attention(const fa8_kv_attention_params* p, void* cuda_stream) {
                              static_cast<int64_t>(a.c.table_width) << a.c.page_shift};
   const int64_t need = workspace_of(z, sms);
   if (need > 0 && (!p->workspace || !aligned(p->workspace, 256) || p->workspace_bytes < need)) return FA8_ERR_BAD_ARG;
-  // The pool's tensor maps depend on its address and shape only: a thread keeps those of its last call.
+  // The pool's tensor maps depend on its address and shape, and on what the kernel copies at a time: a thread keeps those of its last call.
   struct Maps {
     const void *k, *v;
     int64_t slices;
-    int32_t page_size, head_dim;
+    int32_t page_size, head_dim, keys;
     bool valid;
     CUtensorMap tk, tv;
   };
   thread_local Maps m{};
   const fa8_kv_cache& c = p->cache;
+  const bool prefill = fa8::kv_prefill_takes(z);
   const int64_t slices = static_cast<int64_t>(c.num_pages) * c.heads_kv;
-  if (!(m.valid && m.k == c.k && m.v == c.v && m.slices == slices && m.page_size == c.page_size && m.head_dim == c.head_dim)) {
+  const int32_t keys = std::min(c.page_size, prefill ? fa8::kv_prefill_copy_keys(c.head_dim <= 128 ? 128 : 256) : fa8::kv_attend_step_keys(z));
+  if (!(m.valid && m.k == c.k && m.v == c.v && m.slices == slices && m.page_size == c.page_size && m.head_dim == c.head_dim && m.keys == keys)) {
     m.valid = false;
-    const uint32_t inner = static_cast<uint32_t>(fa8::kv_box_bytes(c.head_dim)), rows = static_cast<uint32_t>(fa8::kv_box_rows(c.head_dim, c.page_size));
-    const uint64_t row = static_cast<uint64_t>(fa8::kv_map_bytes(c.head_dim));
-    const uint64_t n_rows = static_cast<uint64_t>(c.page_size) * c.head_dim / row;
-    if (!fa8::make_byte_map(&m.tk, c.k, row, n_rows, slices, inner, rows)) return FA8_ERR_CUDA;
-    if (!fa8::make_byte_map(&m.tv, c.v, row, n_rows, slices, inner, rows)) return FA8_ERR_CUDA;
+    const uint64_t row = static_cast<uint64_t>(fa8::kv_map_bytes(c.head_dim)), rows = static_cast<uint64_t>(c.page_size) * c.head_dim / row;
+    const uint32_t inner = static_cast<uint32_t>(fa8::kv_box_bytes(c.head_dim)), box = static_cast<uint32_t>(keys * c.head_dim / row);
+    if (!fa8::make_byte_map(&m.tk, c.k, row, rows, slices, inner, box)) return FA8_ERR_CUDA;
+    if (!fa8::make_byte_map(&m.tv, c.v, row, rows, slices, inner, box)) return FA8_ERR_CUDA;
     m.k = c.k;
     m.v = c.v;
     m.slices = slices;
     m.page_size = c.page_size;
     m.head_dim = c.head_dim;
+    m.keys = keys;
     m.valid = true;
   }
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   if (const int rc = begin(&p->cache, &a.c, stream)) return rc;
   const bool e5m2 = c.fp8_format == FA8_FP8_E5M2;
-  return launched(fa8::kv_prefill_takes(z) ? fa8::launch_kv_prefill(m.tk, m.tv, a, z, p->workspace, e5m2, sms, stream)
-                                           : fa8::launch_kv_attend(m.tk, m.tv, a, z, p->workspace, e5m2, sms, stream));
+  return launched(prefill ? fa8::launch_kv_prefill(m.tk, m.tv, a, z, p->workspace, e5m2, sms, stream)
+                          : fa8::launch_kv_attend(m.tk, m.tv, a, z, p->workspace, e5m2, sms, stream));
 }
 
 }  // extern "C"

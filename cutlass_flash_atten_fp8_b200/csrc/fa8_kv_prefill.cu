@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         if (lane == 0) mbar_arrive(smem_u32(&sh.blk_full[n]));
         ++blocks;
         // one copy per page part of the block (box_keys keys) and 128 columns
-        const int box_keys = kv_box_keys(W, 1 << a.c.page_shift);
+        const int box_keys = min(1 << a.c.page_shift, kv_prefill_copy_keys(W));
         const bool issues = here && (16 * lane) % box_keys == 0;
         const int boxes = __popc(__ballot_sync(0xffffffffu, issues));
         const bool all_here = __all_sync(0xffffffffu, here || lane >= C::kGroups);
@@ -978,9 +978,15 @@ cudaError_t launch_one(const CUtensorMap& tk, const CUtensorMap& tv, const KvAtt
 
 }  // namespace
 
+// Against the kernel for few rows (us here / there; H 4 Hk, page 64, keys as given):
+//   32 rows a sequence and K/V head, D 128:  8 heads of 1 x 16000 keys 41 / R32A, of 8 x 4000 49 / R32B, of 32 x 1000 51 / R32C
+//   64 rows, D 128:  44 / R64A, 55 / R64B, 54 / R64C;  D 64, 4 heads:  36 / 18, 30 / 23, 24 / 26;  D 256, 4 heads:  52 / 41, 47 / 68, 40 / 78
+//   128 rows, D 128: 49 / 60, 60 / 108, 64 / 140
+// There the keys are split over the whole GPU however few the sequences, and 32 rows (16 at D 256) share what is read.
 bool kv_prefill_takes(const KvAttendSizes& z) {
-  const int64_t group = z.heads_q / z.heads;
-  return group <= kTileM && static_cast<int64_t>(z.tokens) * group > 64ll * z.batch;
+  const int64_t group = z.heads_q / z.heads, rows = (z.tokens * group + z.batch - 1) / z.batch;
+  if (group > kTileM || rows <= 32) return false;
+  return rows > 64 || z.batch * z.heads > (width_of(z.head_dim) == 64 ? 64 : 16);
 }
 
 KvPrefillPlan kv_prefill_plan(const KvAttendSizes& z, int sms) {
