@@ -91,7 +91,8 @@ struct Shared {
   uint64_t ring_full[C::kRing], ring_empty[C::kRing];
   uint64_t q_full[2], s_full[2][2], p_full[2][2], o_final[2], o_done;        // by tile, and score buffer
   uint64_t blk_full[kBlockSlots];
-  uint64_t drain;
+  uint64_t drain, given;
+  uint4 answer;                          // to the request for another CTA's item
   Item item[kItemSlots];                 // seq < 0: no more
   uint32_t factor[C::kRaw][C::kGroups];  // fp16 pair to multiply a group of 16 keys by
   int valid[C::kRaw];                    // rows of the tile that are keys
@@ -129,6 +130,19 @@ __device__ __forceinline__ bool wait_bounded(const Wait& w, uint64_t* barrier, u
       }
     }
   }
+}
+
+// Takes over the work of a CTA of this grid that has not started (there is one to an item): the answer arrives at `bar`.
+__device__ __forceinline__ void ask_for_cta(uint32_t answer, uint32_t bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+// Its number, or -1: all have started or been taken, and there must be no further request.
+__device__ __forceinline__ int taken_cta(uint32_t answer) {
+  uint32_t id;
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b128 a;\n\tld.shared.b128 a, [%1];\n\t"
+               "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\tmov.u32 %0, 0xffffffff;\n\t"
+               "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, a;\n\t}" : "=r"(id) : "r"(answer) : "memory");
+  return static_cast<int>(id);
 }
 
 // kind::f16 products: D[tmem] (+)= A B, fp16 operands, fp32 sums.
@@ -288,6 +302,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     init(sh.o_final, 2, 1);
     init(sh.blk_full, kBlockSlots, 1);
     init(&sh.drain, 1, 1);
+    init(&sh.given, 1, 1);
     sh.abort = 0;
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -330,11 +345,10 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
   if constexpr (C::kDeal) setmaxnreg_dec<C::kOtherRegs>();
   if (warp == C::kLoadWarp) {
     // ---------------------------------------------------------------- producer
-    bool ok = true;
     uint32_t tiles = 0, blocks = 0;                              // raw tiles and blocks filled so far
-    if (blockIdx.x == 0)                                         // a bad range has no rows that would find it
-      for (int b = lane; b < a.c.batch; b += 32)
-        if (kv_seq(a.c, b).bad) report_bad_index(a.c);
+    // once a wait has run out, the CTAs that are still to come have nothing to do
+    const int before = a.c.status ? *static_cast<volatile int*>(a.c.status) : 0;
+    bool ok = true, more = before == 0 || before == kBadIndex, asked = false;
     auto push = [&](const Item& it) {
       const int slot = n_items % kItemSlots;
       ok = wait_bounded(wctx, &sh.item_empty[slot], ((n_items / kItemSlots) & 1) ^ 1, 0xb200);
@@ -346,12 +360,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       }
       ++n_items;
     };
-    for (int64_t round = 0; ok; ++round) {
-      // a round deals one item to each CTA, every other one in the opposite order: the heavier ones come first
-      const int64_t at = (round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-      if (round * gridDim.x >= plan.items) break;
-      const int64_t id = round * gridDim.x + at;
-      if (id >= plan.items) continue;
+    auto load_item = [&](int64_t id) {
       Item it;
       const int64_t sh_id = id / plan.parts;
       it.part = static_cast<int>(id - sh_id * plan.parts);
@@ -361,7 +370,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       kv_find_slot(a.c, slot, plan.block_tokens, 1, &it.seq, &j);
       const KvSeq s = kv_seq(a.c, it.seq);
       const int tiles_of = (s.n + plan.block_tokens - 1) / plan.block_tokens;
-      if (j >= tiles_of) continue;
+      if (j >= tiles_of) return;
       it.first = s.first;
       it.n = s.n;
       it.len = s.len;
@@ -371,9 +380,9 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       const int n_blk = max(1, (it.vis + C::kN - 1) / C::kN);
       it.blk0 = static_cast<int>(static_cast<int64_t>(n_blk) * it.part / plan.parts);
       it.blk1 = static_cast<int>(static_cast<int64_t>(n_blk) * (it.part + 1) / plan.parts);
-      if (it.blk0 == it.blk1) continue;
+      if (it.blk0 == it.blk1) return;
       push(it);
-      if (!ok) break;
+      if (!ok) return;
 
       // Lane g < kGroups looks after the g-th sixteen keys of a block: page numbers are loaded two blocks ahead, scales one.
       const int* const table = a.c.table + static_cast<int64_t>(it.seq) * a.c.table_stride;
@@ -461,6 +470,32 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         kd = kd1;
         vd = vd1;
       }
+    };
+    uint32_t answers = 0;
+    // A CTA to an item is launched; those on the GPU take over the others, one after another, as they get through their own, so that
+    // all end together whatever the items' lengths (dealt out in turns, 148 CTAs differed by a fifth at 2048 and 4096 new tokens).
+    for (int64_t id = blockIdx.x; ok && more;) {
+      if (id == 0)                                               // a bad range has no rows that would find it
+        for (int b = lane; b < a.c.batch; b += 32)
+          if (kv_seq(a.c, b).bad) report_bad_index(a.c);
+      load_item(id);
+      // One item waits while one is worked on, no more: others may be through before.
+      if (ok && n_items > 0) ok = wait_bounded(wctx, &sh.item_empty[(n_items - 1) % kItemSlots], ((n_items - 1) / kItemSlots) & 1, 0xb200);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) {
+        fence_proxy_async_smem();                                // the last answer has been read
+        mbar_arrive_expect_tx(smem_u32(&sh.given), 16);
+        ask_for_cta(smem_u32(&sh.answer), smem_u32(&sh.given));
+      }
+      asked = true;
+      ok = __all_sync(0xffffffffu, wait_bounded(wctx, &sh.given, answers & 1, 0xb210));
+      if (!ok) break;
+      asked = false;
+      ++answers;
+      id = taken_cta(smem_u32(&sh.answer));
+      more = id >= 0;
+      __syncwarp();
     }
     if (ok) {
       Item none{};
@@ -468,7 +503,11 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       push(none);
     }
     if (!ok) {
-      // copies in flight land before the CTA's memory is given back (a wait each, with a limit)
+      // copies in flight, and an answer, land before the CTA's memory is given back (a wait each, with a limit)
+      if (asked) {
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(smem_u32(&sh.given), answers & 1) && global_timer_ns() - t0 < 20000000ull) {}
+      }
       for (uint32_t i = tiles > C::kRaw ? tiles - C::kRaw : 0; i < tiles; ++i) {
         const uint64_t t0 = global_timer_ns();
         while (!mbar_try_wait(smem_u32(&sh.raw_full[i % C::kRaw]), (i / C::kRaw) & 1) && global_timer_ns() - t0 < 20000000ull) {}
@@ -944,7 +983,7 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a, cons
 int width_of(int head_dim) { return head_dim <= 64 ? 64 : (head_dim <= 128 ? 128 : 256); }
 
 template <int W, bool kE5M2>
-cudaError_t launch_one(const CUtensorMap& tk, const CUtensorMap& tv, const KvAttendArgs& a, const KvPrefillPlan& plan, int sms, cudaStream_t stream) {
+cudaError_t launch_one(const CUtensorMap& tk, const CUtensorMap& tv, const KvAttendArgs& a, const KvPrefillPlan& plan, cudaStream_t stream) {
   using C = PCfg<W>;
   auto kernel = &kv_prefill_kernel<W, kE5M2>;
   constexpr int smem = C::kSharedOffset + static_cast<int>(sizeof(Shared<W>));
@@ -960,7 +999,7 @@ cudaError_t launch_one(const CUtensorMap& tk, const CUtensorMap& tv, const KvAtt
     if (cached) ready[dev].store(true, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(plan.items < sms ? plan.items : sms), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(plan.items), 1, 1);      // below 2^31 / 32: kv_prefill_takes wants 33 rows a sequence
   cfg.blockDim = dim3(C::kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -1018,9 +1057,9 @@ cudaError_t launch_kv_prefill(const CUtensorMap& tk, const CUtensorMap& tv, cons
     p.partial_ml = p.partial_o + static_cast<int64_t>(p.parts) * z.tokens * z.heads_q * z.head_dim;
   }
   switch (width_of(a.c.head_dim)) {
-    case 64: return e5m2 ? launch_one<64, true>(tk, tv, a, p, sms, stream) : launch_one<64, false>(tk, tv, a, p, sms, stream);
-    case 128: return e5m2 ? launch_one<128, true>(tk, tv, a, p, sms, stream) : launch_one<128, false>(tk, tv, a, p, sms, stream);
-    default: return e5m2 ? launch_one<256, true>(tk, tv, a, p, sms, stream) : launch_one<256, false>(tk, tv, a, p, sms, stream);
+    case 64: return e5m2 ? launch_one<64, true>(tk, tv, a, p, stream) : launch_one<64, false>(tk, tv, a, p, stream);
+    case 128: return e5m2 ? launch_one<128, true>(tk, tv, a, p, stream) : launch_one<128, false>(tk, tv, a, p, stream);
+    default: return e5m2 ? launch_one<256, true>(tk, tv, a, p, stream) : launch_one<256, false>(tk, tv, a, p, stream);
   }
 }
 
