@@ -43,10 +43,11 @@ template <int W>
 struct PCfg {
   static constexpr int kTiles = W == 256 ? 1 : 2;
   static constexpr int kN = W == 256 ? 64 : 128;               // keys of a block
-  // Score buffers of a tile: one where two tiles take turns.  (Two of 64 keys each for the tiles of head dim 128 would keep a
-  // tile's scores ahead of its softmax, but a product of N = 64 is bound by reading Q: 80 cycles a step of 16 against 64 for N = 128,
-  // 327 us against 26x for 1024 tokens and 16384 keys.)
-  static constexpr int kBufs = kTiles == 2 ? 1 : 2;
+  // Score buffers, which the blocks of both tiles take in turn: what tensor memory holds beside O.  The scores of a block go out kBufs
+  // blocks ahead, so a tile whose turn it is finds its next scores ready when there are more buffers than tiles.  (Four of 64 keys
+  // would do that at head dim 128, but a product of N = 64 is bound by reading Q: 80 cycles a step of 16 against 64 for N = 128,
+  // and 1024 tokens over 16384 keys took R64N us against R128N.)
+  static constexpr int kBufs = W == 64 ? 3 : 2;
   static constexpr int kGroups = kN / 16;                      // of keys that share a page
   static constexpr int kCols = W / 64;                         // column blocks of 64 fp16 (128 bytes)
   static constexpr int kRawRow = W < 128 ? W : 128;            // bytes of a row of a raw (fp8) tile
@@ -57,21 +58,21 @@ struct PCfg {
   static constexpr int kRing = 4;                              // widened tiles
   static constexpr int kRingBytes = kN * W * 2;
   static constexpr int kQBytes = kTileM * W * 2;               // of a tile
-  // Columns of tensor memory: a tile's score buffers (P over them), then its O.
-  static constexpr int kOCol = kN * kBufs, kTileCols = kOCol + W;
+  // Columns of tensor memory: the score buffers (P over them), then O of each tile.
+  static constexpr int kOCol = kN * kBufs;
   static constexpr int kSoftWarps = 8 * kTiles;
   static constexpr int kWideWarp0 = kSoftWarps;
   static constexpr int kLoadWarp = kWideWarp0 + 4;
   static constexpr int kMmaWarp = kLoadWarp + 1;
-  // Whole warpgroups (two warps stand by), so that registers can be dealt out anew: 512 * 88 + 128 * 72 + 128 * 56 = 768 * 80.
+  // Whole warpgroups (two warps stand by), so that registers can be dealt out anew: 512 * 96 + 128 * 48 + 128 * 48 = 768 * 80.
   static constexpr bool kDeal = kTiles == 2;
   static constexpr int kThreads = 32 * (kLoadWarp + 4);
-  static constexpr uint32_t kSoftRegs = 88, kWideRegs = 72, kOtherRegs = 56;
+  static constexpr uint32_t kSoftRegs = 96, kWideRegs = 48, kOtherRegs = 48;
   static_assert(!kDeal || 32 * kSoftWarps * kSoftRegs + 128 * (kWideRegs + kOtherRegs) <= kThreads * 80, "registers of the launch");
   static constexpr int kRawOffset = kTiles * kQBytes;
   static constexpr int kRingOffset = kRawOffset + kRaw * kRawBytes;
   static constexpr int kSharedOffset = kRingOffset + kRing * kRingBytes;
-  static_assert(kTileCols * kTiles <= 512, "tensor memory");
+  static_assert(kOCol + W * kTiles <= 512, "tensor memory");
 };
 
 struct Item {
@@ -89,7 +90,8 @@ struct Shared {
   uint64_t item_full[kItemSlots], item_empty[kItemSlots];
   uint64_t raw_full[C::kRaw], raw_empty[C::kRaw];
   uint64_t ring_full[C::kRing], ring_empty[C::kRing];
-  uint64_t q_full[2], s_full[2][2], p_full[2][2], o_final[2], o_done;        // by tile, and score buffer
+  uint64_t s_full[C::kBufs], p_full[C::kBufs];
+  uint64_t q_full[2], o_done[2], o_final[2];     // by tile
   uint64_t blk_full[kBlockSlots];
   uint64_t drain, given;
   uint4 answer;                          // to the request for another CTA's item
@@ -296,9 +298,9 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     init(sh.ring_full, C::kRing, 4);
     init(sh.ring_empty, C::kRing, 1);
     init(sh.q_full, 2, 8);
-    init(&sh.s_full[0][0], 4, 1);
-    init(&sh.p_full[0][0], 4, 8);
-    init(&sh.o_done, 1, 1);
+    init(sh.s_full, C::kBufs, 1);
+    init(sh.p_full, C::kBufs, 8);
+    init(sh.o_done, 2, 1);
     init(sh.o_final, 2, 1);
     init(sh.blk_full, kBlockSlots, 1);
     init(&sh.drain, 1, 1);
@@ -522,23 +524,21 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       bool ok = true;
       uint32_t ld = 0;                                           // widened tiles used so far: K, V, K, V ...
       uint32_t qn[2] = {0, 0};                                   // q_full phases by tile
-      uint32_t pn[2] = {0, 0};                                   // blocks by tile
+      uint32_t turns = 0;                                        // of the score buffers, before this item
       auto ring_wait = [&](uint32_t i) { return wait_bounded(wctx, &sh.ring_full[i % C::kRing], (i / C::kRing) & 1, 0xb400); };
       auto ring_release = [&](uint32_t i) { tc_commit(smem_u32(&sh.ring_empty[i % C::kRing])); };
       auto issue_qk = [&](int tile, uint32_t b, uint32_t i) {
         const uint32_t kk = k_lo + (i % C::kRing) * (C::kRingBytes / 16), qq = q_lo + tile * (C::kQBytes / 16);
 #pragma unroll
         for (int k = 0; k < W / 16; ++k)
-          mma_f16_ss(tmem + C::kTileCols * tile + C::kN * b, desc(qq + (k >> 2) * kColQ + 2 * (k & 3)), desc(kk + (k >> 2) * kColK + 2 * (k & 3)),
-                     kIdescQK, k > 0);
-        tc_commit(smem_u32(&sh.s_full[tile][b]));
+          mma_f16_ss(tmem + C::kN * b, desc(qq + (k >> 2) * kColQ + 2 * (k & 3)), desc(kk + (k >> 2) * kColK + 2 * (k & 3)), kIdescQK, k > 0);
+        tc_commit(smem_u32(&sh.s_full[b]));
       };
       auto issue_pv = [&](int tile, uint32_t b, uint32_t i, bool more) {
         const uint32_t vv = v_lo + (i % C::kRing) * (C::kRingBytes / 16);
 #pragma unroll
         for (int k = 0; k < C::kN / 16; ++k)
-          mma_f16_ts(tmem + C::kTileCols * tile + C::kOCol, tmem + C::kTileCols * tile + C::kN * b + 8 * k, desc(vv + k * 128), kIdescPV, more || k > 0);
-        if (C::kBufs > 1) tc_commit(smem_u32(&sh.o_done));
+          mma_f16_ts(tmem + C::kOCol + W * tile, tmem + C::kN * b + 8 * k, desc(vv + k * 128), kIdescPV, more || k > 0);
       };
       Item it;
       while (ok && (ok = next_item(it))) {
@@ -546,35 +546,39 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         if (it.seq < 0) break;
         const int n = it.blk1 - it.blk0;
         const int nt = C::kTiles == 2 && it.n_tokens > tile_tokens ? 2 : 1;
-        // The scores run kBufs blocks ahead: S(j + kBufs) goes into the buffer that P V (j) has read.
-        for (int j = -C::kBufs; j < n && ok; ++j) {
-          const uint32_t lv = ld + 2 * j + 1, lk = ld + 2 * (j + C::kBufs);
-          const bool qk = j + C::kBufs < n;
-          if (j >= 0) ok = ring_wait(lv);
-          for (int i = 0; i < nt && ok; ++i) {
-            const uint32_t b = (pn[i] + j) % C::kBufs;
-            if (j >= 0) {
-              ok = wait_bounded(wctx, &sh.p_full[i][b], ((pn[i] + j) / C::kBufs) & 1, 0xb600 + 2 * i + b);
-              if (!ok) break;
-              tc_fence_after();
-              issue_pv(i, b, lv, j > 0);
-              if (j + 1 == n) tc_commit(smem_u32(&sh.o_final[i]));
-            } else if (j == -C::kBufs) {
-              ok = wait_bounded(wctx, &sh.q_full[i], qn[i]++ & 1, 0xb500 + i);
-              if (!ok) break;
-            }
-            if (qk) {
-              if (i == 0) ok = ring_wait(lk);
-              if (!ok) break;
-              tc_fence_after();
-              issue_qk(i, b, lk);
+        // Turn t is block t / nt of tile t % nt; the scores run kBufs turns ahead: S(t + kBufs) goes into the buffer that P V (t) has read.
+        int tile_v = 0, blk_v = 0, tile_k = 0, blk_k = 0;
+        for (int t = -C::kBufs; t < n * nt && ok; ++t) {
+          if (t >= 0) {
+            const uint32_t turn = turns + t, b = turn % C::kBufs, lv = ld + 2 * blk_v + 1;
+            if (tile_v == 0) ok = ring_wait(lv);
+            if (ok) ok = wait_bounded(wctx, &sh.p_full[b], (turn / C::kBufs) & 1, 0xb600 + b);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(tile_v, b, lv, blk_v > 0);
+            if (nt < C::kBufs) tc_commit(smem_u32(&sh.o_done[tile_v]));      // otherwise the tile's next scores come after it
+            if (blk_v + 1 == n) tc_commit(smem_u32(&sh.o_final[tile_v]));
+            if (++tile_v == nt) {
+              ring_release(lv);
+              tile_v = 0;
+              ++blk_v;
             }
           }
-          if (!ok) break;
-          if (j >= 0) ring_release(lv);
-          if (qk) ring_release(lk);
+          if (blk_k < n) {
+            const uint32_t b = (turns + t + C::kBufs) % C::kBufs, lk = ld + 2 * blk_k;
+            if (blk_k == 0) ok = wait_bounded(wctx, &sh.q_full[tile_k], qn[tile_k]++ & 1, 0xb500 + tile_k);
+            if (ok && tile_k == 0) ok = ring_wait(lk);
+            if (!ok) break;
+            tc_fence_after();
+            issue_qk(tile_k, b, lk);
+            if (++tile_k == nt) {
+              ring_release(lk);
+              tile_k = 0;
+              ++blk_k;
+            }
+          }
         }
-        for (int i = 0; i < nt; ++i) pn[i] += n;
+        turns += n * nt;
         ld += 2 * n;
       }
       {
@@ -622,19 +626,23 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           st_shared16(to + (((2 * q + 1) ^ r8) << 4), hi);
         };
         if (sh.complete[st]) {
-          // all loads go out before the first is used
-          uint4 x[kMine];
-          uint32_t f[kMine];
+          // four loads go out before the first is used
 #pragma unroll
-          for (int k = 0; k < kMine; ++k) {
-            x[k] = ld_shared16(from(w + 4 * k));
-            f[k] = sh.factor[st][(w + 4 * k) / C::kCols / 2];
-          }
+          for (int k0 = 0; k0 < kMine; k0 += 4) {
+            uint4 x[4];
+            uint32_t f[4];
 #pragma unroll
-          for (int k = 0; k < kMine; ++k) {
-            uint4 lo, hi;
-            widen16<kE5M2>(x[k], f[k], lo, hi);
-            put(w + 4 * k, lo, hi);
+            for (int k = 0; k < 4; ++k) {
+              const int p = w + 4 * (k0 + k);
+              x[k] = ld_shared16(from(p));
+              f[k] = sh.factor[st][p / C::kCols / 2];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint4 lo, hi;
+              widen16<kE5M2>(x[k], f[k], lo, hi);
+              put(w + 4 * (k0 + k), lo, hi);
+            }
           }
         } else {
 #pragma unroll 1
@@ -659,7 +667,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     // Two warps to 32 rows (lanes of tensor memory): each takes half of a block's keys, of O's columns and of the rows of Q.
     const int tile = warp / 8, sub = warp % 4, part = warp / 4 % 2;
     const uint32_t lanes = static_cast<uint32_t>(32 * sub) << 16;
-    const uint32_t t_tile = tmem + lanes + C::kTileCols * tile, t_o = t_tile + C::kOCol + part * (W / 2);
+    const uint32_t t_o = tmem + lanes + C::kOCol + W * tile + part * (W / 2);
     constexpr int kMyKeys = C::kN / 2, kMyCols = W / 2;
     const int r = 32 * sub + lane;                               // this thread's row
     const int pair_bar = 1 + tile * 4 + sub;
@@ -689,7 +697,8 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       return part == 1 ? y : *p;
     };
     uint32_t blocks = 0;                                         // of all items (the residual ring), also those this tile sits out
-    uint32_t mine = 0;                                           // blocks this tile took part in
+    uint32_t turns = 0;                                          // of the score buffers, before this item
+    uint32_t ahead = 0;                                          // blocks of this tile in items whose scores run ahead
     uint32_t taken = 0;                                          // items this tile took part in
     Item it;
     bool ok = true;
@@ -703,8 +712,10 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       const int nb = it.blk1 - it.blk0;
       const int tok0 = it.token0 + tile * tile_tokens;
       const int n_rows = min(tile_tokens, it.n_tokens - tile * tile_tokens) * group;
+      const int nt = C::kTiles == 2 && it.n_tokens > tile_tokens ? 2 : 1;
       if (n_rows <= 0) {
         blocks += nb;
+        turns += nb;
         continue;
       }
       const int D = a.c.head_dim;
@@ -763,12 +774,12 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       row.lim = a.causal ? max(0, min(it.len, it.len - it.n + my_token + 1)) : it.len;
       const int least = a.causal ? max(0, min(it.len, it.len - it.n + tok0 + 1)) : it.len;       // of the tile's first row
       float vref = 1.f;
-      for (int j = 0; j < nb && ok; ++j, ++mine) {
-        const int buf = mine % C::kBufs;
+      for (int j = 0; j < nb && ok; ++j, ahead += nt < C::kBufs) {
+        const uint32_t turn = turns + j * nt + tile, buf = turn % C::kBufs;
         const uint32_t n = (blocks + j) % kBlockSlots;
-        const uint32_t t_s = t_tile + C::kN * buf + part * kMyKeys;
+        const uint32_t t_p = tmem + lanes + C::kN * buf, t_s = t_p + part * kMyKeys;
         ok = wait_bounded(wctx, &sh.blk_full[n], ((blocks + j) / kBlockSlots) & 1, 0xb900);
-        if (ok) ok = wait_bounded(wctx, &sh.s_full[tile][buf], (mine / C::kBufs) & 1, 0xba00 + buf);
+        if (ok) ok = wait_bounded(wctx, &sh.s_full[buf], (turn / C::kBufs) & 1, 0xba00 + buf);
         __syncwarp();
         tc_fence_after();
         const int key0 = (it.blk0 + j) * C::kN, lim = row.lim - key0 - part * kMyKeys;
@@ -819,7 +830,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           }
           if (!any || raised) break;
           // Some row has outgrown its reference (or holds a NaN): take this block's maximum in and rescale O, for which the products
-          // before have to be done (with one buffer they are: this block's scores came after them).
+          // before have to be done (they are, when this block's scores came after them).
           raised = true;
           const float mine_top = top_of() - kHeadroom, top = over ? mine_top : -INFINITY;
           const float m = fmaxf(fmaxf(row.m, top), exchange(top));
@@ -830,7 +841,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           row.most = m == -INFINITY ? 0.f : kRaiseAbove;
           row.l *= alpha;
           if (j > 0) {
-            if (C::kBufs > 1) ok = wait_bounded(wctx, &sh.o_done, (mine - 1) & 1, 0xbb00) && ok;
+            if (nt < C::kBufs) ok = wait_bounded(wctx, &sh.o_done[tile], (ahead - 1) & 1, 0xbb00 + tile) && ok;
             __syncwarp();
             tc_fence_after();
             rescale(t_o, kMyCols, alpha);
@@ -838,14 +849,15 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         }
         if (!ok) break;
         row.l += l;
-        if constexpr (kMyKeys == 64) tmem_st_32x32b_x32(t_tile + C::kN * buf + part * 32, pk);       // over the scores
-        else tmem_st_32x32b_x16(t_tile + C::kN * buf + part * 16, pk);
+        if constexpr (kMyKeys == 64) tmem_st_32x32b_x32(t_p + part * 32, pk);       // over the scores
+        else tmem_st_32x32b_x16(t_p + part * 16, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[tile][buf]));
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[buf]));
       }
       blocks += nb;
+      turns += nb * nt;
       if (!ok) break;
 
       // ---- O ----
