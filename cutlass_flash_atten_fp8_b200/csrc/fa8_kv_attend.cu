@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
   __shared__ __align__(16) float s_scale[kWarps * C::kStages][4];
   // the first unit of the item that a warp's last, and (where it had several) its first segment is of; -1: whole items only
   __shared__ int s_last[kWarps], s_head[kWarps];
-  __shared__ bool s_single[kWarps];
+  __shared__ bool s_single[kWarps], s_nan[kWarps];       // (s_nan: NaNs were taken out of the segment's V)
   __shared__ Segment s_item[kLone ? 1 : kWarps];
   __shared__ float s_m[C::kRows], s_l[C::kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
   // partial sums of warp w: [row][column], then the rows' references and sums
   auto part_of = [&](int w) { return reinterpret_cast<float*>(smem_raw + (ring0 - smem_u32(smem_raw)) + w * C::kRingBytes); };
   if (lane == 0) {
+    s_nan[warp] = false;
     for (int i = 0; i < C::kStages; ++i) mbar_init(bars + 8 * i, 1);
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -157,17 +158,17 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
   // ---- what this warp has to do: units [pos, end) of the call's (kLone: steps of the item's) ----
   int pos, end, at = 0, cta_lo = 0, cta_hi = 0, share = 1;
   int seq = 0, lone_row0 = 0, lone_head = 0;
-  KvSeq s;
+  KvSeq s{0, 0, 0, false};
   int steps, items;
   if constexpr (kLone) {
     const int rank = static_cast<int>(blockIdx.x) % a.n_split, id = static_cast<int>(blockIdx.x) / a.n_split;
     const int slot = id / a.c.heads;
     lone_head = id - slot * a.c.heads;
     int j;
+    const bool bad = warp == 0 && kv_bad(a.c, blockIdx.x, false);      // there are more CTAs than sequences
     kv_find_slot(a.c, slot, a.block_tokens, 1, &seq, &j);
     s = kv_seq(a.c, seq);
-    if (s.bad && warp == 0 && lane == 0) report_bad_index(a.c);
-    // (a range that is out of range has n = 0 and so no items, but has slots: some CTA comes here for it)
+    if (bad) report_bad_index(a.c);
     const int64_t token0 = static_cast<int64_t>(j) * a.block_tokens;
     if (token0 >= s.n) return;                           // the whole cluster
     lone_row0 = static_cast<int>(token0) * a.group;
@@ -200,7 +201,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
     end = pos + each + (warp < rest ? 1 : 0);
     // The sequence that pos is in.  (A warp without steps may stand behind the last one: it looks where the CTA begins.)
     const int from = pos < end ? pos : cta_lo;
-    for (int b0 = 0;; b0 += 32) {
+    for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
       KvSeq x = mine;
       int u = units;
       if (b0 > 0) {
@@ -227,6 +228,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
     }
     steps = item_steps(s, kStepKeys);
     items = row_blocks(s, a.group, C::kRows) * a.c.heads;
+    if (items == 0) end = pos;                           // lengths that changed since they were added up
   }
 
   // This CTA has the last part of an item that begins at `item_at`: what the combining kernel needs to know.
@@ -254,7 +256,8 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       const int units = item_units(a, steps);
       if (pos >= at + items * units) {                     // the next sequence that has items
         at += items * units;
-        s = kv_seq(a.c, ++seq);
+        if (++seq >= a.c.batch) break;                     // lengths that changed since they were added up
+        s = kv_seq(a.c, seq);
         steps = item_steps(s, kStepKeys);
         items = row_blocks(s, a.group, C::kRows) * a.c.heads;
         continue;
@@ -557,6 +560,20 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
           pb[b][2 * i + 1] = pack_half2(p[2], p[3]);
         }
       }
+      if (!whole && least < vis && key0 + kStepKeys > least) {      // only some rows see all these keys
+#pragma unroll 1
+        for (int i = lane; i < C::kBlocks * C::kTile / 16; i += 32) {
+          const int row = W == 64 ? ((16 * i) ^ ((i & 32) ? flip : 0u)) >> 6 : (i >> 3) % kStepKeys;
+          if (key0 + row >= vis || (kHalves > 1 && row >= 16 ? kd[1] : kd[0]) == -1.f) continue;
+          uint4 v = ld_shared16(sv + 16 * i);
+          if (drop_nans<kE5M2>(v)) {
+            s_nan[warp] = true;
+            st_shared_v4(sv + 16 * i, v.x, v.y, v.z, v.w);
+            fence_proxy_async_smem();                     // before the next copy to this place
+          }
+        }
+        __syncwarp();
+      }
 #pragma unroll
       for (int blk = 0; blk < C::kBlocks; ++blk) {
         uint32_t vr[4 * kHalves][C::kVWords];
@@ -684,6 +701,21 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
           }
         }
       }
+    }
+    __syncwarp();
+    if (s_nan[warp]) {
+#pragma unroll 1
+      for (int in = 0; in < n_rows; ++in) {
+        const int r = row0 + in;
+        uint16_t* const po = static_cast<uint16_t*>(a.o) + (static_cast<int64_t>(s.first + r / a.group) * a.heads_q + h * a.group + r % a.group) * D;
+        write_nans<kE5M2>(a.c, seq, h, max(least / kStepKeys, step0) * kStepKeys, min(seen(r), last * kStepKeys), lane, D, [&](int col) {
+          if (alone) po[col] = 0x7fff;                     // a NaN in either type
+          else part[in * part_row + col] = NAN;
+        });
+      }
+      __syncwarp();
+      s_nan[warp] = false;
+      __syncwarp();
     }
     if (!more) break;
     pos = item_end;

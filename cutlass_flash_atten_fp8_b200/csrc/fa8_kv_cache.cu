@@ -24,6 +24,12 @@ constexpr int kWarpWork = 32 * kHold * kVec;
 constexpr int kMaxThreads = 512;
 constexpr int kWarpsPerCta = 4;        // units of a CTA where a warp takes one
 
+// Units past the last look at the sequences, a thread each: one that is out of range may have no unit that finds it.  (Asked by the
+// units themselves the prompts of append took 50 to 53 us for 47.)
+__device__ __forceinline__ void check_sequence(const KvArgs& a, int64_t b) {
+  if (kv_bad(a, b, true)) report_bad_index(a);
+}
+
 // The part of a page that a unit is about.
 struct Unit {
   int head;
@@ -46,7 +52,6 @@ __device__ __forceinline__ Unit find_unit(const KvArgs& a, int64_t u) {
   const KvSeq s = kv_seq(a, b);
   const int P = 1 << a.page_shift;
   if (s.bad || s.n > s.len) {
-    if (i == 0 && j == 0) report_bad_index(a);
     const int64_t lo = static_cast<int64_t>(j) * P;
     if (kRead && lo < s.n) {
       r.off = -1;
@@ -131,7 +136,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_ap
   let_successor_start();
   const int tid = kWarp ? threadIdx.x & 31 : threadIdx.x, n_threads = kWarp ? 32 : blockDim.x;
   const int64_t u = kWarp ? static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5) : blockIdx.x;
-  if (u >= units) return;
+  if (u >= units) return check_sequence(a, (u - units) * n_threads + tid);
   const Unit w = find_unit<false>(a, u);
   if (w.rows == 0) return;                                // the same for all threads of the unit, as below
   const int D = a.head_dim, per_row = D / kVec, n = w.rows * per_row;
@@ -205,7 +210,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_re
   let_successor_start();
   const int tid = kWarp ? threadIdx.x & 31 : threadIdx.x, n_threads = kWarp ? 32 : blockDim.x;
   const int64_t u = kWarp ? static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5) : blockIdx.x;
-  if (u >= units) return;
+  if (u >= units) return check_sequence(a, (u - units) * n_threads + tid);
   const Unit w = find_unit<true>(a, u);
   if (w.rows == 0) return;
   const int D = a.head_dim, per_row = D / kVec, n = w.rows * per_row;
@@ -214,7 +219,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_re
   const uint8_t* x = (w.of_v ? a.v : a.k) + ((page_head << a.page_shift) + max(w.off, 0)) * D;
   const float d = page < 0 ? 0.f : ld_global((w.of_v ? a.v_descale : a.k_descale) + page_head);
   const int64_t row = static_cast<int64_t>(a.heads) * D;
-  uint16_t* const y = (w.of_v ? v_out : k_out) + w.row0 * row + w.head * D;
+  uint16_t* const y = (w.of_v ? v_out : k_out) + w.row0 * row + static_cast<int64_t>(w.head) * D;
   for (int i0 = tid; i0 < n; i0 += kHold * n_threads) {
     uint2 c[kHold];
 #pragma unroll
@@ -260,7 +265,9 @@ bool plan_units(const KvArgs& a, cudaStream_t stream, cudaLaunchAttribute* attr,
   p->threads = p->warp ? 32 * kWarpsPerCta : (work / (kHold * kVec) + 31) / 32 * 32;
   if (p->threads > kMaxThreads) p->threads = kMaxThreads;
   p->magic = (1u << 20) / static_cast<uint32_t>(a.head_dim / kVec) + 1u;
-  const int64_t ctas = p->warp ? (p->units + kWarpsPerCta - 1) / kWarpsPerCta : p->units;
+  const int at_a_time = p->warp ? 32 : p->threads;
+  const int64_t all = p->units + (a.batch + at_a_time - 1) / at_a_time;
+  const int64_t ctas = p->warp ? (all + kWarpsPerCta - 1) / kWarpsPerCta : all;
   if (ctas > 0x7fffffff) return false;
   p->cfg = cudaLaunchConfig_t{};
   p->cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);

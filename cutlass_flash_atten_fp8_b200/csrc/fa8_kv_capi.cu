@@ -15,6 +15,9 @@ namespace {
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
+constexpr int64_t kMost = 0x7fffff00;     // positions of a sequence, rows
+constexpr int32_t kMostHeads = 65536;
+
 // Checks of a cache description, and the kernels' form of it.
 int check_cache(const fa8_kv_cache* c, fa8::KvArgs* a) {
   if (!c || !c->k || !c->v || !c->k_descale || !c->v_descale || !c->page_table || !c->seqlens) return FA8_ERR_BAD_ARG;
@@ -28,8 +31,8 @@ int check_cache(const fa8_kv_cache* c, fa8::KvArgs* a) {
   int shift = 4;
   while (shift < 7 && (1 << shift) != c->page_size) ++shift;
   if ((1 << shift) != c->page_size) return FA8_ERR_UNSUPPORTED;
-  // positions are 32-bit numbers
-  if (static_cast<int64_t>(c->table_width) * c->page_size > 0x7fffffff) return FA8_ERR_UNSUPPORTED;
+  // positions and rows are 32-bit numbers, also when rounded up to whole blocks
+  if (static_cast<int64_t>(c->table_width) * c->page_size > kMost || c->tokens > kMost || c->heads_kv > kMostHeads) return FA8_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(c->num_pages) * c->heads_kv > 0x7fffffff) return FA8_ERR_UNSUPPORTED;
   if (!c->cu_seqlens && c->tokens % c->batch != 0) return FA8_ERR_BAD_ARG;
   a->k = static_cast<uint8_t*>(c->k);
@@ -130,7 +133,7 @@ int fa8_kv_attention(const fa8_kv_attention_params* p, void* cuda_stream) {
   if (p->heads <= 0 || p->heads % p->cache.heads_kv != 0) return FA8_ERR_BAD_ARG;
   if (!(p->softmax_scale > 0.f) || !std::isfinite(p->softmax_scale)) return FA8_ERR_BAD_ARG;
   if (!aligned(p->lse, 4)) return FA8_ERR_BAD_ARG;
-  if (static_cast<int64_t>(a.c.tokens) * p->heads > 0x7fffffff) return FA8_ERR_UNSUPPORTED;      // rows are 32-bit numbers
+  if (static_cast<int64_t>(a.c.tokens) * p->heads > kMost) return FA8_ERR_UNSUPPORTED;
   if (a.c.tokens == 0) return FA8_OK;
   if (!rows_ok(p->q, p->q_token_stride, p->q_head_stride) || !rows_ok(p->o, 0, 0)) return FA8_ERR_BAD_ARG;
   a.q = {p->q, p->q_token_stride, p->q_head_stride};

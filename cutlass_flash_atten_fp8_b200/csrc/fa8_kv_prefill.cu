@@ -96,6 +96,7 @@ struct Shared {
   uint64_t drain, given;
   uint4 answer;                          // to the request for another CTA's item
   Item item[kItemSlots];                 // seq < 0: no more
+  int with_nan[kItemSlots];              // NaNs of V of keys that only some of the item's rows see were taken out (see drop_nans)
   uint32_t factor[C::kRaw][C::kGroups];  // fp16 pair to multiply a group of 16 keys by
   int valid[C::kRaw];                    // rows of the tile that are keys
   int complete[C::kRaw];                 // all are, and of pages that exist
@@ -340,6 +341,8 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     it = sh.item[slot];
     return true;
   };
+  // From the block of this key on NaNs of V are left to the end: the item's rows do not all see its keys.
+  auto apart = [&](const Item& i) { return a.causal ? max(0, min(i.len, i.len - i.n + i.token0 + 1)) / C::kN : 0x7fffffff; };
   auto item_read = [&] { mbar_arrive(smem_u32(&sh.item_empty[n_items++ % kItemSlots])); };
 
   __syncwarp();
@@ -358,6 +361,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       if (!ok) return;
       if (lane == 0) {
         sh.item[slot] = it;
+        sh.with_nan[slot] = 0;
         mbar_arrive(smem_u32(&sh.item_full[slot]));
       }
       ++n_items;
@@ -602,7 +606,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       if (lane == 0) item_read();
       else ++n_items;
       if (it.seq < 0) break;
-      const int n_tiles = 2 * (it.blk1 - it.blk0);
+      const int n_tiles = 2 * (it.blk1 - it.blk0), apart_blk = apart(it);
       for (int i = 0; i < n_tiles && ok; ++i, ++tiles) {
         const uint32_t st = tiles % C::kRaw, rg = tiles % C::kRing;
         ok = wait_bounded(wctx, &sh.raw_full[st], (tiles / C::kRaw) & 1, 0xb700 + st);
@@ -625,6 +629,18 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           st_shared16(to + (((2 * q) ^ r8) << 4), lo);
           st_shared16(to + (((2 * q + 1) ^ r8) << 4), hi);
         };
+        if ((i & 1) && it.blk0 + (i >> 1) >= apart_blk) {
+#pragma unroll 1
+          for (int p = w; p < kParts; p += 4) {
+            if (sh.factor[st][p / C::kCols / 2] == 0u || (p / C::kCols) * 8 + r8 >= valid) continue;
+            uint4 x = ld_shared16(from(p));
+            if (drop_nans<kE5M2>(x)) {
+              st_shared16(from(p), x);
+              sh.with_nan[(n_items - 1) % kItemSlots] = 1;
+            }
+          }
+          __syncwarp();
+        }
         if (sh.complete[st]) {
           // four loads go out before the first is used
 #pragma unroll
@@ -928,6 +944,23 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         }
       }
       pair_sync();                                               // both warps are through with these rows of Q's memory
+      const int slot = (n_items - 1) % kItemSlots;               // still this item's: no more than one other waits
+      if (*static_cast<volatile int*>(&sh.with_nan[slot]) != 0) {
+        const Item i = sh.item[slot];
+        const int token0 = i.token0 + tile * tile_tokens, rows = min(tile_tokens, i.n_tokens - tile * tile_tokens) * group;
+#pragma unroll 1
+        for (int q = 32 * sub; q < min(32 * sub + 32, rows); ++q) {
+          const int t = (q * over_group) >> 16;
+          const int64_t to = ((static_cast<int64_t>(i.first) + token0 + t) * a.heads_q + i.head * group + (q - t * group)) * a.c.head_dim;
+          float* const partial = plan.partial_o + static_cast<int64_t>(i.part) * a.c.tokens * a.heads_q * a.c.head_dim;
+          write_nans<kE5M2>(a.c, i.seq, i.head, max(apart(i), i.blk0) * C::kN, min(i.len - i.n + token0 + t + 1, i.blk1 * C::kN),
+                            part * kMyCols + lane, min(a.c.head_dim, (part + 1) * kMyCols), [&](int col) {
+            if (plan.parts == 1) static_cast<uint16_t*>(a.o)[to + col] = 0x7fff;       // a NaN in either type
+            else partial[to + col] = NAN;
+          });
+        }
+        __syncwarp();
+      }
     }
   }
   let_successor_start();

@@ -50,6 +50,14 @@ __device__ __forceinline__ KvSeq kv_seq(const KvArgs& a, int b) {
   return s;
 }
 
+// Sequence b is out of range (with_len: or has fewer tokens than it is to write or read).  Asked once for every sequence of a call: token
+// ranges that decrease can hide a sequence from the search below.
+__device__ __forceinline__ bool kv_bad(const KvArgs& a, int64_t b, bool with_len) {
+  if (b >= a.batch) return false;
+  const KvSeq s = kv_seq(a, static_cast<int>(b));
+  return s.bad || (with_len && s.n > s.len);
+}
+
 // Work is dealt out in slots of a host-known number, a slot being one block of T tokens of one sequence at most.  Even
 // batches have the same number for each.  Otherwise sequence b has the slots from cu[b] / T + extra * b on.  extra = 1 covers blocks counted
 // from a sequence's first new token (ceil(n / T) <= floor(cu[b+1] / T) - floor(cu[b] / T) + 1), extra = 2 blocks at fixed places of
@@ -130,6 +138,40 @@ __device__ __forceinline__ uint32_t fp8_pair(float lo, float hi) {
   if (kE5M2) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   else asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// A product adds 0 * V for keys that a row's mask leaves out, and a NaN there would stay one.  So where rows of a tile see different
+// keys, NaNs of V are taken out of the tile before the product, and the rows that do see them get theirs afterwards, in what was
+// stored for them (write_nans).
+template <bool kE5M2>
+__device__ __forceinline__ bool drop_nans(uint4& x) {
+  // sign bits of the bytes that hold a NaN
+  auto of = [](uint32_t w) { return ((w & 0x7f7f7f7fu) + (kE5M2 ? 0x03030303u : 0x01010101u)) & 0x80808080u; };
+  const uint32_t n[4] = {of(x.x), of(x.y), of(x.z), of(x.w)};
+  if ((n[0] | n[1] | n[2] | n[3]) == 0u) return false;
+  x.x &= ~((n[0] >> 7) * 0xffu);
+  x.y &= ~((n[1] >> 7) * 0xffu);
+  x.z &= ~((n[2] >> 7) * 0xffu);
+  x.w &= ~((n[3] >> 7) * 0xffu);
+  return true;
+}
+// Calls put(column) for the columns col, col + 32 ... below `end` in which a key from lo to hi - 1 of a sequence holds a NaN.  Goes through the
+// pool byte by byte, but only after a NaN has been met.
+template <bool kE5M2, typename Put>
+__device__ __forceinline__ void write_nans(const KvArgs& a, int seq, int head, int lo, int hi, int col, int end, Put put) {
+#pragma unroll 1
+  for (; col < end; col += 32) {
+#pragma unroll 1
+    for (int key = lo; key < hi; ++key) {
+      const int page = ld_int(a.table + static_cast<int64_t>(seq) * a.table_stride + (key >> a.page_shift));
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.num_pages)) continue;
+      const int64_t row = ((static_cast<int64_t>(page) * a.heads + head) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+      if ((a.v[row * a.head_dim + col] & 0x7f) >= (kE5M2 ? 0x7d : 0x7f)) {
+        put(col);
+        break;
+      }
+    }
+  }
 }
 
 }  // namespace fa8

@@ -90,6 +90,8 @@ def _check_tables(device, page_table, seqlens, cu_seqlens, tokens):
         raise RuntimeError("there are tokens but no sequences or no pages to hold them")
     if batch > 1 and page_table.stride(0) < page_table.shape[1]:
         raise RuntimeError("page_table's rows must not overlap")
+    if batch > 1 and page_table.stride(0) > 0x7fffffff:
+        raise RuntimeError(f"page_table's rows are {page_table.stride(0)} entries apart: more than 32 bits hold")
     if cu_seqlens is None and batch > 0 and tokens % batch != 0:
         raise RuntimeError(f"{tokens} tokens cannot be divided evenly over {batch} sequences: give cu_seqlens")
 

@@ -98,7 +98,11 @@ def attention(q, cache, page_table, seqlens, causal, scale, cu_seqlens=None):
         p = torch.exp(s - torch.where(m == -math.inf, 0.0, m))
         l = p.sum(-1, keepdim=True)
         p = p / torch.where(l == 0, 1.0, l)
-        o[first:first + n] = torch.einsum("hij,jhd->ihd", p, vq)
+        # what a row does not see does not count, whatever is held there
+        seen = (s > -math.inf) | torch.isnan(s)
+        nan = torch.einsum("hij,jhd->ihd", seen.double(), torch.isnan(vq).double()) > 0
+        vq = torch.where(torch.isnan(vq), 0.0, vq)
+        o[first:first + n] = torch.where(nan, math.nan, torch.einsum("hij,jhd->ihd", p, vq))
         a[first:first + n] = torch.einsum("hij,jhd->ihd", p, vq.abs())
         lse[first:first + n] = (m + torch.log(l)).squeeze(-1).t()
     return o, lse, a

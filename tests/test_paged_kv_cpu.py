@@ -27,7 +27,8 @@ BAD_CACHES = [dict(k=None), dict(v=None), dict(k_descale=None), dict(v_descale=N
               dict(v_descale=FAKE + 1), dict(page_table=FAKE + 2), dict(seqlens=FAKE + 1), dict(cu_seqlens=FAKE + 2),
               dict(status_word=FAKE + 3), dict(tokens=3)]
 UNSUPPORTED_CACHES = [dict(head_dim=0), dict(head_dim=48), dict(head_dim=288), dict(page_size=8), dict(page_size=24), dict(page_size=256),
-                      dict(page_size=0), dict(table_width=1 << 27, table_stride=1 << 27, page_size=16), dict(num_pages=1 << 30, heads_kv=2)]
+                      dict(page_size=0), dict(table_width=1 << 27, table_stride=1 << 27, page_size=16), dict(num_pages=1 << 30, heads_kv=2),
+                      dict(table_width=(1 << 24) - 1, table_stride=1 << 24, page_size=128), dict(num_pages=1, heads_kv=65537), dict(tokens=0x7ffffffe)]
 
 
 def calls(lib, c):
@@ -74,6 +75,23 @@ def test_bad_rows_are_refused():
         assert lib.fa8_kv_attention(ctypes.byref(_lib.Fa8KvAttentionParams(**{**good, **kw})), None) == bad, kw
     for args in ((0, 1, 1, 1, 64, 16, 1, 148), (1, -1, 1, 1, 64, 16, 1, 148), (1, 1, 3, 2, 64, 16, 1, 148), (1, 1, 1, 1, 64, 16, 1, 0)):
         assert lib.fa8_kv_attention_workspace(*args) == bad
+
+
+def test_rows_past_32_bits_are_unsupported():
+    c = cache_params(tokens=1 << 24, batch=2)
+    p = _lib.Fa8KvAttentionParams(cache=c, q=FAKE, q_token_stride=64 * 128, q_head_stride=64, o=FAKE, dtype=0, heads=128, is_causal=1, softmax_scale=0.125)
+    assert _lib.load().fa8_kv_attention(ctypes.byref(p), None) == _lib.FA8_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("batch,tokens", [(1, 1), (3, 3), (7, 100), (64, 64), (1000, 1000), (2, 5000)])
+@pytest.mark.parametrize("heads,heads_kv,head_dim", [(1, 1, 32), (32, 8, 128), (160, 1, 64), (9, 3, 256)])
+def test_workspace_is_a_matter_of_sizes(batch, tokens, heads, heads_kv, head_dim):
+    """Never negative, and bounded: a partial result for each of the GPU's warps, or sixteen of the output."""
+    lib = _lib.load()
+    for width in (1, 40, 5000):
+        n = lib.fa8_kv_attention_workspace(batch, tokens, heads, heads_kv, head_dim, 64, width, 148)
+        assert 0 <= n <= max(148 * 18 * 32 * (head_dim + 2) * 4 + 8192, 16 * tokens * heads * (head_dim + 2) * 4)
+        assert n == lib.fa8_kv_attention_workspace(batch, tokens, heads, heads_kv, head_dim, 64, width, 148)
 
 
 def test_no_tokens_is_no_launch():

@@ -243,6 +243,144 @@ def test_nan_and_infinity_in_held_keys_come_through():
     assert bool(nan[0, :, 5].all()) and int(nan.sum()) == 2       # column 5 of that sequence alone
 
 
+GROUPS = [(160, 1, 64), (48, 1, 128), (7, 1, 128), (128, 1, 32), (129, 1, 64), (100, 2, 256)]
+
+
+@pytest.mark.parametrize("H,Hk,D", GROUPS)
+@pytest.mark.parametrize("seqs", [[(1, 300), (1, 40)], [(3, 70), (2, 2), (5, 260)], [(70, 90), (1, 200), (33, 33)]], ids=["tokens", "drafts", "prompts"])
+def test_attention_with_groups_of_any_size(H, Hk, D, seqs):
+    """Query heads of a K/V head that fill no block of rows, or more than one."""
+    attend(seqs, H, Hk, D, 32, torch.bfloat16, E4M3, True, seed=21)
+
+
+RAGGED = {"forty": [(i % 4, i % 4 + 9 * i % 130) for i in range(40)], "a thousand": [(i % 3, i % 3 + 5 * i % 40) for i in range(1100)],
+          "forty prompts": [(33 + 11 * i % 60, 33 + 11 * i % 60 + 7 * (i % 5)) for i in range(40)],
+          "one prompt among tokens": [(1, 1 + i % 50) if i != 20 else (900, 900) for i in range(45)]}
+
+
+@pytest.mark.parametrize("name", RAGGED)
+@pytest.mark.parametrize("D,P", [(64, 16), (128, 64)])
+def test_attention_of_many_sequences(name, D, P):
+    attend(RAGGED[name], 4, 2, D, P, torch.float16, E4M3, True, seed=22, lead=2, tail=1)
+
+
+@pytest.mark.parametrize("name", ["forty", "a thousand", "forty prompts"])
+def test_append_and_read_of_many_sequences(name):
+    seqs, heads, D, P, half = RAGGED[name], 2, 64, 16, torch.bfloat16
+    cu, T, lens = ranges(seqs, 2, 3)
+    cache, table = filled(heads, D, P, E4M3, seqs, seed=23)
+    k, v = (rows(T, heads, D, half, s, False, cu, seqs) for s in (24, 25))
+    dev, where = PagedKVCache(*to(DEV, *cache)), to(DEV, table, lens)
+    paged_kv_append(dev, k, v, *where, cu_seqlens=cu.to(DEV))
+    got = paged_kv_read(dev, *where, T, cu_seqlens=cu.to(DEV), dtype=half)
+    check_status(DEV)
+    after = po.append(cache, k.cpu(), v.cpu(), table, lens, cu)
+    for x, y in zip(dev, after):
+        assert torch.equal(x.cpu().float().nan_to_num(-1.0), y.float().nan_to_num(-1.0))
+    for x, y in zip(got, po.read(after, table, lens, T, cu)):
+        assert torch.equal(x[int(cu[0]):int(cu[-1])].cpu().double(), y[int(cu[0]):int(cu[-1])].to(half).double())
+
+
+@pytest.mark.parametrize("seqs,H,Hk,D,P", [([(130, 3000)], 1, 1, 64, 64), ([(130, 3000)], 4, 2, 128, 16), ([(257, 2600)], 2, 1, 256, 128),
+                                            ([(70, 70), (150, 2900)], 2, 1, 128, 32), ([(600, 600)] * 5, 16, 16, 64, 64), ([(300, 333), (0, 3), (700, 700)], 16, 8, 128, 16)],
+                         ids=["parts 64", "parts 128", "parts 256", "parts of which some are empty", "more items than SMs", "ragged"])
+@pytest.mark.parametrize("half,fp8,causal", [(torch.float16, E4M3, True), (torch.bfloat16, E5M2, False)])
+def test_attention_of_prompts_in_parts_and_in_many_items(seqs, H, Hk, D, P, half, fp8, causal):
+    """Few items, whose keys are cut into parts and joined; many, which CTAs take over from one another."""
+    attend(seqs, H, Hk, D, P, half, fp8, causal, seed=26)
+
+
+@pytest.mark.parametrize("n_seqs,Hk,length", [(1, 1, 6000), (1, 2, 1500), (12, 2, 900), (20, 2, 700), (2, 4, 100), (30, 4, 1000)])
+@pytest.mark.parametrize("H,D", [(1, 64), (4, 128), (9, 256), (8, 32)])
+def test_attention_of_single_tokens_by_clusters(n_seqs, Hk, length, H, D):
+    """Items few and short enough for a cluster of one to eight CTAs each (and some for which they are not)."""
+    attend([(1, max(0, length - 37 * b)) for b in range(n_seqs)], H * Hk, Hk, D, 64, torch.float16, E4M3, True, seed=27)
+
+
+@pytest.mark.parametrize("seqs", [[(1, 300), (1, 40)], [(4, 300), (4, 40)], [(150, 300), (150, 150)]], ids=["tokens", "drafts", "prompts"])
+@pytest.mark.parametrize("D,fp8", [(64, E4M3), (128, E5M2), (256, E4M3)])
+def test_scales_of_zero(seqs, D, fp8):
+    """A page of scale zero holds zeros: keys that count, with scores of 0, and values that add nothing."""
+    H, Hk, P, half = 4, 2, 16, torch.float16
+    cu, T, lens = ranges(seqs)
+    cache, table = filled(Hk, D, P, fp8, seqs, seed=28)
+    cache[2][table[0, 0]] = 0.0
+    cache[2][table[0, 2]] = 0.0
+    cache[3][table[0, 1]] = 0.0
+    cache[3][table[1, 0]] = 0.0
+    cache[2][table[1, 1]] = cache[3][table[1, 1]] = 0.0
+    q = rows(T, H, D, half, 29, False, cu, seqs)
+    out, lse = flash_attention_paged_kv(q, to(DEV, *cache), *to(DEV, table, lens), True, 0.2, return_lse=True)
+    check_status(DEV)
+    check_attention(q, cache, table, lens, True, 0.2, cu, out, lse)
+
+
+@pytest.mark.parametrize("seqs", [[(3, 40), (4, 300)], [(40, 200), (5, 5)], [(150, 500), (300, 300), (129, 140)], [(260, 3000)]], ids=["drafts", "pieces", "prompts", "parts"])
+@pytest.mark.parametrize("H,Hk,D,P", [(2, 2, 64, 16), (8, 2, 128, 32), (3, 1, 256, 64), (2, 1, 32, 128), (4, 4, 96, 16)])
+@pytest.mark.parametrize("fp8", [E4M3, E5M2])
+def test_nan_in_keys_that_only_some_rows_see(seqs, H, Hk, D, P, fp8):
+    """NaNs among the new tokens' keys and values reach the rows that see them, in the columns that hold them, and no others."""
+    half = torch.bfloat16
+    cu, T, lens = ranges(seqs)
+    cache, table = filled(Hk, D, P, fp8, seqs, seed=30)
+    for b, (n, s) in enumerate(seqs):
+        for i, col in ((n - 1, 3), (n // 2, D - 1), (n // 2, 17), (max(0, n - 130), 0)):
+            key = s - n + i
+            cache[1][int(table[b, key // P]), 0, key % P, col] = math.nan
+        key = s - n + n // 3
+        cache[0][int(table[b, key // P]), Hk - 1, key % P, 7] = math.nan
+    q = rows(T, H, D, half, 31, False, cu, seqs)
+    where = to(DEV, table, lens, cu)
+    out, lse = flash_attention_paged_kv(q, to(DEV, *cache), where[0], where[1], True, 0.1, cu_seqlens=where[2], return_lse=True)
+    check_status(DEV)
+    want, want_lse, A = po.attention(q.cpu(), cache, table, lens, True, 0.1, cu)
+    got = out.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isnan(lse.cpu()), torch.isnan(want_lse))
+    limit = torch.finfo(half).eps / 2 * want.abs() + 1.25 * 2.0 ** -11 * A + 2.0 ** -25
+    held = ~torch.isnan(want)
+    assert bool(((got - want).abs() <= limit)[held].all())
+
+
+def test_page_table_of_wider_rows():
+    """A view of a table that has more columns: as many as the longest sequence of this call needs."""
+    seqs, H, Hk, D, P = [(1, 50), (1, 90), (1, 33)], 4, 2, 64, 16
+    cu, T, lens = ranges(seqs)
+    cache, table = filled(Hk, D, P, E4M3, seqs, seed=32)
+    wide = torch.full((3, 40), -1, dtype=torch.int32)
+    wide[:, 3:3 + table.shape[1]] = table
+    q = rows(T, H, D, torch.float16, 33, False, cu, seqs)
+    dev = to(DEV, *cache)
+    a = flash_attention_paged_kv(q, dev, wide.to(DEV)[:, 3:9], lens.to(DEV), True, 0.1)[0]
+    b = flash_attention_paged_kv(q, dev, table.to(DEV)[:, :6].contiguous(), lens.to(DEV), True, 0.1)[0]
+    check_status(DEV)
+    assert torch.equal(bits(a), bits(b))
+
+
+@pytest.mark.parametrize("op", ["append", "read", "attend"])
+@pytest.mark.parametrize("cu", [[0, 1000, 0, 8], [0, 2000, 1, 2], [5, 3, 2, 1], [0, 0, -9, 4]], ids=str)
+@pytest.mark.parametrize("rows_of", [8, 1000])
+def test_token_ranges_that_decrease_are_always_reported(op, cu, rows_of):
+    """Also where no token is found to be of the sequence that has such a range."""
+    T, Hk, D, P = rows_of, 2, 64, 16
+    cache = PagedKVCache.empty(80, Hk, D, P, device=DEV)
+    for t in cache:
+        t.zero_()
+    table = torch.arange(72, dtype=torch.int32, device=DEV).view(3, 24)
+    lens = torch.full((3,), 300, dtype=torch.int32, device=DEV)
+    where = dict(cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=DEV))
+    x = torch.ones(T, Hk, D, dtype=torch.float16, device=DEV)
+    if op == "append":
+        paged_kv_append(cache, x, x, table, lens, **where)
+    elif op == "read":
+        paged_kv_read(cache, table, lens, T, **where)
+    else:
+        flash_attention_paged_kv(x, cache, table, lens, True, 0.1, **where)
+    with pytest.raises(RuntimeError, match="out of range"):
+        check_status(DEV)
+    check_status(DEV)
+
+
 # ---- a run of them, graphs, streams ---------------------------------------------------------------------------
 
 def test_generation_step_by_step_and_read_back():
