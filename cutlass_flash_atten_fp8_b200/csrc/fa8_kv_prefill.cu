@@ -3,21 +3,27 @@
 // The formulas and the treatment of scales are those of fa8_kv_attend.cu; here a K/V head's query rows come in tiles of 128, and both
 // products run on the tensor cores in fp16 with fp32 accumulators in tensor memory (tcgen05.mma kind::f16): fp8 products would
 // need P, and Q, rounded to three bits.  What bounds it: per 128 keys and tile 1024 cycles of products and 1024 of
-// exponentials (16 per cycle and SM) at head dim 128.
+// exponentials (16 per cycle and SM) at head dim 128, and shared memory: widening a tile of K or V moves as many bytes as a product reads.
 //
 // A CTA per SM, warps with roles, work items of two tiles (one at head dims above 128) of one sequence and K/V head:
 //   producer   looks up items and pages, copies K and V tiles of kN keys from the pages (fp8) into shared memory
 //   widening   four warps turn a tile into fp16, in the layout that the products want, times the power of two by which its pages' scales
-//              differ from the item's first page; keys past the last one become zeros (a NaN there must not meet a zero P)
+//              differ from the item's first page; keys past the last one become zeros (a NaN there must not meet a zero P).  Eight warps
+//              were no faster (330 us for 1024 tokens over 16384 keys, four 322)
 //   issuer     one thread: S = Q K^T into tensor memory, O += P V with P from tensor memory
-//   softmax    four warps a tile, a row to a thread: P = 2^(c s - m) over S as it lies, in halves of 64 keys that are handed over
-//              one by one; O to global memory at the end.
+//   softmax    eight warps a tile, two to 32 rows (four, a row to a thread, took 26 % longer): each has half of a block's keys, P = 2^(c s - m) over
+//              S as it lies, and at the end half of O's columns
 // Two tiles keep the tensor cores and the exponentials busy in turns; at head dims above 128 O takes half of tensor memory
 // and the one tile has two score buffers instead.
 //
 // The row reference m lies 6 below the maximum over the item's first kN keys, so that P, at 2^6, has its full precision twenty
-// binades down, and is raised when a half's sum of P nears fp16's largest number, which is also when O is rescaled.  Scales that differ by more than fp16 can take in, or are no powers of two, go
-// through a slower form of the softmax that multiplies them in (`residual`).
+// binades down, and is raised, and O rescaled, when the sum of P over half a block nears fp16's largest number.  Scales that differ by
+// more than fp16 can take in, or are no powers of two, go through a slower form of the softmax that multiplies them in (`residual`).
+//
+// Measured: 1024 tokens, 32 heads over 8, over 16384 keys, head dim 128: 322 us, 826 TFLOP/s, half of what a plain fp16 product
+// reaches on this GPU; four prompts of 4096: 466 us.  A block of 128 keys takes some 4000 cycles for two tiles where the tensor cores are busy for
+// 2048: a tile's chain S, softmax (1024 cycles of exponentials alone, 2350 beside the other tile's), P V is longer than the other tile's
+// work.  A quarter of the exponentials by a polynomial instead gained 2 % and was left out.
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -44,9 +50,9 @@ struct PCfg {
   static constexpr int kTiles = W == 256 ? 1 : 2;
   static constexpr int kN = W == 256 ? 64 : 128;               // keys of a block
   // Score buffers, which the blocks of both tiles take in turn: what tensor memory holds beside O.  The scores of a block go out kBufs
-  // blocks ahead, so a tile whose turn it is finds its next scores ready when there are more buffers than tiles.  (Four of 64 keys
-  // would do that at head dim 128, but a product of N = 64 is bound by reading Q: 80 cycles a step of 16 against 64 for N = 128,
-  // and 1024 tokens over 16384 keys took R64N us against R128N.)
+  // blocks ahead, so a tile whose turn it is finds its next scores ready when there are more buffers than tiles: 8 prompts of 2048 at
+  // head dim 64 took 340 us with two, 311 with three.  (Four of 64 keys would do that at head dim 128, but a product of N = 64 is
+  // bound by reading Q from shared memory: 80 cycles a step of 16 against 64 for N = 128.)
   static constexpr int kBufs = W == 64 ? 3 : 2;
   static constexpr int kGroups = kN / 16;                      // of keys that share a page
   static constexpr int kCols = W / 64;                         // column blocks of 64 fp16 (128 bytes)
@@ -64,7 +70,8 @@ struct PCfg {
   static constexpr int kWideWarp0 = kSoftWarps;
   static constexpr int kLoadWarp = kWideWarp0 + 4;
   static constexpr int kMmaWarp = kLoadWarp + 1;
-  // Whole warpgroups (two warps stand by), so that registers can be dealt out anew: 512 * 96 + 128 * 48 + 128 * 48 = 768 * 80.
+  // Whole warpgroups (two warps stand by), so that registers can be dealt out anew: 512 * 96 + 128 * 48 + 128 * 48 = 768 * 80.  (A thread of
+  // the softmax holds 32 scores and 32 pairs of P beside its row: with 88 registers 328 us for 1024 tokens over 16384 keys, 320 with 96.)
   static constexpr bool kDeal = kTiles == 2;
   static constexpr int kThreads = 32 * (kLoadWarp + 4);
   static constexpr uint32_t kSoftRegs = 96, kWideRegs = 48, kOtherRegs = 48;
@@ -347,253 +354,253 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
 
   __syncwarp();
   if (warp >= C::kLoadWarp) {
-  if constexpr (C::kDeal) setmaxnreg_dec<C::kOtherRegs>();
-  if (warp == C::kLoadWarp) {
-    // ---------------------------------------------------------------- producer
-    uint32_t tiles = 0, blocks = 0;                              // raw tiles and blocks filled so far
-    // once a wait has run out, the CTAs that are still to come have nothing to do
-    const int before = a.c.status ? *static_cast<volatile int*>(a.c.status) : 0;
-    bool ok = true, more = before == 0 || before == kBadIndex, asked = false;
-    auto push = [&](const Item& it) {
-      const int slot = n_items % kItemSlots;
-      ok = wait_bounded(wctx, &sh.item_empty[slot], ((n_items / kItemSlots) & 1) ^ 1, 0xb200);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return;
-      if (lane == 0) {
-        sh.item[slot] = it;
-        sh.with_nan[slot] = 0;
-        mbar_arrive(smem_u32(&sh.item_full[slot]));
-      }
-      ++n_items;
-    };
-    auto load_item = [&](int64_t id) {
-      Item it;
-      const int64_t sh_id = id / plan.parts;
-      it.part = static_cast<int>(id - sh_id * plan.parts);
-      const int64_t slot = sh_id / a.c.heads;
-      it.head = static_cast<int>(sh_id - slot * a.c.heads);
-      int j;
-      kv_find_slot(a.c, slot, plan.block_tokens, 1, &it.seq, &j);
-      const KvSeq s = kv_seq(a.c, it.seq);
-      const int tiles_of = (s.n + plan.block_tokens - 1) / plan.block_tokens;
-      if (j >= tiles_of) return;
-      it.first = s.first;
-      it.n = s.n;
-      it.len = s.len;
-      it.token0 = (tiles_of - 1 - j) * plan.block_tokens;
-      it.n_tokens = min(plan.block_tokens, s.n - it.token0);
-      it.vis = a.causal ? max(0, min(s.len, s.len - s.n + it.token0 + it.n_tokens)) : s.len;
-      const int n_blk = max(1, (it.vis + C::kN - 1) / C::kN);
-      it.blk0 = static_cast<int>(static_cast<int64_t>(n_blk) * it.part / plan.parts);
-      it.blk1 = static_cast<int>(static_cast<int64_t>(n_blk) * (it.part + 1) / plan.parts);
-      if (it.blk0 == it.blk1) return;
-      push(it);
-      if (!ok) return;
-
-      // Lane g < kGroups looks after the g-th sixteen keys of a block: page numbers are loaded two blocks ahead, scales one.
-      const int* const table = a.c.table + static_cast<int64_t>(it.seq) * a.c.table_stride;
-      auto load_page = [&](int blk) {
-        const int64_t key = static_cast<int64_t>(blk) * C::kN + 16 * lane;
-        return lane < C::kGroups && blk < it.blk1 && key < it.vis ? ld_int(table + (key >> a.c.page_shift)) : -2;
-      };
-      auto in_pool = [&](int page) { return static_cast<unsigned>(page) < static_cast<unsigned>(a.c.num_pages); };
-      auto load_scale = [&](const float* d, int page) { return in_pool(page) ? ld_global(d + static_cast<int64_t>(page) * a.c.heads + it.head) : 1.f; };
-      int page = load_page(it.blk0), page1 = load_page(it.blk0 + 1);
-      float kd = load_scale(a.c.k_descale, page), vd = load_scale(a.c.v_descale, page);
-      // the item's reference scales: its first page's, so that e5m2 (up to 2^15.8) keeps away from fp16's ends
-      const float margin = kE5M2 ? 16.f : 1.f;
-      auto reference = [&](float d) {
-        d = __shfl_sync(0xffffffffu, d, 0);
-        return (d >= 0x1p-100f && d <= 0x1p100f ? d : 1.f) * margin;
-      };
-      const float kref = reference(kd), vref = reference(vd);
-      for (int blk = it.blk0; blk < it.blk1 && ok; ++blk) {
-        const int page2 = load_page(blk + 2);
-        const float kd1 = load_scale(a.c.k_descale, page1), vd1 = load_scale(a.c.v_descale, page1);
-        const bool here = in_pool(page);
-        if (!here && page != -2) report_bad_index(a.c);
-        // factor 2^e that fp16 takes in exactly: e4m3 2^-15 ... 2^7, e5m2 2^-8 ... 1; the rest is residual
-        auto split = [&](float d, float ref, float* rest) {
-          const float f = d / ref;
-          const uint32_t bits = __float_as_uint(f);
-          const int e = static_cast<int>(bits >> 23) - 127;
-          const bool exact = (bits & 0x7fffffu) == 0 && e >= (kE5M2 ? -8 : -15) && e <= (kE5M2 ? 0 : 7);
-          const float take = exact ? f : (kE5M2 ? 0x1p-4f : 1.f);
-          *rest = exact ? 1.f : d / ref / take;
-          const uint32_t h = pack_half2(take, take);
-          return h;
-        };
-        const uint32_t n = blocks % kBlockSlots;
-        float rk = 1.f, rv = 1.f;
-        const uint32_t fk = split(kd, kref, &rk), fv = split(vd, vref, &rv);
-        if (!here) {
-          rv = 1.f;
-          rk = page == -2 ? 1.f : -1.f;                          // past the last key: masked by the row's limit
-        }
-        if (lane < C::kGroups) {
-          sh.residual[n][0][lane] = rk;
-          sh.residual[n][1][lane] = rv;
-        }
-        const bool flagged = __any_sync(0xffffffffu, lane < C::kGroups && (rk != 1.f || rv != 1.f));
+    if constexpr (C::kDeal) setmaxnreg_dec<C::kOtherRegs>();
+    if (warp == C::kLoadWarp) {
+      // ---------------------------------------------------------------- producer
+      uint32_t tiles = 0, blocks = 0;                              // raw tiles and blocks filled so far
+      // once a wait has run out, the CTAs that are still to come have nothing to do
+      const int before = a.c.status ? *static_cast<volatile int*>(a.c.status) : 0;
+      bool ok = true, more = before == 0 || before == kBadIndex, asked = false;
+      auto push = [&](const Item& it) {
+        const int slot = n_items % kItemSlots;
+        ok = wait_bounded(wctx, &sh.item_empty[slot], ((n_items / kItemSlots) & 1) ^ 1, 0xb200);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
         if (lane == 0) {
-          sh.ref[n][0] = kref;
-          sh.ref[n][1] = vref;
-          sh.flagged[n] = flagged;
+          sh.item[slot] = it;
+          sh.with_nan[slot] = 0;
+          mbar_arrive(smem_u32(&sh.item_full[slot]));
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.blk_full[n]));
-        ++blocks;
-        // one copy per page part of the block (box_keys keys) and 128 columns
-        const int box_keys = min(1 << a.c.page_shift, kv_prefill_copy_keys(W));
-        const bool issues = here && (16 * lane) % box_keys == 0;
-        const int boxes = __popc(__ballot_sync(0xffffffffu, issues));
-        const bool all_here = __all_sync(0xffffffffu, here || lane >= C::kGroups);
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const int st = tiles % C::kRaw;
-          ok = __all_sync(0xffffffffu, wait_bounded(wctx, &sh.raw_empty[st], ((tiles / C::kRaw) & 1) ^ 1, 0xb300 + st));
-          if (!ok) break;
-          if (lane < C::kGroups) sh.factor[st][lane] = here ? (kv ? fv : fk) : 0u;
+        ++n_items;
+      };
+      auto load_item = [&](int64_t id) {
+        Item it;
+        const int64_t sh_id = id / plan.parts;
+        it.part = static_cast<int>(id - sh_id * plan.parts);
+        const int64_t slot = sh_id / a.c.heads;
+        it.head = static_cast<int>(sh_id - slot * a.c.heads);
+        int j;
+        kv_find_slot(a.c, slot, plan.block_tokens, 1, &it.seq, &j);
+        const KvSeq s = kv_seq(a.c, it.seq);
+        const int tiles_of = (s.n + plan.block_tokens - 1) / plan.block_tokens;
+        if (j >= tiles_of) return;
+        it.first = s.first;
+        it.n = s.n;
+        it.len = s.len;
+        it.token0 = (tiles_of - 1 - j) * plan.block_tokens;
+        it.n_tokens = min(plan.block_tokens, s.n - it.token0);
+        it.vis = a.causal ? max(0, min(s.len, s.len - s.n + it.token0 + it.n_tokens)) : s.len;
+        const int n_blk = max(1, (it.vis + C::kN - 1) / C::kN);
+        it.blk0 = static_cast<int>(static_cast<int64_t>(n_blk) * it.part / plan.parts);
+        it.blk1 = static_cast<int>(static_cast<int64_t>(n_blk) * (it.part + 1) / plan.parts);
+        if (it.blk0 == it.blk1) return;
+        push(it);
+        if (!ok) return;
+
+        // Lane g < kGroups looks after the g-th sixteen keys of a block: page numbers are loaded two blocks ahead, scales one.
+        const int* const table = a.c.table + static_cast<int64_t>(it.seq) * a.c.table_stride;
+        auto load_page = [&](int blk) {
+          const int64_t key = static_cast<int64_t>(blk) * C::kN + 16 * lane;
+          return lane < C::kGroups && blk < it.blk1 && key < it.vis ? ld_int(table + (key >> a.c.page_shift)) : -2;
+        };
+        auto in_pool = [&](int page) { return static_cast<unsigned>(page) < static_cast<unsigned>(a.c.num_pages); };
+        auto load_scale = [&](const float* d, int page) { return in_pool(page) ? ld_global(d + static_cast<int64_t>(page) * a.c.heads + it.head) : 1.f; };
+        int page = load_page(it.blk0), page1 = load_page(it.blk0 + 1);
+        float kd = load_scale(a.c.k_descale, page), vd = load_scale(a.c.v_descale, page);
+        // the item's reference scales: its first page's, so that e5m2 (up to 2^15.8) keeps away from fp16's ends
+        const float margin = kE5M2 ? 16.f : 1.f;
+        auto reference = [&](float d) {
+          d = __shfl_sync(0xffffffffu, d, 0);
+          return (d >= 0x1p-100f && d <= 0x1p100f ? d : 1.f) * margin;
+        };
+        const float kref = reference(kd), vref = reference(vd);
+        for (int blk = it.blk0; blk < it.blk1 && ok; ++blk) {
+          const int page2 = load_page(blk + 2);
+          const float kd1 = load_scale(a.c.k_descale, page1), vd1 = load_scale(a.c.v_descale, page1);
+          const bool here = in_pool(page);
+          if (!here && page != -2) report_bad_index(a.c);
+          // factor 2^e that fp16 takes in exactly: e4m3 2^-15 ... 2^7, e5m2 2^-8 ... 1; the rest is residual
+          auto split = [&](float d, float ref, float* rest) {
+            const float f = d / ref;
+            const uint32_t bits = __float_as_uint(f);
+            const int e = static_cast<int>(bits >> 23) - 127;
+            const bool exact = (bits & 0x7fffffu) == 0 && e >= (kE5M2 ? -8 : -15) && e <= (kE5M2 ? 0 : 7);
+            const float take = exact ? f : (kE5M2 ? 0x1p-4f : 1.f);
+            *rest = exact ? 1.f : d / ref / take;
+            const uint32_t h = pack_half2(take, take);
+            return h;
+          };
+          const uint32_t n = blocks % kBlockSlots;
+          float rk = 1.f, rv = 1.f;
+          const uint32_t fk = split(kd, kref, &rk), fv = split(vd, vref, &rv);
+          if (!here) {
+            rv = 1.f;
+            rk = page == -2 ? 1.f : -1.f;                          // past the last key: masked by the row's limit
+          }
+          if (lane < C::kGroups) {
+            sh.residual[n][0][lane] = rk;
+            sh.residual[n][1][lane] = rv;
+          }
+          const bool flagged = __any_sync(0xffffffffu, lane < C::kGroups && (rk != 1.f || rv != 1.f));
           if (lane == 0) {
-            sh.valid[st] = max(0, min(C::kN, it.vis - blk * C::kN));
-            sh.complete[st] = all_here && it.vis >= (blk + 1) * C::kN;
+            sh.ref[n][0] = kref;
+            sh.ref[n][1] = vref;
+            sh.flagged[n] = flagged;
           }
           __syncwarp();
-          const uint32_t bar = smem_u32(&sh.raw_full[st]);
-          if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_keys * C::kRawRow * C::kRawBlocks);
-          __syncwarp();
-          if (issues) {
-            const int row = ((blk * C::kN + 16 * lane) & ((1 << a.c.page_shift) - 1)) >> (flip ? 1 : 0);
+          if (lane == 0) mbar_arrive(smem_u32(&sh.blk_full[n]));
+          ++blocks;
+          // one copy per page part of the block (box_keys keys) and 128 columns
+          const int box_keys = min(1 << a.c.page_shift, kv_prefill_copy_keys(W));
+          const bool issues = here && (16 * lane) % box_keys == 0;
+          const int boxes = __popc(__ballot_sync(0xffffffffu, issues));
+          const bool all_here = __all_sync(0xffffffffu, here || lane >= C::kGroups);
 #pragma unroll
-            for (int b = 0; b < C::kRawBlocks; ++b)
-              tma_load_3d(s_raw + st * C::kRawBytes + b * C::kRawBlockBytes + 16 * lane * C::kRawRow, kv ? &tv : &tk, bar, 128 * b, row,
-                          page * a.c.heads + it.head);
+          for (int kv = 0; kv < 2; ++kv) {
+            const int st = tiles % C::kRaw;
+            ok = __all_sync(0xffffffffu, wait_bounded(wctx, &sh.raw_empty[st], ((tiles / C::kRaw) & 1) ^ 1, 0xb300 + st));
+            if (!ok) break;
+            if (lane < C::kGroups) sh.factor[st][lane] = here ? (kv ? fv : fk) : 0u;
+            if (lane == 0) {
+              sh.valid[st] = max(0, min(C::kN, it.vis - blk * C::kN));
+              sh.complete[st] = all_here && it.vis >= (blk + 1) * C::kN;
+            }
+            __syncwarp();
+            const uint32_t bar = smem_u32(&sh.raw_full[st]);
+            if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_keys * C::kRawRow * C::kRawBlocks);
+            __syncwarp();
+            if (issues) {
+              const int row = ((blk * C::kN + 16 * lane) & ((1 << a.c.page_shift) - 1)) >> (flip ? 1 : 0);
+#pragma unroll
+              for (int b = 0; b < C::kRawBlocks; ++b)
+                tma_load_3d(s_raw + st * C::kRawBytes + b * C::kRawBlockBytes + 16 * lane * C::kRawRow, kv ? &tv : &tk, bar, 128 * b, row,
+                            page * a.c.heads + it.head);
+            }
+            ++tiles;
           }
-          ++tiles;
+          page = page1;
+          page1 = page2;
+          kd = kd1;
+          vd = vd1;
         }
-        page = page1;
-        page1 = page2;
-        kd = kd1;
-        vd = vd1;
+      };
+      uint32_t answers = 0;
+      // A CTA to an item is launched; those on the GPU take over the others, one after another, as they get through their own, so that
+      // all end together whatever the items' lengths (dealt out in turns, 148 CTAs differed by a fifth at 2048 and 4096 new tokens).
+      for (int64_t id = blockIdx.x; ok && more;) {
+        if (id == 0)                                               // a bad range has no rows that would find it
+          for (int b = lane; b < a.c.batch; b += 32)
+            if (kv_seq(a.c, b).bad) report_bad_index(a.c);
+        load_item(id);
+        // One item waits while one is worked on, no more: others may be through before.
+        if (ok && n_items > 0) ok = wait_bounded(wctx, &sh.item_empty[(n_items - 1) % kItemSlots], ((n_items - 1) / kItemSlots) & 1, 0xb200);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) {
+          fence_proxy_async_smem();                                // the last answer has been read
+          mbar_arrive_expect_tx(smem_u32(&sh.given), 16);
+          ask_for_cta(smem_u32(&sh.answer), smem_u32(&sh.given));
+        }
+        asked = true;
+        ok = __all_sync(0xffffffffu, wait_bounded(wctx, &sh.given, answers & 1, 0xb210));
+        if (!ok) break;
+        asked = false;
+        ++answers;
+        id = taken_cta(smem_u32(&sh.answer));
+        more = id >= 0;
+        __syncwarp();
       }
-    };
-    uint32_t answers = 0;
-    // A CTA to an item is launched; those on the GPU take over the others, one after another, as they get through their own, so that
-    // all end together whatever the items' lengths (dealt out in turns, 148 CTAs differed by a fifth at 2048 and 4096 new tokens).
-    for (int64_t id = blockIdx.x; ok && more;) {
-      if (id == 0)                                               // a bad range has no rows that would find it
-        for (int b = lane; b < a.c.batch; b += 32)
-          if (kv_seq(a.c, b).bad) report_bad_index(a.c);
-      load_item(id);
-      // One item waits while one is worked on, no more: others may be through before.
-      if (ok && n_items > 0) ok = wait_bounded(wctx, &sh.item_empty[(n_items - 1) % kItemSlots], ((n_items - 1) / kItemSlots) & 1, 0xb200);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (lane == 0) {
-        fence_proxy_async_smem();                                // the last answer has been read
-        mbar_arrive_expect_tx(smem_u32(&sh.given), 16);
-        ask_for_cta(smem_u32(&sh.answer), smem_u32(&sh.given));
+      if (ok) {
+        Item none{};
+        none.seq = -1;
+        push(none);
       }
-      asked = true;
-      ok = __all_sync(0xffffffffu, wait_bounded(wctx, &sh.given, answers & 1, 0xb210));
-      if (!ok) break;
-      asked = false;
-      ++answers;
-      id = taken_cta(smem_u32(&sh.answer));
-      more = id >= 0;
+      if (!ok) {
+        // copies in flight, and an answer, land before the CTA's memory is given back (a wait each, with a limit)
+        if (asked) {
+          const uint64_t t0 = global_timer_ns();
+          while (!mbar_try_wait(smem_u32(&sh.given), answers & 1) && global_timer_ns() - t0 < 20000000ull) {}
+        }
+        for (uint32_t i = tiles > C::kRaw ? tiles - C::kRaw : 0; i < tiles; ++i) {
+          const uint64_t t0 = global_timer_ns();
+          while (!mbar_try_wait(smem_u32(&sh.raw_full[i % C::kRaw]), (i / C::kRaw) & 1) && global_timer_ns() - t0 < 20000000ull) {}
+        }
+      }
+    } else if (warp == C::kMmaWarp) {
+      // ---------------------------------------------------------------- issuer
+      if (elect_one()) {
+        constexpr uint32_t kIdescQK = idesc(C::kN, false), kIdescPV = idesc(W, true);
+        constexpr uint32_t kColQ = kTileM * 128 / 16, kColK = C::kN * 128 / 16;     // column blocks of Q and K in 16 bytes
+        const uint32_t q_lo = desc_lo(s_q, 16), k_lo = desc_lo(s_ring, 16), v_lo = desc_lo(s_ring, C::kN * 128);
+        bool ok = true;
+        uint32_t ld = 0;                                           // widened tiles used so far: K, V, K, V ...
+        uint32_t qn[2] = {0, 0};                                   // q_full phases by tile
+        uint32_t turns = 0;                                        // of the score buffers, before this item
+        auto ring_wait = [&](uint32_t i) { return wait_bounded(wctx, &sh.ring_full[i % C::kRing], (i / C::kRing) & 1, 0xb400); };
+        auto ring_release = [&](uint32_t i) { tc_commit(smem_u32(&sh.ring_empty[i % C::kRing])); };
+        auto issue_qk = [&](int tile, uint32_t b, uint32_t i) {
+          const uint32_t kk = k_lo + (i % C::kRing) * (C::kRingBytes / 16), qq = q_lo + tile * (C::kQBytes / 16);
+#pragma unroll
+          for (int k = 0; k < W / 16; ++k)
+            mma_f16_ss(tmem + C::kN * b, desc(qq + (k >> 2) * kColQ + 2 * (k & 3)), desc(kk + (k >> 2) * kColK + 2 * (k & 3)), kIdescQK, k > 0);
+          tc_commit(smem_u32(&sh.s_full[b]));
+        };
+        auto issue_pv = [&](int tile, uint32_t b, uint32_t i, bool more) {
+          const uint32_t vv = v_lo + (i % C::kRing) * (C::kRingBytes / 16);
+#pragma unroll
+          for (int k = 0; k < C::kN / 16; ++k)
+            mma_f16_ts(tmem + C::kOCol + W * tile, tmem + C::kN * b + 8 * k, desc(vv + k * 128), kIdescPV, more || k > 0);
+        };
+        Item it;
+        while (ok && (ok = next_item(it))) {
+          item_read();
+          if (it.seq < 0) break;
+          const int n = it.blk1 - it.blk0;
+          const int nt = C::kTiles == 2 && it.n_tokens > tile_tokens ? 2 : 1;
+          // Turn t is block t / nt of tile t % nt; the scores run kBufs turns ahead: S(t + kBufs) goes into the buffer that P V (t) has read.
+          int tile_v = 0, blk_v = 0, tile_k = 0, blk_k = 0;
+          for (int t = -C::kBufs; t < n * nt && ok; ++t) {
+            if (t >= 0) {
+              const uint32_t turn = turns + t, b = turn % C::kBufs, lv = ld + 2 * blk_v + 1;
+              if (tile_v == 0) ok = ring_wait(lv);
+              if (ok) ok = wait_bounded(wctx, &sh.p_full[b], (turn / C::kBufs) & 1, 0xb600 + b);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv(tile_v, b, lv, blk_v > 0);
+              if (nt < C::kBufs) tc_commit(smem_u32(&sh.o_done[tile_v]));      // otherwise the tile's next scores come after it
+              if (blk_v + 1 == n) tc_commit(smem_u32(&sh.o_final[tile_v]));
+              if (++tile_v == nt) {
+                ring_release(lv);
+                tile_v = 0;
+                ++blk_v;
+              }
+            }
+            if (blk_k < n) {
+              const uint32_t b = (turns + t + C::kBufs) % C::kBufs, lk = ld + 2 * blk_k;
+              if (blk_k == 0) ok = wait_bounded(wctx, &sh.q_full[tile_k], qn[tile_k]++ & 1, 0xb500 + tile_k);
+              if (ok && tile_k == 0) ok = ring_wait(lk);
+              if (!ok) break;
+              tc_fence_after();
+              issue_qk(tile_k, b, lk);
+              if (++tile_k == nt) {
+                ring_release(lk);
+                tile_k = 0;
+                ++blk_k;
+              }
+            }
+          }
+          turns += n * nt;
+          ld += 2 * n;
+        }
+        {
+          // products in flight, and their arrivals, end before tensor and shared memory are freed (with a limit)
+          tc_commit(smem_u32(&sh.drain));
+          const uint64_t t0 = global_timer_ns();
+          while (!mbar_try_wait(smem_u32(&sh.drain), 0) && global_timer_ns() - t0 < 20000000ull) {}
+        }
+      }
       __syncwarp();
     }
-    if (ok) {
-      Item none{};
-      none.seq = -1;
-      push(none);
-    }
-    if (!ok) {
-      // copies in flight, and an answer, land before the CTA's memory is given back (a wait each, with a limit)
-      if (asked) {
-        const uint64_t t0 = global_timer_ns();
-        while (!mbar_try_wait(smem_u32(&sh.given), answers & 1) && global_timer_ns() - t0 < 20000000ull) {}
-      }
-      for (uint32_t i = tiles > C::kRaw ? tiles - C::kRaw : 0; i < tiles; ++i) {
-        const uint64_t t0 = global_timer_ns();
-        while (!mbar_try_wait(smem_u32(&sh.raw_full[i % C::kRaw]), (i / C::kRaw) & 1) && global_timer_ns() - t0 < 20000000ull) {}
-      }
-    }
-  } else if (warp == C::kMmaWarp) {
-    // ---------------------------------------------------------------- issuer
-    if (elect_one()) {
-      constexpr uint32_t kIdescQK = idesc(C::kN, false), kIdescPV = idesc(W, true);
-      constexpr uint32_t kColQ = kTileM * 128 / 16, kColK = C::kN * 128 / 16;     // column blocks of Q and K in 16 bytes
-      const uint32_t q_lo = desc_lo(s_q, 16), k_lo = desc_lo(s_ring, 16), v_lo = desc_lo(s_ring, C::kN * 128);
-      bool ok = true;
-      uint32_t ld = 0;                                           // widened tiles used so far: K, V, K, V ...
-      uint32_t qn[2] = {0, 0};                                   // q_full phases by tile
-      uint32_t turns = 0;                                        // of the score buffers, before this item
-      auto ring_wait = [&](uint32_t i) { return wait_bounded(wctx, &sh.ring_full[i % C::kRing], (i / C::kRing) & 1, 0xb400); };
-      auto ring_release = [&](uint32_t i) { tc_commit(smem_u32(&sh.ring_empty[i % C::kRing])); };
-      auto issue_qk = [&](int tile, uint32_t b, uint32_t i) {
-        const uint32_t kk = k_lo + (i % C::kRing) * (C::kRingBytes / 16), qq = q_lo + tile * (C::kQBytes / 16);
-#pragma unroll
-        for (int k = 0; k < W / 16; ++k)
-          mma_f16_ss(tmem + C::kN * b, desc(qq + (k >> 2) * kColQ + 2 * (k & 3)), desc(kk + (k >> 2) * kColK + 2 * (k & 3)), kIdescQK, k > 0);
-        tc_commit(smem_u32(&sh.s_full[b]));
-      };
-      auto issue_pv = [&](int tile, uint32_t b, uint32_t i, bool more) {
-        const uint32_t vv = v_lo + (i % C::kRing) * (C::kRingBytes / 16);
-#pragma unroll
-        for (int k = 0; k < C::kN / 16; ++k)
-          mma_f16_ts(tmem + C::kOCol + W * tile, tmem + C::kN * b + 8 * k, desc(vv + k * 128), kIdescPV, more || k > 0);
-      };
-      Item it;
-      while (ok && (ok = next_item(it))) {
-        item_read();
-        if (it.seq < 0) break;
-        const int n = it.blk1 - it.blk0;
-        const int nt = C::kTiles == 2 && it.n_tokens > tile_tokens ? 2 : 1;
-        // Turn t is block t / nt of tile t % nt; the scores run kBufs turns ahead: S(t + kBufs) goes into the buffer that P V (t) has read.
-        int tile_v = 0, blk_v = 0, tile_k = 0, blk_k = 0;
-        for (int t = -C::kBufs; t < n * nt && ok; ++t) {
-          if (t >= 0) {
-            const uint32_t turn = turns + t, b = turn % C::kBufs, lv = ld + 2 * blk_v + 1;
-            if (tile_v == 0) ok = ring_wait(lv);
-            if (ok) ok = wait_bounded(wctx, &sh.p_full[b], (turn / C::kBufs) & 1, 0xb600 + b);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(tile_v, b, lv, blk_v > 0);
-            if (nt < C::kBufs) tc_commit(smem_u32(&sh.o_done[tile_v]));      // otherwise the tile's next scores come after it
-            if (blk_v + 1 == n) tc_commit(smem_u32(&sh.o_final[tile_v]));
-            if (++tile_v == nt) {
-              ring_release(lv);
-              tile_v = 0;
-              ++blk_v;
-            }
-          }
-          if (blk_k < n) {
-            const uint32_t b = (turns + t + C::kBufs) % C::kBufs, lk = ld + 2 * blk_k;
-            if (blk_k == 0) ok = wait_bounded(wctx, &sh.q_full[tile_k], qn[tile_k]++ & 1, 0xb500 + tile_k);
-            if (ok && tile_k == 0) ok = ring_wait(lk);
-            if (!ok) break;
-            tc_fence_after();
-            issue_qk(tile_k, b, lk);
-            if (++tile_k == nt) {
-              ring_release(lk);
-              tile_k = 0;
-              ++blk_k;
-            }
-          }
-        }
-        turns += n * nt;
-        ld += 2 * n;
-      }
-      {
-        // products in flight, and their arrivals, end before tensor and shared memory are freed (with a limit)
-        tc_commit(smem_u32(&sh.drain));
-        const uint64_t t0 = global_timer_ns();
-        while (!mbar_try_wait(smem_u32(&sh.drain), 0) && global_timer_ns() - t0 < 20000000ull) {}
-      }
-    }
-    __syncwarp();
-  }
   } else if (warp >= C::kWideWarp0) {
     // ---------------------------------------------------------------- widening
     if constexpr (C::kDeal) setmaxnreg_dec<C::kWideRegs>();
@@ -1044,7 +1051,7 @@ cudaError_t launch_one(const CUtensorMap& tk, const CUtensorMap& tv, const KvAtt
     if (cached) ready[dev].store(true, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(plan.items), 1, 1);      // below 2^31 / 32: kv_prefill_takes wants 33 rows a sequence
+  cfg.gridDim = dim3(static_cast<unsigned>(plan.items), 1, 1);      // below 2^28: kv_prefill_takes wants 17 rows of a sequence
   cfg.blockDim = dim3(C::kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -1062,15 +1069,22 @@ cudaError_t launch_one(const CUtensorMap& tk, const CUtensorMap& tv, const KvAtt
 
 }  // namespace
 
-// Against the kernel for few rows (us here / there; H 4 Hk, page 64, keys as given):
-//   32 rows a sequence and K/V head, D 128:  8 heads of 1 x 16000 keys 41 / R32A, of 8 x 4000 49 / R32B, of 32 x 1000 51 / R32C
-//   64 rows, D 128:  44 / R64A, 55 / R64B, 54 / R64C;  D 64, 4 heads:  36 / 18, 30 / 23, 24 / 26;  D 256, 4 heads:  52 / 41, 47 / 68, 40 / 78
-//   128 rows, D 128: 49 / 60, 60 / 108, 64 / 140
-// There the keys are split over the whole GPU however few the sequences, and 32 rows (16 at D 256) share what is read.
+// The kernel for few rows reads a K/V head's keys once for every 32 rows (16 at head dims above 128), so its time goes with blocks of rows
+// times keys, a block counting for some 400 keys more: about 10 us, and 1 us per 9300 of these at head dim 128, per 19000 at 64 and per 9300 of
+// the smaller blocks at 256.  This kernel reads them once for 256 (128) rows, but starts later.  Measured, few rows / this one, us
+// (H = 4 Hk; 8 K/V heads at head dim 128, otherwise 4):
+//   rows of a sequence      32             64             128            32, D 64   64      128      32, D 256  64      128
+//   1 x 16000 keys          31 / 39        42 / 41        65 / 45        17 / 33  18 / 34  24 / 35   30 / 51  43 / 52  69 / 56
+//   8 x  4000               42 / 45        67 / 47       117 / 53        17 / 27  23 / 28  37 / 28   42 / 45  70 / 47 129 / 50
+//  32 x  1000               48 / 48        79 / 49       140 / 55        19 / 21  28 / 22  43 / 24   47 / 40  80 / 40 150 / 42
+//   1 x  1000               13 / 21        14 / 22        15 / 24        10 / 17  10 / 17  10 / 19   13 / 27  14 / 28  15 / 33
+// and 16 sequences of 17 to 300 new tokens and up to 512 keys, a row a token, 47 / 27.  They meet near 300000 blocks times keys.  The host
+// knows how many keys the page table can hold, and takes that.
+constexpr int64_t kFewRowsMost = 128, kFewRowsKeys = 300000, kBlockKeys = 400;
 bool kv_prefill_takes(const KvAttendSizes& z) {
-  const int64_t group = z.heads_q / z.heads, rows = (z.tokens * group + z.batch - 1) / z.batch;
-  if (group > kTileM || rows <= 32) return false;
-  return rows > 64 || z.batch * z.heads > (width_of(z.head_dim) == 64 ? 64 : 16);
+  const int64_t group = z.heads_q / z.heads, rows = (z.tokens * group + z.batch - 1) / z.batch, block = width_of(z.head_dim) == 256 ? 16 : 32;
+  if (group > kTileM || rows <= block) return false;
+  return rows > kFewRowsMost || z.batch * z.heads * ((rows + block - 1) / block) * (z.keys_most + kBlockKeys) > kFewRowsKeys;
 }
 
 KvPrefillPlan kv_prefill_plan(const KvAttendSizes& z, int sms) {
