@@ -134,7 +134,7 @@ def paged_kv_append(cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.T
     strides allowed (parts of a fused projection).  Per page and head, and K and V apart, the scale is the smallest
     power of two 2^e, -64 <= e <= 64, by which the largest finite |x| written to the page fits the fp8 range.  It starts
     anew with the page's first token and otherwise only grows; when it does, the page's older tokens are rounded anew.
-    x8 = fp8(x / descale), to the nearest, infinities as the largest number.  No two sequences may write to the same page.
+    x8 = fp8(x / descale), to the nearest, infinities (and what is beyond 2^64 times the range) as the largest number.  No two sequences may write to the same page.
     Stream-ordered; one kernel, nothing allocated."""
     native = _native()
     if native:
@@ -203,7 +203,7 @@ def flash_attention_paged_kv(q: torch.Tensor, cache, page_table: torch.Tensor, s
     q: float16 or bfloat16 [tokens, heads, head_dim], a view with strides allowed; heads a multiple of the cache's (query
     head h reads K/V head h // (heads // heads_kv)).  With is_causal new token i of sequence b sees the keys up to its
     own position, seqlens[b] - n_b + i; without it every key of its sequence.  A row that sees no key is zeros (its
-    log-sum-exp -inf).  Scores, softmax and sums are fp32; K and V enter exactly as the cache holds them.
+    log-sum-exp -inf); a NaN reaches the rows that see its key and no others.  Scores, softmax and sums are fp32; K and V enter exactly as the cache holds them.
     Returns [O], O in q's type [tokens, heads, head_dim] (`out` if given: contiguous), and with return_lse the fp32
     [tokens, heads] log-sum-exp of the scaled scores.  Rows outside cu_seqlens are left as they were.  Stream-ordered;
     nothing synchronises."""

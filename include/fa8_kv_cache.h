@@ -11,7 +11,8 @@
  * The cache.  Keys and values of all sequences live in a pool of pages of `page_size` tokens:
  *   k, v                  fp8 [num_pages, heads_kv, page_size, head_dim], contiguous
  *   k_descale, v_descale  fp32 [num_pages, heads_kv]: a scale for each block of page_size tokens and
- *                         head, x = descale * x8
+ *                         head, x = descale * x8; finite and not negative (as fa8_kv_append leaves
+ *                         them) where a token of the page is held
  * Sequence b has seqlens[b] tokens, those that the call is about included; its token p lies in slot
  * p % page_size of page page_table[b][p / page_size].  A call is about the last n_b tokens of each
  * sequence ("new" ones): rows cu_seqlens[b] .. cu_seqlens[b+1]-1 of the token-major tensors, or
@@ -25,6 +26,9 @@
  * device only, so the kernels check them: such a page or sequence is left out (read: zeros;
  * attention: its keys do not count), nothing outside the tensors is touched, and FA8_ERR_BAD_INDEX
  * is reported the way expired waits are, by fa8_check_status and by the next call on the device.
+ *
+ * Limits (FA8_ERR_UNSUPPORTED past them): table_width * page_size, tokens and tokens * heads up to
+ * 2^31 - 256, num_pages * heads_kv up to 2^31 - 1, 65536 heads_kv.
  */
 #ifndef FA8_KV_CACHE_H_
 #define FA8_KV_CACHE_H_
@@ -64,8 +68,8 @@ typedef struct fa8_kv_cache {
  * 8; bases 16-byte aligned), so both may be views of a fused projection's output.
  *
  * Per touched page and head, for K and V apart: a = max |x| over the page's new finite values and
- * e = the smallest exponent in [-64, 64] with a <= MAX * 2^e (a = 0: -64), MAX = 448 (e4m3) or
- * 57344 (e5m2).  If the page's first slot is among the new tokens the page starts anew with descale
+ * e = the smallest exponent in [-64, 64] with a <= MAX * 2^e (a = 0: -64; above all of them: 64, and
+ * what does not fit becomes +-MAX), MAX = 448 (e4m3) or 57344 (e5m2).  If the page's first slot is among the new tokens the page starts anew with descale
  * 2^e.  Otherwise its descale d becomes max(d, 2^e), and if that is larger the older tokens of the
  * page are rounded anew, x8 = fp8(x8 * d_old / d_new).  New tokens: x8 = fp8(x / d), to the nearest,
  * ties to even; infinities become +-MAX, NaN stays NaN.  Scales are powers of two: fp8 keeps its
@@ -96,7 +100,8 @@ typedef struct fa8_kv_attention_params {
   int64_t workspace_bytes;
 } fa8_kv_attention_params;
 
-/* Attention of the new tokens' queries over their sequences' pages. */
+/* Attention of the new tokens' queries over their sequences' pages.  What a row does not see does not
+ * count, whatever is held there: a NaN reaches the rows that see its key, in the columns that hold it. */
 int fa8_kv_attention(const fa8_kv_attention_params* params, void* cuda_stream);
 
 /* Bytes of workspace for a call of these sizes on a device of `sm_count` SMs; host arithmetic only.
