@@ -381,6 +381,88 @@ def test_token_ranges_that_decrease_are_always_reported(op, cu, rows_of):
     check_status(DEV)
 
 
+@pytest.mark.parametrize("n", [1, 4, 140])
+def test_sequences_that_share_pages_and_rows_that_share_memory(n):
+    """Two sequences with the same first pages; q, k and v whose rows or heads are one (strides of zero)."""
+    H, Hk, D, P, half = 4, 2, 64, 16, torch.float16
+    cache, table = filled(Hk, D, P, E4M3, [(n, 200 + n), (n, 200 + n)], seed=35)
+    table[1, :12] = table[0, :12]                                 # 192 tokens
+    lens = torch.tensor([200 + n] * 2, dtype=torch.int32)
+    where = to(DEV, table, lens)
+    g = torch.Generator().manual_seed(36)
+    dev = PagedKVCache(*to(DEV, *cache))
+    k = torch.randn(2 * n, 1, D, generator=g).to(half).to(DEV).expand(2 * n, Hk, D)
+    v = torch.randn(1, Hk, D, generator=g).to(half).to(DEV).expand(2 * n, Hk, D)
+    q = torch.randn(2 * n, 1, D, generator=g).to(half).to(DEV).expand(2 * n, H, D)
+    paged_kv_append(dev, k, v, *where)
+    after = po.append(cache, k.cpu(), v.cpu(), table, lens)
+    for x, y in zip(dev, after):
+        assert torch.equal(x.cpu().float().nan_to_num(-1.0), y.float().nan_to_num(-1.0))
+    out, lse = flash_attention_paged_kv(q, dev, *where, True, 0.2, return_lse=True)
+    check_status(DEV)
+    check_attention(q, after, table, lens, True, 0.2, None, out, lse)
+
+
+def test_offsets_past_32_bits_of_the_pool():
+    """A pool of more than 2^32 bytes for K and for V, of which the last pages are used: as in a pool of those pages alone."""
+    Hk, D, P, half, pages = 8, 128, 64, torch.bfloat16, 70000
+    if torch.cuda.mem_get_info(DEV)[0] < 20 * 2 ** 30:
+        pytest.skip("needs 20 GB")
+    seqs = [(1, 300), (3, 70), (150, 150)]
+    cu, T, lens = ranges(seqs)
+    g = torch.Generator().manual_seed(37)
+    big, small = PagedKVCache.empty(pages, Hk, D, P, device=DEV), PagedKVCache.empty(40, Hk, D, P, device=DEV)
+    assert big.k.numel() > 2 ** 32
+    table = torch.randperm(40, generator=g)[:15].view(3, 5).to(torch.int32)
+    for t in small:
+        t.zero_()
+    for t in big:
+        t[-40:].zero_()
+    k, v, q = (torch.randn(T, h, D, generator=g).to(half).to(DEV) for h in (Hk, Hk, 4 * Hk))
+    results = []
+    for cache, first in ((small, 0), (big, pages - 40)):
+        where = to(DEV, table + first, lens)
+        paged_kv_append(cache, k, v, *where, cu_seqlens=cu.to(DEV))
+        results.append([x[-40:] for x in cache] + list(paged_kv_read(cache, *where, T, cu_seqlens=cu.to(DEV), dtype=half))
+                       + flash_attention_paged_kv(q, cache, *where, True, 0.1, cu_seqlens=cu.to(DEV)))
+        results[-1] += flash_attention_paged_kv(q[:3], cache, *where, True, 0.1)
+    check_status(DEV)
+    for x, y in zip(*results):
+        assert torch.equal(bits(x), bits(y))
+
+
+def test_offsets_past_32_bits_of_the_rows():
+    """More than 2^31 elements of rows: the last sequence's are those of a call of its own."""
+    heads, D, P, half, n, B = 256, 128, 64, torch.float16, 10, 7000
+    if torch.cuda.mem_get_info(DEV)[0] < 40 * 2 ** 30:
+        pytest.skip("needs 40 GB")
+    T = n * B
+    x = torch.empty(T, heads, D, dtype=half, device=DEV)
+    assert x.numel() > 2 ** 31
+    x[:-4 * n].zero_()
+    g = torch.Generator().manual_seed(38)
+    x[-4 * n:] = torch.randn(4 * n, heads, D, generator=g).to(half).to(DEV)
+    cache = PagedKVCache.empty(B, heads, D, P, device=DEV)
+    table = torch.arange(B, dtype=torch.int32, device=DEV).view(B, 1)
+    lens = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    paged_kv_append(cache, x, x, table, lens)
+    alone = PagedKVCache.empty(4, heads, D, P, device=DEV)
+    paged_kv_append(alone, x[-4 * n:], x[-4 * n:], table[:4], lens[:4])
+    for a, b in zip(cache, alone):
+        a, b = (a[-4:], b) if a.dim() == 2 else (a[-4:, :, :n], b[:, :, :n])
+        assert torch.equal(bits(a), bits(b))
+    got = paged_kv_read(cache, table, lens, T, dtype=half)
+    want = paged_kv_read(alone, table[:4], lens[:4], 4 * n, dtype=half)
+    assert torch.equal(bits(got[0][-4 * n:]), bits(want[0])) and torch.equal(bits(got[1][-4 * n:]), bits(want[1]))
+    del got
+    out = flash_attention_paged_kv(x, cache, table, lens, True, 0.1)[0]
+    check_status(DEV)
+    last = x[-n:].cpu()
+    o, _, A = po.attention(last, [t.cpu() for t in alone], table[3:4].cpu(), lens[:1].cpu(), True, 0.1)
+    assert bool(((out[-n:].double().cpu() - o).abs() <= torch.finfo(half).eps / 2 * o.abs() + 1.25 * 2.0 ** -11 * A + 2.0 ** -25).all())
+    assert not bool(out[:-4 * n].any())
+
+
 # ---- a run of them, graphs, streams ---------------------------------------------------------------------------
 
 def test_generation_step_by_step_and_read_back():
