@@ -26,6 +26,7 @@
 // work.  A quarter of the exponentials by a polynomial instead gained 2 % and was left out.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "fa8_kernel.h"
@@ -88,7 +89,7 @@ struct Item {
   int token0, n_tokens;                  // its new tokens in the item
   int blk0, blk1;                        // key blocks
   int vis;                               // keys that the item's last row sees
-  int part;
+  int part;                              // of its keys; -1: all of them
 };
 
 template <int W>
@@ -199,6 +200,10 @@ __device__ __forceinline__ void widen16(const uint4& x, uint32_t f, uint4& lo, u
   lo = make_uint4(r[0], r[1], r[2], r[3]);
   hi = make_uint4(r[4], r[5], r[6], r[7]);
 }
+
+// Parts that an item of n_blk blocks is cut into, at most `most`.
+constexpr int kPartBlocks = 4;
+__device__ __forceinline__ int parts_of(int n_blk, int most) { return max(1, min(most, n_blk / kPartBlocks)); }
 
 // What the softmax of a row carries from block to block.
 struct Row {
@@ -391,9 +396,11 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         it.n_tokens = min(plan.block_tokens, s.n - it.token0);
         it.vis = a.causal ? max(0, min(s.len, s.len - s.n + it.token0 + it.n_tokens)) : s.len;
         const int n_blk = max(1, (it.vis + C::kN - 1) / C::kN);
-        it.blk0 = static_cast<int>(static_cast<int64_t>(n_blk) * it.part / plan.parts);
-        it.blk1 = static_cast<int>(static_cast<int64_t>(n_blk) * (it.part + 1) / plan.parts);
-        if (it.blk0 == it.blk1) return;
+        const int parts = parts_of(n_blk, plan.parts);
+        if (it.part >= parts) return;
+        it.blk0 = static_cast<int>(static_cast<int64_t>(n_blk) * it.part / parts);
+        it.blk1 = static_cast<int>(static_cast<int64_t>(n_blk) * (it.part + 1) / parts);
+        if (parts == 1) it.part = -1;
         push(it);
         if (!ok) return;
 
@@ -884,7 +891,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       if (!ok) break;
 
       // ---- O ----
-      const bool whole = plan.parts == 1;
+      const bool whole = it.part < 0;
       row.l += exchange(row.l);
       ok = !pair_any(!wait_bounded(wctx, &sh.o_final[tile], taken & 1, 0xbc00 + tile));
       if (!ok) break;
@@ -962,7 +969,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           float* const partial = plan.partial_o + static_cast<int64_t>(i.part) * a.c.tokens * a.heads_q * a.c.head_dim;
           write_nans<kE5M2>(a.c, i.seq, i.head, max(apart(i), i.blk0) * C::kN, min(i.len - i.n + token0 + t + 1, i.blk1 * C::kN),
                             part * kMyCols + lane, min(a.c.head_dim, (part + 1) * kMyCols), [&](int col) {
-            if (plan.parts == 1) static_cast<uint16_t*>(a.o)[to + col] = 0x7fff;       // a NaN in either type
+            if (i.part < 0) static_cast<uint16_t*>(a.o)[to + col] = 0x7fff;       // a NaN in either type
             else partial[to + col] = NAN;
           });
         }
@@ -993,18 +1000,16 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a, cons
   const int token0 = (token - s.first) / plan.block_tokens * plan.block_tokens;
   const int n_tokens = min(plan.block_tokens, s.n - token0);
   const int vis = a.causal ? max(0, min(s.len, s.len - s.n + token0 + n_tokens)) : s.len;
-  const int64_t n_blk = max(1, (vis + block_keys - 1) / block_keys);
+  const int parts = parts_of(max(1, (vis + block_keys - 1) / block_keys), plan.parts);
+  if (parts == 1) return;
   const int D = a.c.head_dim, quads = D >> 2;
   const int64_t rows = static_cast<int64_t>(a.c.tokens) * a.heads_q;
-  auto empty = [&](int p) { return n_blk * p / plan.parts == n_blk * (p + 1) / plan.parts; };
   float m = -INFINITY;
-  for (int p = 0; p < plan.parts; ++p)
-    if (!empty(p)) m = fmaxf(m, ld_global(plan.partial_ml + 2 * (p * rows + row)));
+  for (int p = 0; p < parts; ++p) m = fmaxf(m, ld_global(plan.partial_ml + 2 * (p * rows + row)));
   float l = 0.f;
   float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll 4
-  for (int p = 0; p < plan.parts; ++p) {
-    if (empty(p)) continue;
+  for (int p = 0; p < parts; ++p) {
     const float* ml = plan.partial_ml + 2 * (p * rows + row);
     const float mp = ld_global(ml);
     const float f = mp == -INFINITY ? 0.f : ex2_approx(mp - m);
@@ -1087,18 +1092,19 @@ bool kv_prefill_takes(const KvAttendSizes& z) {
   return rows > kFewRowsMost || z.batch * z.heads * ((rows + block - 1) / block) * (z.keys_most + kBlockKeys) > kFewRowsKeys;
 }
 
+constexpr int kPartsMost = 16;
 KvPrefillPlan kv_prefill_plan(const KvAttendSizes& z, int sms) {
   KvPrefillPlan p{};
   const int width = width_of(z.head_dim), tiles = width == 256 ? 1 : 2;
   p.block_tokens = kTileM / (z.heads_q / z.heads) * tiles;
   p.items = kv_slots(z.batch, z.tokens, z.tokens / z.batch, z.ragged, p.block_tokens, 1) * z.heads;
   p.parts = 1;
-  // Few items: their keys are cut into as many parts as fill the GPU once.
-  const int64_t blocks = (z.keys_most + PCfg<128>::kN - 1) / PCfg<128>::kN;
-  int64_t parts = sms / (p.items > 0 ? p.items : 1);
-  if (parts > 16) parts = 16;
-  if (parts > blocks / 4) parts = blocks / 4;
-  if (parts > 1) p.parts = static_cast<int>(parts);
+  // Few items: their keys are cut into as many parts as fill the GPU once, where they have that many (parts_of).  More parts than CTAs at once
+  // (to even out sequences of different lengths) helped some and hurt others: 11 short chunks over 500 to 12000 keys 96 -> 73 us, 3
+  // over 3000 to 9000 116 -> 136.
+  const int64_t blocks = (z.keys_most + (width == 256 ? PCfg<256>::kN : PCfg<128>::kN) - 1) / (width == 256 ? PCfg<256>::kN : PCfg<128>::kN);
+  const int64_t parts = std::min(blocks / kPartBlocks, sms / std::max<int64_t>(1, p.items));
+  p.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kPartsMost, parts)));
   p.items *= p.parts;
   return p;
 }
