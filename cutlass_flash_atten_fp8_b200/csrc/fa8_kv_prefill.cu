@@ -1098,11 +1098,10 @@ KvPrefillPlan kv_prefill_plan(const KvAttendSizes& z, int sms) {
   const int width = width_of(z.head_dim), tiles = width == 256 ? 1 : 2;
   p.block_tokens = kTileM / (z.heads_q / z.heads) * tiles;
   p.items = kv_slots(z.batch, z.tokens, z.tokens / z.batch, z.ragged, p.block_tokens, 1) * z.heads;
-  p.parts = 1;
   // Few items: their keys are cut into as many parts as fill the GPU once, where they have that many (parts_of).  More parts than CTAs at once
   // (to even out sequences of different lengths) helped some and hurt others: 11 short chunks over 500 to 12000 keys 96 -> 73 us, 3
   // over 3000 to 9000 116 -> 136.
-  const int64_t blocks = (z.keys_most + (width == 256 ? PCfg<256>::kN : PCfg<128>::kN) - 1) / (width == 256 ? PCfg<256>::kN : PCfg<128>::kN);
+  const int64_t block = width == 256 ? PCfg<256>::kN : PCfg<128>::kN, blocks = (z.keys_most + block - 1) / block;
   const int64_t parts = std::min(blocks / kPartBlocks, sms / std::max<int64_t>(1, p.items));
   p.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kPartsMost, parts)));
   p.items *= p.parts;
