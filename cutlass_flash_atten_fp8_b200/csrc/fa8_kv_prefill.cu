@@ -32,6 +32,7 @@
 #include "fa8_kernel.h"
 #include "fa8_kv.h"
 #include "kv_common.cuh"
+#include "kv_turns.h"
 
 namespace fa8 {
 
@@ -98,7 +99,7 @@ struct Shared {
   uint64_t item_full[kItemSlots], item_empty[kItemSlots];
   uint64_t raw_full[C::kRaw], raw_empty[C::kRaw];
   uint64_t ring_full[C::kRing], ring_empty[C::kRing];
-  uint64_t s_full[C::kBufs], p_full[C::kBufs];
+  uint64_t s_full[C::kTiles][C::kBufs], p_full[C::kBufs];     // kv_turns.h
   uint64_t q_full[2], o_done[2], o_final[2];     // by tile
   uint64_t blk_full[kBlockSlots];
   uint64_t drain, given;
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     init(sh.ring_full, C::kRing, 4);
     init(sh.ring_empty, C::kRing, 1);
     init(sh.q_full, 2, 8);
-    init(sh.s_full, C::kBufs, 1);
+    init(&sh.s_full[0][0], C::kTiles * C::kBufs, 1);
     init(sh.p_full, C::kBufs, 8);
     init(sh.o_done, 2, 1);
     init(sh.o_final, 2, 1);
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
 #pragma unroll
           for (int k = 0; k < W / 16; ++k)
             mma_f16_ss(tmem + C::kN * b, desc(qq + (k >> 2) * kColQ + 2 * (k & 3)), desc(kk + (k >> 2) * kColK + 2 * (k & 3)), kIdescQK, k > 0);
-          tc_commit(smem_u32(&sh.s_full[b]));
+          tc_commit(smem_u32(&sh.s_full[tile][b]));
         };
         auto issue_pv = [&](int tile, uint32_t b, uint32_t i, bool more) {
           const uint32_t vv = v_lo + (i % C::kRing) * (C::kRingBytes / 16);
@@ -568,9 +569,9 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           int tile_v = 0, blk_v = 0, tile_k = 0, blk_k = 0;
           for (int t = -C::kBufs; t < n * nt && ok; ++t) {
             if (t >= 0) {
-              const uint32_t turn = turns + t, b = turn % C::kBufs, lv = ld + 2 * blk_v + 1;
+              const uint32_t turn = turns + t, b = turn_buffer<C::kBufs>(turn), lv = ld + 2 * blk_v + 1;
               if (tile_v == 0) ok = ring_wait(lv);
-              if (ok) ok = wait_bounded(wctx, &sh.p_full[b], (turn / C::kBufs) & 1, 0xb600 + b);
+              if (ok) ok = wait_bounded(wctx, &sh.p_full[b], turn_parity<C::kBufs>(turn), 0xb600 + b);
               if (!ok) break;
               tc_fence_after();
               issue_pv(tile_v, b, lv, blk_v > 0);
@@ -583,7 +584,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
               }
             }
             if (blk_k < n) {
-              const uint32_t b = (turns + t + C::kBufs) % C::kBufs, lk = ld + 2 * blk_k;
+              const uint32_t b = turn_buffer<C::kBufs>(turns + t + C::kBufs), lk = ld + 2 * blk_k;
               if (blk_k == 0) ok = wait_bounded(wctx, &sh.q_full[tile_k], qn[tile_k]++ & 1, 0xb500 + tile_k);
               if (ok && tile_k == 0) ok = ring_wait(lk);
               if (!ok) break;
@@ -728,8 +729,8 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     };
     uint32_t blocks = 0;                                         // of all items (the residual ring), also those this tile sits out
     uint32_t turns = 0;                                          // of the score buffers, before this item
-    uint32_t ahead = 0;                                          // blocks of this tile in items whose scores run ahead
-    uint32_t taken = 0;                                          // items this tile took part in
+    uint32_t seen = 0;                                           // of this tile's barriers (kv_turns.h)
+    constexpr uint32_t kDone = kSeenDone<C::kBufs>, kFinal = kSeenFinal<C::kBufs>;
     Item it;
     bool ok = true;
     while (true) {
@@ -804,12 +805,13 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       row.lim = a.causal ? max(0, min(it.len, it.len - it.n + my_token + 1)) : it.len;
       const int least = a.causal ? max(0, min(it.len, it.len - it.n + tok0 + 1)) : it.len;       // of the tile's first row
       float vref = 1.f;
-      for (int j = 0; j < nb && ok; ++j, ahead += nt < C::kBufs) {
-        const uint32_t turn = turns + j * nt + tile, buf = turn % C::kBufs;
+      for (int j = 0; j < nb && ok; ++j) {
+        const uint32_t buf = turn_buffer<C::kBufs>(turns + j * nt + tile);
         const uint32_t n = (blocks + j) % kBlockSlots;
         const uint32_t t_p = tmem + lanes + C::kN * buf, t_s = t_p + part * kMyKeys;
         ok = wait_bounded(wctx, &sh.blk_full[n], ((blocks + j) / kBlockSlots) & 1, 0xb900);
-        if (ok) ok = wait_bounded(wctx, &sh.s_full[buf], (turn / C::kBufs) & 1, 0xba00 + buf);
+        if (ok) ok = wait_bounded(wctx, &sh.s_full[tile][buf], seen_parity(seen, buf), 0xba00 + buf);
+        seen = seen_next(seen, buf);
         __syncwarp();
         tc_fence_after();
         const int key0 = (it.blk0 + j) * C::kN, lim = row.lim - key0 - part * kMyKeys;
@@ -871,7 +873,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           row.most = m == -INFINITY ? 0.f : kRaiseAbove;
           row.l *= alpha;
           if (j > 0) {
-            if (nt < C::kBufs) ok = wait_bounded(wctx, &sh.o_done[tile], (ahead - 1) & 1, 0xbb00 + tile) && ok;
+            if (nt < C::kBufs) ok = wait_bounded(wctx, &sh.o_done[tile], seen_parity(seen, kDone) ^ 1u, 0xbb00 + tile) && ok;
             __syncwarp();
             tc_fence_after();
             rescale(t_o, kMyCols, alpha);
@@ -885,6 +887,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[buf]));
+        if (nt < C::kBufs) seen = seen_next(seen, kDone);
       }
       blocks += nb;
       turns += nb * nt;
@@ -893,9 +896,9 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       // ---- O ----
       const bool whole = it.part < 0;
       row.l += exchange(row.l);
-      ok = !pair_any(!wait_bounded(wctx, &sh.o_final[tile], taken & 1, 0xbc00 + tile));
+      ok = !pair_any(!wait_bounded(wctx, &sh.o_final[tile], seen_parity(seen, kFinal), 0xbc00 + tile));
       if (!ok) break;
-      ++taken;
+      seen = seen_next(seen, kFinal);
       tc_fence_after();
       const float inv = (row.l == 0.f ? 0.f : (whole ? 1.f / row.l : 1.f)) * vref;
       const int token = (r * over_group) >> 16;

@@ -342,6 +342,35 @@ def test_nan_in_keys_that_only_some_rows_see(seqs, H, Hk, D, P, fp8):
     assert bool(((got - want).abs() <= limit)[held].all())
 
 
+ITEMS = [(300, 300), (100, 500), (640, 640), (129, 700), (513, 1000), (90, 90), (257, 300), (20, 1200)]
+
+
+@pytest.mark.parametrize("H,Hk,D,P", [(16, 16, 128, 64), (32, 16, 96, 16), (16, 16, 256, 32), (48, 24, 128, 128)])
+@pytest.mark.parametrize("half,fp8", [(torch.float16, E4M3), (torch.bfloat16, E5M2)])
+@pytest.mark.parametrize("far", [False, True], ids=["scales near", "scales far apart"])
+def test_more_items_than_sms_of_which_some_have_one_tile(H, Hk, D, P, half, fp8, far):
+    """CTAs that take over one item after another, where the last new tokens of a sequence fill no second tile of rows; with
+    scales so far apart that they go through the softmax, which is slower, and without."""
+    cu, T, lens = ranges(ITEMS)
+    cache, table = filled(Hk, D, P, fp8, ITEMS, seed=80)
+    if far:
+        g = torch.Generator().manual_seed(81)
+        for d, least in zip(cache[2:], (-30, -40)):
+            d.copy_(torch.exp2(torch.randint(least, -7, d.shape, generator=g).float()))
+    q = rows(T, H, D, half, 82, False, cu, ITEMS)
+    where = to(DEV, table, lens, cu)
+    out, lse = flash_attention_paged_kv(q, to(DEV, *cache), where[0], where[1], True, 0.05, cu_seqlens=where[2], return_lse=True)
+    check_status(DEV)
+    if not far:
+        return check_attention(q, cache, table, lens, True, 0.05, cu, out, lse)
+    # A probability (times its V's scale) below fp16's normal range is off by 2^-25 at most where the row's largest is 2^6 or more, so
+    # n keys move a column by n 2^-25 448 / 2^6 of the largest value: less than 448 2^-25 of the row's largest sum, for n = 1200.
+    want, want_lse, A = po.attention(q.cpu(), cache, table, lens, True, 0.05, cu)
+    limit = torch.finfo(half).eps / 2 * want.abs() + 1.25 * 2.0 ** -11 * A + 448 * 2.0 ** -25 * A.amax(-1, keepdim=True) + 2.0 ** -25
+    assert bool(((out.double().cpu() - want).abs() <= limit).all())
+    assert bool(((lse.double().cpu() - want_lse).abs() <= 2.0 ** -20 * (want_lse.abs() + 16)).all())
+
+
 def test_page_table_of_wider_rows():
     """A view of a table that has more columns: as many as the longest sequence of this call needs."""
     seqs, H, Hk, D, P = [(1, 50), (1, 90), (1, 33)], 4, 2, 64, 16
