@@ -100,7 +100,8 @@ struct Shared {
   uint64_t raw_full[C::kRaw], raw_empty[C::kRaw];
   uint64_t ring_full[C::kRing], ring_empty[C::kRing];
   uint64_t s_full[C::kTiles][C::kBufs], p_full[C::kBufs];     // kv_turns.h
-  uint64_t q_full[2], o_done[2], o_final[2];     // by tile
+  uint64_t q_full[2], o_final[2];        // by tile
+  uint64_t o_done[C::kTiles][C::kBufs];
   uint64_t blk_full[kBlockSlots];
   uint64_t drain, given;
   uint4 answer;                          // to the request for another CTA's item
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     init(sh.q_full, 2, 8);
     init(&sh.s_full[0][0], C::kTiles * C::kBufs, 1);
     init(sh.p_full, C::kBufs, 8);
-    init(sh.o_done, 2, 1);
+    init(&sh.o_done[0][0], C::kTiles * C::kBufs, 1);
     init(sh.o_final, 2, 1);
     init(sh.blk_full, kBlockSlots, 1);
     init(&sh.drain, 1, 1);
@@ -575,7 +576,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
               if (!ok) break;
               tc_fence_after();
               issue_pv(tile_v, b, lv, blk_v > 0);
-              if (nt < C::kBufs) tc_commit(smem_u32(&sh.o_done[tile_v]));      // otherwise the tile's next scores come after it
+              if (nt < C::kBufs) tc_commit(smem_u32(&sh.o_done[tile_v][b]));      // otherwise the tile's next scores come after it
               if (blk_v + 1 == n) tc_commit(smem_u32(&sh.o_final[tile_v]));
               if (++tile_v == nt) {
                 ring_release(lv);
@@ -873,7 +874,10 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           row.most = m == -INFINITY ? 0.f : kRaiseAbove;
           row.l *= alpha;
           if (j > 0) {
-            if (nt < C::kBufs) ok = wait_bounded(wctx, &sh.o_done[tile], seen_parity(seen, kDone) ^ 1u, 0xbb00 + tile) && ok;
+            if (nt < C::kBufs) {
+              const uint32_t b = turn_buffer<C::kBufs>(turns + (j - 1) * nt + tile);
+              ok = wait_bounded(wctx, &sh.o_done[tile][b], seen_parity(seen, kDone + b) ^ 1u, 0xbb00 + tile) && ok;
+            }
             __syncwarp();
             tc_fence_after();
             rescale(t_o, kMyCols, alpha);
@@ -887,7 +891,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[buf]));
-        if (nt < C::kBufs) seen = seen_next(seen, kDone);
+        if (nt < C::kBufs) seen = seen_next(seen, kDone + buf);
       }
       blocks += nb;
       turns += nb * nt;

@@ -11,6 +11,12 @@
 //                     its turns, and may find the one before the awaited one still to come, which passes, or two gone by, which does not.)
 //   p_full[b]         a phase for each turn in buffer b, waited for by the issuer, which waits for them all, in their order; a warp adds to it
 //                     after its turn's s_full, and that turn's scores were issued after P V of the turn before it in the buffer.
+//   o_done[tile][b]   a phase for each turn of the tile's own in buffer b, in items with fewer tiles than buffers (in others the tile's next
+//                     scores come after the product), when its product P V is complete.  Asked for the tile's turn before the one whose
+//                     scores are there: that turn's own scores, there before, were issued after all earlier products from the buffer, and
+//                     the next product from it comes after that of the present turn, which needs P of the tile.
+//                     (One barrier for all of a tile's products will not do with three buffers and one tile: the scores of the first three
+//                     turns are issued ahead of all products, so that two can be outstanding.)
 //   o_final[tile]     a phase for each item that the tile is part of, all of which it waits for.
 #pragma once
 #include <cstdint>
@@ -28,12 +34,12 @@ namespace fa8 {
 template <int kBufs>
 FA8_HD constexpr uint32_t turn_buffer(uint32_t turn) { return turn % kBufs; }
 
-// `seen`: parities of the numbers of phases that a warp of a tile has waited for, or may take as gone by: bit b of s_full[tile][b] (below
-// kBufs), then of o_done and o_final.
+// `seen`: parities of the numbers of phases that a warp of a tile has waited for, or counts as gone by: bit b of s_full[tile][b], bit
+// kSeenDone + b of o_done[tile][b], bit kSeenFinal of o_final[tile].
 FA8_HD constexpr uint32_t seen_parity(uint32_t seen, uint32_t bit) { return (seen >> bit) & 1u; }
 FA8_HD constexpr uint32_t seen_next(uint32_t seen, uint32_t bit) { return seen ^ (1u << bit); }
 template <int kBufs> constexpr uint32_t kSeenDone = kBufs;
-template <int kBufs> constexpr uint32_t kSeenFinal = kBufs + 1;
+template <int kBufs> constexpr uint32_t kSeenFinal = 2 * kBufs;
 
 // Parity for a barrier with a phase for every turn in the buffer.
 template <int kBufs>

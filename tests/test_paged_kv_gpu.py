@@ -371,6 +371,30 @@ def test_more_items_than_sms_of_which_some_have_one_tile(H, Hk, D, P, half, fp8,
     assert bool(((lse.double().cpu() - want_lse).abs() <= 2.0 ** -20 * (want_lse.abs() + 16)).all())
 
 
+
+@pytest.mark.parametrize("H,Hk,D,P", [(16, 16, 64, 64), (16, 8, 32, 16), (4, 4, 128, 32), (4, 2, 256, 16)])
+@pytest.mark.parametrize("half,fp8", [(torch.float16, E4M3), (torch.bfloat16, E5M2)])
+def test_scores_that_rise_from_block_to_block(H, Hk, D, P, half, fp8):
+    """References are raised, and sums rescaled, at one block after another, in items of one tile and of two: a key's score is
+    about 14 times one more than the number of its 128 keys."""
+    seqs = [(100, 1000), (40, 700), (60, 60), (128, 129), (300, 900)] * (3 if D <= 64 else 1)
+    cu, T, lens = ranges(seqs)
+    cache, table = filled(Hk, D, P, fp8, seqs, seed=84)
+    g = torch.Generator().manual_seed(86)
+    for b, (_, s) in enumerate(seqs):
+        for key in range(0, s, 16):                               # sixteen keys lie in one page
+            row = torch.full((Hk, min(16, s - key), D), 1.0 + key // 128)
+            row[:, :, 0] = torch.randint(0, 4, row.shape[:2], generator=g).float()
+            cache[0][int(table[b, key // P]), :, key % P:key % P + row.shape[1]] = row.to(fp8)
+        cache[2][table[b, :-(-s // P)].long()] = 1.0
+    q = rows(T, H, D, half, 85, False, cu, seqs).abs()
+    scale = 14 / (0.8 * D)                                        # the mean of a normal number's size is 0.8
+    where = to(DEV, table, lens, cu)
+    out, lse = flash_attention_paged_kv(q, to(DEV, *cache), where[0], where[1], True, scale, cu_seqlens=where[2], return_lse=True)
+    check_status(DEV)
+    check_attention(q, cache, table, lens, True, scale, cu, out, lse)
+
+
 def test_page_table_of_wider_rows():
     """A view of a table that has more columns: as many as the longest sequence of this call needs."""
     seqs, H, Hk, D, P = [(1, 50), (1, 90), (1, 33)], 4, 2, 64, 16

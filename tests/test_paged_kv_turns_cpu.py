@@ -18,9 +18,9 @@ MODEL = r"""
 #include <vector>
 #include "kv_turns.h"
 struct Item { int blocks, tiles; };
-struct Op { bool pv; int turn, tile; bool last; };            // last: with a phase of o_final
+struct Op { bool pv; int turn, tile; bool done, last; };      // done, last: with a phase of o_done, of o_final
 enum Kind { kRead, kQ, kScores, kProbs, kFinal, kIssue, kAskProbs, kAskQ };
-struct Event { Kind kind; int at, before; uint32_t seen; };   // at: item, turn or op; before: items of the tile before
+struct Event { Kind kind; int at, before; bool ask_done; uint32_t seen, dones; };   // at: item, turn or op; before: the tile's turn before it in the item, or -1; dones: o_done's before that one
 static bool passes(uint32_t completed, uint32_t parity) { return ((completed & 1u) ^ 1u) == parity; }
 
 template <int kTiles, int kBufs>
@@ -28,44 +28,47 @@ struct Model {
   std::vector<Op> ops;
   std::vector<int> tile_of, s_op, pv_op;                      // of turns
   std::vector<Event> issuer, warp[2];
-  long wrong = 0, wrong_shared = 0;
+  long wrong = 0, wrong_shared = 0, wrong_done = 0;            // with one barrier a buffer for the scores, one a tile for the products
 
   explicit Model(const std::vector<Item>& items) {
     int turns = 0, asked[2] = {0, 0};
+    uint32_t dones[2] = {0, 0};
     uint32_t seen[2] = {0, 0};
     for (int i = 0; i < static_cast<int>(items.size()); ++i) {
       const int n = items[i].blocks, nt = items[i].tiles;
       for (int t = 0; t < n * nt; ++t) tile_of.push_back(t % nt);
       s_op.resize(turns + n * nt);
       pv_op.resize(turns + n * nt);
-      issuer.push_back({kRead, i, 0, 0});
+      issuer.push_back({kRead, i, 0, false, 0, 0});
       for (int t = -kBufs; t < n * nt; ++t) {
         if (t >= 0) {
-          issuer.push_back({kAskProbs, turns + t, 0, 0});
-          issuer.push_back({kIssue, static_cast<int>(ops.size()), 0, 0});
+          issuer.push_back({kAskProbs, turns + t, 0, false, 0, 0});
+          issuer.push_back({kIssue, static_cast<int>(ops.size()), 0, false, 0, 0});
           pv_op[turns + t] = static_cast<int>(ops.size());
-          ops.push_back({true, turns + t, t % nt, t / nt + 1 == n});
+          ops.push_back({true, turns + t, t % nt, nt < kBufs, t / nt + 1 == n});
         }
         const int s = t + kBufs;
         if (s < n * nt) {
-          if (s < nt) issuer.push_back({kAskQ, s, asked[s]++, 0});
-          issuer.push_back({kIssue, static_cast<int>(ops.size()), 0, 0});
+          if (s < nt) issuer.push_back({kAskQ, s, asked[s]++, false, 0, 0});
+          issuer.push_back({kIssue, static_cast<int>(ops.size()), 0, false, 0, 0});
           s_op[turns + s] = static_cast<int>(ops.size());
-          ops.push_back({false, turns + s, s % nt, false});
+          ops.push_back({false, turns + s, s % nt, false, false});
         }
       }
       for (int tile = 0; tile < kTiles; ++tile) {
         auto& w = warp[tile];
-        w.push_back({kRead, i, 0, 0});
+        w.push_back({kRead, i, 0, false, 0, 0});
         if (tile >= nt) continue;                             // sits the item out
-        w.push_back({kQ, i, 0, 0});
+        w.push_back({kQ, i, 0, false, 0, 0});
         for (int j = 0; j < n; ++j) {
           const int turn = turns + j * nt + tile;
-          w.push_back({kScores, turn, 0, seen[tile]});
+          w.push_back({kScores, turn, 0, false, seen[tile], 0});
           seen[tile] = fa8::seen_next(seen[tile], fa8::turn_buffer<kBufs>(turn));
-          w.push_back({kProbs, turn, 0, 0});
+          w.push_back({kProbs, turn, j > 0 ? turn - nt : -1, j > 0 && nt < kBufs, seen[tile], dones[tile] - 1});
+          dones[tile] += nt < kBufs;
+          if (nt < kBufs) seen[tile] = fa8::seen_next(seen[tile], fa8::kSeenDone<kBufs> + fa8::turn_buffer<kBufs>(turn));
         }
-        w.push_back({kFinal, turns + (n - 1) * nt + tile, 0, seen[tile]});
+        w.push_back({kFinal, turns + (n - 1) * nt + tile, 0, false, seen[tile], 0});
         seen[tile] = fa8::seen_next(seen[tile], fa8::kSeenFinal<kBufs>);
       }
       turns += n * nt;
@@ -127,6 +130,18 @@ struct Model {
         wrong_shared += passes(completed(in_b), fa8::turn_parity<kBufs>(e.at)) != have;
         return have;
       }
+      case kProbs:
+        if (e.ask_done) {
+          const bool have = pv_op[e.before] < s.done;
+          const uint32_t b = fa8::turn_buffer<kBufs>(e.before);
+          auto of_tile = [&](const Op& o) { return o.done && o.tile == tile; };
+          wrong += passes(completed([&](const Op& o) { return of_tile(o) && fa8::turn_buffer<kBufs>(o.turn) == b; }),
+                          fa8::seen_parity(e.seen, fa8::kSeenDone<kBufs> + b) ^ 1u) != have;
+          wrong_done += passes(completed(of_tile), e.dones & 1u) != have;
+        }
+        // otherwise the product before it came before these scores
+        else if (e.before >= 0) wrong += !(pv_op[e.before] < s.done);
+        return true;
       case kFinal: {
         const bool have = pv_op[e.at] < s.done;
         wrong += passes(completed([&](const Op& o) { return o.last && o.tile == tile; }), fa8::seen_parity(e.seen, fa8::kSeenFinal<kBufs>)) != have;
@@ -187,7 +202,7 @@ struct Model {
 
 template <int kTiles, int kBufs>
 void all() {
-  long wrong = 0, shared_two = 0, shared_mixed = 0, stuck = 0, runs = 0;
+  long wrong = 0, shared_two = 0, shared_mixed = 0, done = 0, stuck = 0, runs = 0;
   std::vector<std::vector<Item>> lists;
   for (int a = 1; a <= 3; ++a)
     for (int at = 1; at <= kTiles; ++at)
@@ -204,9 +219,10 @@ void all() {
     for (const Item& i : items) mixed = mixed || i.tiles < kTiles;
     wrong += m.wrong;
     (mixed ? shared_mixed : shared_two) += m.wrong_shared;
+    done += m.wrong_done;
     ++runs;
   }
-  std::printf("%ld %ld %ld %ld %ld\n", runs, wrong, stuck, shared_two, shared_mixed);
+  std::printf("%ld %ld %ld %ld %ld %ld\n", runs, wrong, stuck, shared_two, shared_mixed, done);
 }
 int main() {
   all<2, 2>();
@@ -225,11 +241,13 @@ def test_waits_pass_exactly_when_they_should(tmp_path):
     src.write_text(MODEL)
     subprocess.run([cxx, "-std=c++17", "-O2", "-I" + CSRC, str(src), "-o", exe], check=True)
     out = subprocess.run([exe], check=True, capture_output=True, text=True).stdout
-    for line, tiles in zip(out.splitlines(), (2, 2, 1)):
-        runs, wrong, stuck, shared_two, shared_mixed = map(int, line.split())
+    for line, tiles, buffers in zip(out.splitlines(), (2, 2, 1), (2, 3, 2)):
+        runs, wrong, stuck, shared_two, shared_mixed, done = map(int, line.split())
         assert runs > 10 and wrong == 0 and stuck == 0
         # a barrier per buffer for both tiles would do only while no tile sits an item out
         assert shared_two == 0 and (shared_mixed > 0) == (tiles == 2)
+        # one for all products of a tile while two buffers are all there are
+        assert (done > 0) == (buffers == 3)
 
 
 def test_the_kernel_uses_these_rules():
@@ -237,5 +255,6 @@ def test_the_kernel_uses_these_rules():
         text = f.read()
     for part in ("turn_buffer<C::kBufs>(turns + j * nt + tile)", "&sh.s_full[tile][buf], seen_parity(seen, buf)", "seen = seen_next(seen, buf)",
                  "tc_commit(smem_u32(&sh.s_full[tile][b]))", "&sh.p_full[b], turn_parity<C::kBufs>(turn)",
+                 "&sh.o_done[tile][b], seen_parity(seen, kDone + b) ^ 1u", "if (nt < C::kBufs) seen = seen_next(seen, kDone + buf)",
                  "&sh.o_final[tile], seen_parity(seen, kFinal)", "seen = seen_next(seen, kFinal)"):
         assert part in text, part
