@@ -901,10 +901,10 @@ __global__ void __launch_bounds__(32 * kCombineWarps) kv_combine_kernel(const Kv
         if (lane + 32 < quads) v[i][1] = ld_global(reinterpret_cast<const uint4*>(p + in * D) + lane + 32);
       }
     }
+    // (A reference of -inf is that of no keys, or of scores that are all NaN: its sums get the factor 0, which a NaN survives.)
     float top = m;
 #pragma unroll
     for (int i = 0; i < kAt; ++i) top = fmaxf(top, mp[i]);
-    if (top == -INFINITY) continue;
     const float back = m == -INFINITY ? 0.f : ex2_approx(m - top);
     m = top;
     l *= back;

@@ -362,7 +362,8 @@ def test_more_items_than_sms_of_which_some_have_one_tile(H, Hk, D, P, half, fp8,
     out, lse = flash_attention_paged_kv(q, to(DEV, *cache), where[0], where[1], True, 0.05, cu_seqlens=where[2], return_lse=True)
     check_status(DEV)
     if not far:
-        return check_attention(q, cache, table, lens, True, 0.05, cu, out, lse)
+        check_attention(q, cache, table, lens, True, 0.05, cu, out, lse)
+        return
     # A probability (times its V's scale) below fp16's normal range is off by 2^-25 at most where the row's largest is 2^6 or more, so
     # n keys move a column by n 2^-25 448 / 2^6 of the largest value: less than 448 2^-25 of the row's largest sum, for n = 1200.
     want, want_lse, A = po.attention(q.cpu(), cache, table, lens, True, 0.05, cu)
@@ -393,6 +394,28 @@ def test_scores_that_rise_from_block_to_block(H, Hk, D, P, half, fp8):
     out, lse = flash_attention_paged_kv(q, to(DEV, *cache), where[0], where[1], True, scale, cu_seqlens=where[2], return_lse=True)
     check_status(DEV)
     check_attention(q, cache, table, lens, True, scale, cu, out, lse)
+
+
+@pytest.mark.parametrize("seqs", [[(1, 20000), (1, 300)], [(3, 9000), (2, 12000)], [(1, 1500)], [(2, 700), (1, 40)], [(260, 3000)], [(150, 150), (300, 420)]],
+                         ids=["tokens over CTAs", "drafts over CTAs", "a cluster", "clusters", "parts", "prompts"])
+@pytest.mark.parametrize("H,Hk,D", [(4, 1, 128), (4, 2, 64), (2, 1, 256)])
+def test_nan_in_queries(seqs, H, Hk, D):
+    """A query row that holds a NaN is NaN, its log-sum-exp too, however its keys were shared out; the rows beside it are as they should be."""
+    P, half = 64, torch.bfloat16
+    cu, T, lens = ranges(seqs)
+    cache, table = filled(Hk, D, P, E4M3, seqs, seed=90)
+    q = rows(T, H, D, half, 91, False, cu, seqs)
+    q[0, 1, 5] = math.nan
+    q[T - 1, 0, D - 1] = math.nan
+    q[T // 2, H - 1] = math.nan
+    where = to(DEV, table, lens, cu)
+    out, lse = flash_attention_paged_kv(q, to(DEV, *cache), where[0], where[1], True, 0.1, cu_seqlens=where[2], return_lse=True)
+    check_status(DEV)
+    want, want_lse, A = po.attention(q.cpu(), cache, table, lens, True, 0.1, cu)
+    got, held = out.double().cpu(), ~torch.isnan(want)
+    assert torch.equal(torch.isnan(got), ~held) and torch.equal(torch.isnan(lse.cpu()), torch.isnan(want_lse))
+    limit = torch.finfo(half).eps / 2 * want.abs() + 1.25 * 2.0 ** -11 * A + 2.0 ** -25
+    assert bool(((got - want).abs() <= limit)[held].all())
 
 
 def test_page_table_of_wider_rows():
