@@ -22,7 +22,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libfa8_b200.so")
 HASH_PATH = os.path.join(PKG_DIR, "libfa8_b200.srchash")
 SOURCES = ["fa8_fwd_sm100.cu", "fa8_decode_sm100.cu", "fa8_quant.cu", "fa8_capi.cu",
            "fa8_kv_cache.cu", "fa8_kv_attend.cu", "fa8_kv_prefill.cu", "fa8_kv_capi.cu"]
-HEADERS = ["fa8_kernel.h", "fa8_kv.h", "kv_common.cuh", "kv_turns.h", "phase_rule.h", "ptx_sm100.cuh",
+HEADERS = ["fa8_kernel.h", "fa8_kv.h", "kv_common.cuh", "kv_turns.h", "phase_rule.h", "ptx_sm100.cuh", "status_word.cuh",
            os.path.join(REPO_DIR, "include", "fa8_b200.h"), os.path.join(REPO_DIR, "include", "fa8_kv_cache.h")]
 
 

@@ -41,6 +41,7 @@
 
 #include "fa8_kernel.h"
 #include "ptx_sm100.cuh"
+#include "status_word.cuh"
 
 namespace fa8 {
 
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(32 * DCfg<W, RB>::kMaxWarps, 1) fa8_decode_ker
   let_successor_start();
   // An earlier launch's expired wait is still in the status word: leave O alone, tell the host
   // (as the prefill kernel does).  The barriers below are passed all the same.
-  const bool stale = __any_sync(0xffffffffu, a.status != nullptr && *reinterpret_cast<volatile int*>(a.status) != 0);
+  const bool stale = __any_sync(0xffffffffu, wait_has_expired(a.status));
   if (stale && a.host_status != nullptr && threadIdx.x == 0 && *reinterpret_cast<volatile int*>(a.host_status) == 0)
     *reinterpret_cast<volatile int*>(a.host_status) = 0x5717;
 

@@ -60,6 +60,7 @@
 #include "fa8_kernel.h"
 #include "phase_rule.h"
 #include "ptx_sm100.cuh"
+#include "status_word.cuh"
 
 namespace fa8 {
 
@@ -210,11 +211,7 @@ __device__ __forceinline__ bool wait_bounded(const WaitCtx& w, uint32_t bar, uin
       if (*w.abort_flag) return false;
       if (global_timer_ns() - t0 > w.limit_ns) {
         *w.abort_flag = 1;
-        if (w.status) atomicCAS(w.status, 0, code);
-        if (w.host_status) {
-          *w.host_status = code;
-          __threadfence_system();
-        }
+        report_expired_wait(w.status, w.host_status, code);
         return false;
       }
     }
@@ -553,12 +550,12 @@ fa8_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     fence_mbar_init();
     fence_proxy_async_smem();
   } else if (threadIdx.x == 32) {
-    // A status word that is already non-zero (an earlier CTA of this launch gave up, or the
+    // An expired wait that is already in the status word (an earlier CTA of this launch gave up, or the
     // caller did not clear it) makes the CTA return at once: a failed launch then costs one
     // wait limit, not one per CTA.  skip_flag is written here only; abort_flag is what a
     // wait that gives up raises later.
     start_after_predecessor();
-    const bool stale = args.status != nullptr && *reinterpret_cast<volatile int*>(args.status) != 0;
+    const bool stale = wait_has_expired(args.status);
     *abort_flag = stale ? 2 : 0;
     *skip_flag = stale ? 1 : 0;
     // The skipped launch leaves O unwritten: the host must hear of it even if the word's first

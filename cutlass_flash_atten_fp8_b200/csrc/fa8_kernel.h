@@ -9,6 +9,9 @@
 
 namespace fa8 {
 
+// Code in the status words of an index out of range, which the kernels of the paged cache report; all others are of expired waits.
+constexpr int kBadIndex = 0xbad1;
+
 // By-value kernel arguments.  Plays the role of the reference's
 // Flash_fwd_params (csrc/flash.h:6-61) minus its dead fields; tensor addresses
 // and strides travel in the three TMA descriptors instead.
@@ -35,7 +38,7 @@ struct KernelArgs {
                                   // slice s has the scale descale_q[s * q_fold + r / (seqlen / q_fold)]
   float* lse;                     // optional [batch*heads, seqlen] fp32: log-sum-exp of the scaled scores
   float softmax_scale;            // as given by the caller (natural-log units, for lse)
-  int* status;                    // device word; non-zero after a bounded wait expired (later CTAs then return at once)
+  int* status;                    // device word; holds a code after a bounded wait expired (later CTAs then return at once)
   int* host_status;               // optional word in mapped host memory: receives the same code, so that
                                   // the host learns of it without a copy or a synchronisation
   unsigned long long timeout_ns;  // bound of every mbarrier wait
@@ -71,7 +74,7 @@ struct DecodeArgs {
   const float* descale_k;
   const float* descale_v;
   int descale_per_head;
-  int* status;                    // non-zero at launch: nothing is computed or written
+  int* status;                    // an expired wait at launch: nothing is computed or written
   int* host_status;
   // Filled in by launch_decode: blocks of rows a slice is cut into, CTAs (one cluster) its keys
   // are split over.

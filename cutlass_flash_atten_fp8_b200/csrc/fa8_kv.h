@@ -6,6 +6,8 @@
 
 #include <cstdint>
 
+#include "fa8_kernel.h"
+
 namespace fa8 {
 
 // By-value description of the cache and of the tokens a call is about (struct fa8_kv_cache).
@@ -29,9 +31,6 @@ struct KvArgs {
   int* status;                    // device word and mapped host word that an index out of range is reported into
   int* host_status;
 };
-
-// Code of an index out of range in the status words (codes of expired waits are others).
-constexpr int kBadIndex = 0xbad1;
 
 // Token-major tensors in and out: element strides.
 struct KvRows {

@@ -458,10 +458,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       if (!wait_copies(bars + 8 * stage, phase)) {
         // Give up: report, wait (with a limit each) for the copies in flight, which write to this CTA's memory, and go where the
         // others will be waiting.
-        if (lane == 0) {
-          if (a.c.status != nullptr) atomicCAS(a.c.status, 0, kExpiredWait);
-          if (a.c.host_status != nullptr) *reinterpret_cast<volatile int*>(a.c.host_status) = kExpiredWait;
-        }
+        if (lane == 0) report_expired_wait(a.c.status, a.c.host_status, kExpiredWait);
         for (int i = step; i < min(step + C::kStages, last); ++i) {
           wait_copies(bars + 8 * stage, phase);
           if (++stage == C::kStages) {

@@ -134,11 +134,7 @@ __device__ __forceinline__ bool wait_bounded(const Wait& w, uint64_t* barrier, u
       if (*w.abort) return false;
       if (global_timer_ns() - t0 > kLimitNs) {
         *w.abort = 1;
-        if (w.status) atomicCAS(w.status, 0, code);
-        if (w.host_status) {
-          *w.host_status = code;
-          __threadfence_system();
-        }
+        report_expired_wait(w.status, w.host_status, code);
         return false;
       }
     }
@@ -339,8 +335,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
   if (threadIdx.x == 0 && (base & 1023u) != 0u) {            // never seen; the tiles would be garbage, and it is reported
     sh.abort = 1;
-    if (wctx.status) atomicCAS(wctx.status, 0, 0xb000);
-    if (wctx.host_status) *wctx.host_status = 0xb000;
+    report_expired_wait(wctx.status, wctx.host_status, 0xb000);
   }
 
   // rows of 64 bytes lie two to a swizzled line of 128: the halves of every other four lines are exchanged
@@ -366,8 +361,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       // ---------------------------------------------------------------- producer
       uint32_t tiles = 0, blocks = 0;                              // raw tiles and blocks filled so far
       // once a wait has run out, the CTAs that are still to come have nothing to do
-      const int before = a.c.status ? *static_cast<volatile int*>(a.c.status) : 0;
-      bool ok = true, more = before == 0 || before == kBadIndex, asked = false;
+      bool ok = true, more = !wait_has_expired(a.c.status), asked = false;
       auto push = [&](const Item& it) {
         const int slot = n_items % kItemSlots;
         ok = wait_bounded(wctx, &sh.item_empty[slot], ((n_items / kItemSlots) & 1) ^ 1, 0xb200);

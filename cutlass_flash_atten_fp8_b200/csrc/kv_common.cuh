@@ -6,6 +6,7 @@
 
 #include "fa8_kv.h"
 #include "ptx_sm100.cuh"
+#include "status_word.cuh"
 
 namespace fa8 {
 

@@ -68,7 +68,9 @@ typedef struct fa8_fwd_params {
                           softmax_scale */
   int32_t* status_word; /* optional device int32, zero before the call; the kernel stores a
                            non-zero code there if one of its bounded waits runs out, and CTAs that
-                           find it non-zero return without writing O.  NULL = a word the library
+                           find it non-zero return without writing O (unless it holds what a call of
+                           fa8_kv_cache.h left there for an index out of range: that concerns the
+                           call in question alone).  NULL = a word the library
                            keeps per device.  Either way the failure also reaches the host through
                            a flag of the library's own, see fa8_fwd. */
   float* softmax_lse;   /* optional device fp32 [batch, heads, seqlen]: log(sum_j exp(softmax_scale *

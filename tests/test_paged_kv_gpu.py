@@ -11,8 +11,8 @@ import math
 import pytest
 import torch
 
-from cutlass_flash_atten_fp8_b200 import (PagedKVCache, _lib, api, check_status, flash_attention_paged_kv, paged_kv_append,
-                                          paged_kv_read)
+from cutlass_flash_atten_fp8_b200 import (PagedKVCache, _lib, api, check_status, flash_attention_paged_kv, flash_attention_v2_cutlass,
+                                          paged_kv_append, paged_kv_read)
 from oracle import paged_kv_oracle as po
 
 pytestmark = pytest.mark.gpu
@@ -416,6 +416,47 @@ def test_nan_in_queries(seqs, H, Hk, D):
     assert torch.equal(torch.isnan(got), ~held) and torch.equal(torch.isnan(lse.cpu()), torch.isnan(want_lse))
     limit = torch.finfo(half).eps / 2 * want.abs() + 1.25 * 2.0 ** -11 * A + 2.0 ** -25
     assert bool(((got - want).abs() <= limit)[held].all())
+
+
+@pytest.mark.parametrize("S,Sk", [(256, 256), (4, 1024)], ids=["forward", "few rows"])
+@pytest.mark.parametrize("op", ["append", "read", "attend"])
+def test_an_index_out_of_range_leaves_the_calls_behind_it_alone(S, Sk, op):
+    """A page out of range is left out of its own call and reported; a forward enqueued behind it, before anyone can know, is computed."""
+    D = 64
+    g = torch.Generator(device=DEV).manual_seed(100)
+    q8, k8, v8 = (torch.randn(1, 2, s, D, generator=g, device=DEV).to(E4M3) for s in (S, Sk, Sk))
+    want = flash_attention_v2_cutlass(q8, k8, v8, False, 0.125, v_layout="natural")[0]
+    cache = PagedKVCache.empty(4, 2, D, 16, device=DEV)
+    for t in cache:
+        t.zero_()
+    table, lens = torch.full((1, 2), 99, dtype=torch.int32, device=DEV), torch.tensor([3], dtype=torch.int32, device=DEV)
+    x, out = torch.zeros(3, 2, D, dtype=torch.float16, device=DEV), torch.full_like(want, 7.0)
+    call = {"append": lambda t: paged_kv_append(cache, x, x, t, lens), "read": lambda t: paged_kv_read(cache, t, lens, 3),
+            "attend": lambda t: flash_attention_paged_kv(x, cache, t, lens)}[op]
+    call(torch.zeros_like(table))                                 # what a first call sets up is there
+    check_status(DEV)
+    torch.cuda._sleep(200_000_000)                                # a tenth of a second: the calls below are enqueued before the first has run
+    call(table)
+    flash_attention_v2_cutlass(q8, k8, v8, False, 0.125, v_layout="natural", out=out)
+    with pytest.raises(RuntimeError, match="out of range"):
+        check_status(DEV)
+    assert torch.equal(bits(out), bits(want))
+    check_status(DEV)
+
+
+def test_an_expired_wait_behind_an_index_out_of_range_is_reported():
+    lib, word = _lib.load(), api.status_word(DEV)
+    cache = PagedKVCache.empty(4, 2, 64, 16, device=DEV)
+    table, lens = torch.full((1, 2), 99, dtype=torch.int32, device=DEV), torch.tensor([3], dtype=torch.int32, device=DEV)
+    x = torch.zeros(3, 2, 64, dtype=torch.float16, device=DEV)
+    paged_kv_append(cache, x, x, torch.zeros_like(table), lens)
+    check_status(DEV)
+    torch.cuda._sleep(200_000_000)
+    paged_kv_append(cache, x, x, table, lens)
+    assert lib.fa8_selftest_expired_wait(word.data_ptr(), 2000, torch.cuda.current_stream(DEV).cuda_stream) == _lib.FA8_OK
+    with pytest.raises(RuntimeError, match="bounded wait"):
+        check_status(DEV)
+    check_status(DEV)
 
 
 def test_page_table_of_wider_rows():
