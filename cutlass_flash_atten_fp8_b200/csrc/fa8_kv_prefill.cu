@@ -410,11 +410,12 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         auto load_scale = [&](const float* d, int page) { return in_pool(page) ? ld_global(d + static_cast<int64_t>(page) * a.c.heads + it.head) : 1.f; };
         int page = load_page(it.blk0), page1 = load_page(it.blk0 + 1);
         float kd = load_scale(a.c.k_descale, page), vd = load_scale(a.c.v_descale, page);
-        // the item's reference scales: its first page's, so that e5m2 (up to 2^15.8) keeps away from fp16's ends
+        // The item's reference scales: its first page's, or 1 where that is so far out that another page's, from 2^-64 to 2^64, might be
+        // infinite or nothing relative to it; times what keeps e5m2 (up to 2^15.8) away from fp16's ends.
         const float margin = kE5M2 ? 16.f : 1.f;
         auto reference = [&](float d) {
           d = __shfl_sync(0xffffffffu, d, 0);
-          return (d >= 0x1p-100f && d <= 0x1p100f ? d : 1.f) * margin;
+          return (d >= 0x1p-32f && d <= 0x1p32f ? d : 1.f) * margin;
         };
         const float kref = reference(kd), vref = reference(vd);
         for (int blk = it.blk0; blk < it.blk1 && ok; ++blk) {

@@ -459,6 +459,30 @@ def test_an_expired_wait_behind_an_index_out_of_range_is_reported():
     check_status(DEV)
 
 
+@pytest.mark.parametrize("seqs", [[(150, 500), (300, 300)]], ids=["prompts"])
+@pytest.mark.parametrize("of", ["K", "V", "K and V"])
+@pytest.mark.parametrize("H,Hk,D,fp8", [(4, 2, 64, E4M3), (4, 1, 128, E5M2), (2, 1, 256, E4M3), (4, 2, 96, E5M2)])
+def test_first_pages_of_zeros_before_pages_of_the_largest_scale(seqs, of, H, Hk, D, fp8):
+    """The scales that an append of zeros and of numbers past 2^70 leaves: 2^-64 on a sequence's first page, 2^64 on the others."""
+    P, half = 16, torch.bfloat16
+    cu, T, lens = ranges(seqs)
+    cache, table = filled(Hk, D, P, fp8, seqs, seed=94)
+    scale = 0.05
+    for name, x8, d in (("K", cache[0], cache[2]), ("V", cache[1], cache[3])):
+        if name in of:
+            d.fill_(2.0 ** 64)
+            for b, (_, s) in enumerate(seqs):
+                x8[table[b, 0], :, :s] = 0.0
+                d[table[b, 0]] = 2.0 ** -64
+    if "K" in of:
+        scale = 0.05 * 2.0 ** -70
+    q = rows(T, H, D, half, 95, False, cu, seqs)
+    where = to(DEV, table, lens, cu)
+    out, lse = flash_attention_paged_kv(q, to(DEV, *cache), where[0], where[1], True, scale, cu_seqlens=where[2], return_lse=True)
+    check_status(DEV)
+    check_attention(q, cache, table, lens, True, scale, cu, out, lse)
+
+
 def test_page_table_of_wider_rows():
     """A view of a table that has more columns: as many as the longest sequence of this call needs."""
     seqs, H, Hk, D, P = [(1, 50), (1, 90), (1, 33)], 4, 2, 64, 16
