@@ -46,7 +46,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr float kHeadroom = 6.f, kRaiseBy = 14.f;       // log2 of the largest P under a fresh reference, and at all
-constexpr float kLog2Least = -100.f;                   // log2 of the smallest scale of V that the reference m follows
+// log2 of the smallest scale of V that the reference m follows: exponentials reach 2^(kRaiseBy + 80), of which fp32 adds up 2^31
+constexpr float kLog2Least = -80.f;
 constexpr unsigned long long kLimitNs = 2000000000ull; // bound of every wait
 constexpr int kExpiredWait = 0xa77e;                   // code in the status words
 
@@ -129,8 +130,8 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
   constexpr int kWarps = C::kWarps, kStepKeys = C::kStepKeys, kHalves = C::kHalves;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_bar[kWarps * C::kStages];
-  // scales of K of the step's halves (-1: no page), log2 of those of V
-  __shared__ __align__(16) float s_scale[kWarps * C::kStages][4];
+  // scales of K of the step's halves (-1: no page), those of V, log2 of those
+  __shared__ __align__(16) float s_scale[kWarps * C::kStages][8];
   // the first unit of the item that a warp's last, and (where it had several) its first segment is of; -1: whole items only
   __shared__ int s_last[kWarps], s_head[kWarps];
   __shared__ bool s_single[kWarps], s_nan[kWarps];       // (s_nan: NaNs were taken out of the segment's V)
@@ -366,12 +367,12 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       }
       __syncwarp();
     };
-    // Lane l looks after the step's half l & 1: the scale of K (l & 2 = 0), -1 where there is no page, or log2 of that of V.
+    // Lane l looks after the step's half l & 1: the scale of K (l < 2), -1 where there is no page, that of V (l < 4), or its log2.
     auto put_scales = [&](int step, int st) {
       const int key = step * kStepKeys + (lane & (kHalves - 1)) * 16;
       const int src = ((key >> a.c.page_shift) - page0) & 31;
       const float kd = __shfl_sync(0xffffffffu, kd_of, src), vd = __shfl_sync(0xffffffffu, vd_of, src);
-      if (lane < 4) s_scale[warp * C::kStages + st][lane] = (lane & 2) ? fmaxf(__log2f(vd), kLog2Least) : (key < vis ? kd : -1.f);
+      if (lane < 6) s_scale[warp * C::kStages + st][lane] = lane < 2 ? (key < vis ? kd : -1.f) : (lane < 4 ? vd : fmaxf(__log2f(vd), kLog2Least));
     };
     // (Code that runs once a launch is kept short: its instructions have to be fetched past the pages that are being read.)
     {
@@ -471,7 +472,8 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       }
       const uint32_t sk = ring + stage * C::kStageBytes, sv = sk + C::kBlocks * C::kTile;
       const float4 scale = *reinterpret_cast<const float4*>(s_scale[warp * C::kStages + stage]);
-      const float kd[2] = {scale.x, scale.y}, lv[2] = {scale.z, scale.w};
+      const float2 logs = *reinterpret_cast<const float2*>(s_scale[warp * C::kStages + stage] + 4);
+      const float kd[2] = {scale.x, scale.y}, dv[2] = {scale.z, scale.w}, lv[2] = {logs.x, logs.y};
       // a step that holds keys past some row's last, or of a page that is out of range
       const int key0 = step * kStepKeys;
       const bool whole = key0 + kStepKeys <= least && kd[0] != -1.f && (kHalves == 1 || kd[1] != -1.f);
@@ -536,8 +538,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
           float mx = fmaxf(top[b], __shfl_xor_sync(0xffffffffu, top[b], 1));
           mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) - kHeadroom, m_row[b]);
           const float nm_new = mx == -INFINITY ? 0.f : -mx;
-          const float alpha = m_row[b] == -INFINITY ? 0.f : ex2_approx(nm_new - nm[b]);
-          l_row[b] *= alpha;
+          const float alpha = to_reference(m_row[b], -nm_new, l_row[b]);
           // rows 2t and 2t + 1 of the row block are the columns of O^T this thread holds
           const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
 #pragma unroll
@@ -549,19 +550,19 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
           nm[b] = nm_new;
         }
       }
-      // P_j = 2^(x_j - m + log2 dv), and 2^(x_j - m) = P_j / dv for the denominators
+      // 2^(x_j - m) for the denominators, P_j = 2^(x_j - m) dv.  (The first from the second, by 1 / dv, would be lost where dv is so small that P_j
+      // is nothing beside what other pages add to O.)
       uint32_t pb[RB][2 * kHalves];
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
 #pragma unroll
         for (int i = 0; i < kHalves; ++i) {
-          const float n = nm[b] + lv[i];
           float p[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = ex2_approx(fmaf(x[2 * i + e / 2][b][e & 1], c_of[b][i], n));
-          l_row[b] = fmaf((p[0] + p[1]) + (p[2] + p[3]), ex2_approx(-lv[i]), l_row[b]);
-          pb[b][2 * i] = pack_half2(p[0], p[1]);
-          pb[b][2 * i + 1] = pack_half2(p[2], p[3]);
+          for (int e = 0; e < 4; ++e) p[e] = ex2_approx(fmaf(x[2 * i + e / 2][b][e & 1], c_of[b][i], nm[b]));
+          l_row[b] += (p[0] + p[1]) + (p[2] + p[3]);
+          pb[b][2 * i] = pack_half2(p[0] * dv[i], p[1] * dv[i]);
+          pb[b][2 * i + 1] = pack_half2(p[2] * dv[i], p[3] * dv[i]);
         }
       }
       if (!whole && least < vis && key0 + kStepKeys > least) {      // only some rows see all these keys
@@ -742,10 +743,11 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
         if (!s_single[w]) continue;
         const float* p = part_of(w);
         const float mw = p[C::kRows * C::kORow + r];
-        const float f = mw == -INFINITY ? 0.f : ex2_approx(mw - m);
+        float lw = p[C::kRows * C::kORow + C::kRows + r];
+        const float f = to_reference(mw, m, lw);
         const float4 x = *reinterpret_cast<const float4*>(p + r * C::kORow + col);
         acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
-        l += p[C::kRows * C::kORow + C::kRows + r] * f;
+        l += lw;
       }
       *reinterpret_cast<float4*>(part_of(0) + r * C::kORow + col) = acc;
       if (col == 0) {
@@ -771,10 +773,11 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
           pm = cluster.map_shared_rank(pm, p);
           pl = cluster.map_shared_rank(pl, p);
         }
-        const float f = *pm == -INFINITY ? 0.f : ex2_approx(*pm - m);
+        float lp = *pl;
+        const float f = to_reference(*pm, m, lp);
         const float4 x = *reinterpret_cast<const float4*>(po);
         acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
-        l += *pl * f;
+        l += lp;
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int row = lone_row0 + r;
@@ -833,9 +836,9 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       m = fmaxf(m, mh);
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       auto add = [&](float mx, float lx, const float4& v) {
-        const float f = mx == -INFINITY ? 0.f : ex2_approx(mx - m);
+        const float f = to_reference(mx, m, lx);
         acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
-        l += lx * f;
+        l += lx;
       };
 #pragma unroll
       for (int x = 0; x < kWarps; ++x) {
@@ -898,21 +901,19 @@ __global__ void __launch_bounds__(32 * kCombineWarps) kv_combine_kernel(const Kv
         if (lane + 32 < quads) v[i][1] = ld_global(reinterpret_cast<const uint4*>(p + in * D) + lane + 32);
       }
     }
-    // (A reference of -inf is that of no keys, or of scores that are all NaN: its sums get the factor 0, which a NaN survives.)
     float top = m;
 #pragma unroll
     for (int i = 0; i < kAt; ++i) top = fmaxf(top, mp[i]);
-    const float back = m == -INFINITY ? 0.f : ex2_approx(m - top);
+    const float back = to_reference(m, top, l);
     m = top;
-    l *= back;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       acc[k].x *= back; acc[k].y *= back; acc[k].z *= back; acc[k].w *= back;
     }
 #pragma unroll
     for (int i = 0; i < kAt; ++i) {
-      const float f = mp[i] == -INFINITY ? 0.f : ex2_approx(mp[i] - m);
-      l += lp[i] * f;
+      const float f = to_reference(mp[i], m, lp[i]);
+      l += lp[i];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         acc[k].x += __uint_as_float(v[i][k].x) * f; acc[k].y += __uint_as_float(v[i][k].y) * f;

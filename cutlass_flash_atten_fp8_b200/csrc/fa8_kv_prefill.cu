@@ -43,7 +43,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr unsigned long long kLimitNs = 2000000000ull;
 constexpr float kRaiseAbove = 60000.f;   // below fp16's largest number
 constexpr float kHeadroom = 6.f;         // a fresh reference puts the row's largest P at 2^6: fp16 is exact to half a step down to 2^-14
-constexpr float kLog2Least = -100.f;
+constexpr float kLog2Least = -80.f;      // see fa8_kv_attend.cu
 constexpr int kItemSlots = 4;
 constexpr int kBlockSlots = 8;           // blocks whose residual scales are kept: the producer is at most four ahead of the softmax
 
@@ -863,11 +863,10 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           const float mine_top = top_of() - kHeadroom, top = over ? mine_top : -INFINITY;
           const float m = fmaxf(fmaxf(row.m, top), exchange(top));
           const float nm = m == -INFINITY ? 0.f : -m;
-          const float alpha = row.m == -INFINITY ? 0.f : ex2_approx(nm - row.nm);
+          const float alpha = to_reference(row.m, -nm, row.l);
           row.m = m;
           row.nm = nm;
           row.most = m == -INFINITY ? 0.f : kRaiseAbove;
-          row.l *= alpha;
           if (j > 0) {
             if (nt < C::kBufs) {
               const uint32_t b = turn_buffer<C::kBufs>(turns + (j - 1) * nt + tile);
@@ -1014,8 +1013,9 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a, cons
   for (int p = 0; p < parts; ++p) {
     const float* ml = plan.partial_ml + 2 * (p * rows + row);
     const float mp = ld_global(ml);
-    const float f = mp == -INFINITY ? 0.f : ex2_approx(mp - m);
-    l += ld_global(ml + 1) * f;
+    float lp = ld_global(ml + 1);
+    const float f = to_reference(mp, m, lp);
+    l += lp;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int q = lane + 32 * i;

@@ -141,6 +141,15 @@ __device__ __forceinline__ uint32_t fp8_pair(float lo, float hi) {
   return r;
 }
 
+// From reference m to reference m_new >= m: what sums of P are multiplied by, and a sum of denominators l.  References follow the scales of
+// V, which denominators know nothing of, so that the factor may be below fp32's range where l times it is not: l takes it in
+// halves.  A reference of -inf (no keys, or scores that are all NaN) leaves nothing but NaNs.
+__device__ __forceinline__ float to_reference(float m, float m_new, float& l) {
+  const float half = m == -INFINITY ? 0.f : ex2_approx(0.5f * (m - m_new));
+  l = l * half * half;
+  return half * half;
+}
+
 // A product adds 0 * V for keys that a row's mask leaves out, and a NaN there would stay one.  So where rows of a tile see different
 // keys, NaNs of V are taken out of the tile before the product, and the rows that do see them get theirs afterwards, in what was
 // stored for them (write_nans).

@@ -30,8 +30,8 @@ _HALF = {torch.float16: _lib.FA8_DTYPE_FP16, torch.bfloat16: _lib.FA8_DTYPE_BF16
 
 class PagedKVCache(NamedTuple):
     """The pool: k, v float8_e4m3fn or float8_e5m2 [num_pages, heads_kv, page_size, head_dim] (page_size 16, 32, 64 or
-    128; head_dim a multiple of 32 up to 256) and k_descale, v_descale float32 [num_pages, heads_kv], all contiguous on
-    one device.  The operators take any four tensors like these.  A page needs no initialisation: its first token
+    128; head_dim a multiple of 32 up to 256) and k_descale, v_descale float32 [num_pages, heads_kv], 0 or from 2^-64 to
+    2^64 where a token of the page is held, all contiguous on one device.  The operators take any four tensors like these.  A page needs no initialisation: its first token
     starts it anew."""
     k: torch.Tensor
     v: torch.Tensor

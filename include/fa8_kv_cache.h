@@ -11,8 +11,8 @@
  * The cache.  Keys and values of all sequences live in a pool of pages of `page_size` tokens:
  *   k, v                  fp8 [num_pages, heads_kv, page_size, head_dim], contiguous
  *   k_descale, v_descale  fp32 [num_pages, heads_kv]: a scale for each block of page_size tokens and
- *                         head, x = descale * x8; finite and not negative (as fa8_kv_append leaves
- *                         them) where a token of the page is held
+ *                         head, x = descale * x8; 0 or from 2^-64 to 2^64 (as fa8_kv_append leaves
+ *                         them; no powers of two are needed) where a token of the page is held
  * Sequence b has seqlens[b] tokens, those that the call is about included; its token p lies in slot
  * p % page_size of page page_table[b][p / page_size].  A call is about the last n_b tokens of each
  * sequence ("new" ones): rows cu_seqlens[b] .. cu_seqlens[b+1]-1 of the token-major tensors, or

@@ -459,7 +459,7 @@ def test_an_expired_wait_behind_an_index_out_of_range_is_reported():
     check_status(DEV)
 
 
-@pytest.mark.parametrize("seqs", [[(150, 500), (300, 300)]], ids=["prompts"])
+@pytest.mark.parametrize("seqs", [[(1, 300), (1, 90)], [(4, 300), (3, 3)], [(150, 500), (300, 300)]], ids=["tokens", "drafts", "prompts"])
 @pytest.mark.parametrize("of", ["K", "V", "K and V"])
 @pytest.mark.parametrize("H,Hk,D,fp8", [(4, 2, 64, E4M3), (4, 1, 128, E5M2), (2, 1, 256, E4M3), (4, 2, 96, E5M2)])
 def test_first_pages_of_zeros_before_pages_of_the_largest_scale(seqs, of, H, Hk, D, fp8):
@@ -481,6 +481,30 @@ def test_first_pages_of_zeros_before_pages_of_the_largest_scale(seqs, of, H, Hk,
     out, lse = flash_attention_paged_kv(q, to(DEV, *cache), where[0], where[1], True, scale, cu_seqlens=where[2], return_lse=True)
     check_status(DEV)
     check_attention(q, cache, table, lens, True, scale, cu, out, lse)
+
+
+@pytest.mark.parametrize("n,keys", [(1, 216), (4, 216), (150, 216), (1, 20000), (3, 9000), (150, 5000)])
+@pytest.mark.parametrize("least", [2.0 ** -64, 0.0])
+@pytest.mark.parametrize("H,Hk,D", [(1, 1, 64), (4, 1, 128), (16, 2, 256)])
+def test_values_of_the_smallest_scale_still_count_in_the_denominators(n, keys, least, H, Hk, D):
+    """Keys of a sequence with scores 6 below the other sixteen's, a third and more of the sum of exponentials, whose values are nothing beside
+    the others': scales of V of 2^-64 (or nothing) and 2^64."""
+    P, half = 16, torch.bfloat16
+    seqs = [(n, keys + (n - 1) // 16 * 16)]
+    cu, T, lens = ranges(seqs)
+    cache, table = filled(Hk, D, P, E4M3, seqs, seed=96)
+    cache[2].fill_(1.0)
+    cache[3].fill_(least)
+    cache[0].fill_(1.0)
+    cache[3][table[0, 2]] = 2.0 ** 64
+    cache[0][table[0, 2]] = 2.0
+    cache[1].copy_(cache[1].float().nan_to_num(0.0).to(E4M3))
+    q = rows(T, H, D, half, 97, False, cu, seqs).abs()
+    q = q / q.float().sum(-1, keepdim=True).to(half)              # rows add up to about 1
+    where = to(DEV, table, lens, cu)
+    out, lse = flash_attention_paged_kv(q, to(DEV, *cache), where[0], where[1], False, 6.0, cu_seqlens=where[2], return_lse=True)
+    check_status(DEV)
+    check_attention(q, cache, table, lens, False, 6.0, cu, out, lse)
 
 
 def test_page_table_of_wider_rows():
