@@ -99,9 +99,8 @@ struct Shared {
   uint64_t item_full[kItemSlots], item_empty[kItemSlots];
   uint64_t raw_full[C::kRaw], raw_empty[C::kRaw];
   uint64_t ring_full[C::kRing], ring_empty[C::kRing];
-  uint64_t s_full[C::kTiles][C::kBufs], p_full[C::kBufs];     // kv_turns.h
-  uint64_t q_full[2], o_final[2];        // by tile
-  uint64_t o_done[C::kTiles][C::kBufs];
+  uint64_t s_full[2][2], p_full[C::kBufs];       // by tile and turn, by buffer: kv_turns.h
+  uint64_t q_full[2], o_done[2], o_final[2];     // by tile
   uint64_t blk_full[kBlockSlots];
   uint64_t drain, given;
   uint4 answer;                          // to the request for another CTA's item
@@ -309,9 +308,9 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     init(sh.ring_full, C::kRing, 4);
     init(sh.ring_empty, C::kRing, 1);
     init(sh.q_full, 2, 8);
-    init(&sh.s_full[0][0], C::kTiles * C::kBufs, 1);
+    init(&sh.s_full[0][0], 4, 1);
     init(sh.p_full, C::kBufs, 8);
-    init(&sh.o_done[0][0], C::kTiles * C::kBufs, 1);
+    init(sh.o_done, 2, 1);
     init(sh.o_final, 2, 1);
     init(sh.blk_full, kBlockSlots, 1);
     init(&sh.drain, 1, 1);
@@ -540,6 +539,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         uint32_t ld = 0;                                           // widened tiles used so far: K, V, K, V ...
         uint32_t qn[2] = {0, 0};                                   // q_full phases by tile
         uint32_t turns = 0;                                        // of the score buffers, before this item
+        uint32_t scored = 0;                                       // bit i: parity of tile i's own turns whose scores have been issued
         auto ring_wait = [&](uint32_t i) { return wait_bounded(wctx, &sh.ring_full[i % C::kRing], (i / C::kRing) & 1, 0xb400); };
         auto ring_release = [&](uint32_t i) { tc_commit(smem_u32(&sh.ring_empty[i % C::kRing])); };
         auto issue_qk = [&](int tile, uint32_t b, uint32_t i) {
@@ -547,7 +547,8 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
 #pragma unroll
           for (int k = 0; k < W / 16; ++k)
             mma_f16_ss(tmem + C::kN * b, desc(qq + (k >> 2) * kColQ + 2 * (k & 3)), desc(kk + (k >> 2) * kColK + 2 * (k & 3)), kIdescQK, k > 0);
-          tc_commit(smem_u32(&sh.s_full[tile][b]));
+          tc_commit(smem_u32(&sh.s_full[tile][score_barrier(scored >> tile)]));
+          scored ^= 1u << tile;
         };
         auto issue_pv = [&](int tile, uint32_t b, uint32_t i, bool more) {
           const uint32_t vv = v_lo + (i % C::kRing) * (C::kRingBytes / 16);
@@ -561,9 +562,10 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           if (it.seq < 0) break;
           const int n = it.blk1 - it.blk0;
           const int nt = C::kTiles == 2 && it.n_tokens > tile_tokens ? 2 : 1;
-          // Turn t is block t / nt of tile t % nt; the scores run kBufs turns ahead: S(t + kBufs) goes into the buffer that P V (t) has read.
+          // Turn t is block t / nt of tile t % nt; the scores run `ahead` turns ahead, into a buffer that P V (t), or one before it, was the last to read.
+          const int ahead = turns_ahead<C::kBufs>(nt);
           int tile_v = 0, blk_v = 0, tile_k = 0, blk_k = 0;
-          for (int t = -C::kBufs; t < n * nt && ok; ++t) {
+          for (int t = -ahead; t < n * nt && ok; ++t) {
             if (t >= 0) {
               const uint32_t turn = turns + t, b = turn_buffer<C::kBufs>(turn), lv = ld + 2 * blk_v + 1;
               if (tile_v == 0) ok = ring_wait(lv);
@@ -571,7 +573,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
               if (!ok) break;
               tc_fence_after();
               issue_pv(tile_v, b, lv, blk_v > 0);
-              if (nt < C::kBufs) tc_commit(smem_u32(&sh.o_done[tile_v][b]));      // otherwise the tile's next scores come after it
+              tc_commit(smem_u32(&sh.o_done[tile_v]));
               if (blk_v + 1 == n) tc_commit(smem_u32(&sh.o_final[tile_v]));
               if (++tile_v == nt) {
                 ring_release(lv);
@@ -580,7 +582,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
               }
             }
             if (blk_k < n) {
-              const uint32_t b = turn_buffer<C::kBufs>(turns + t + C::kBufs), lk = ld + 2 * blk_k;
+              const uint32_t b = turn_buffer<C::kBufs>(turns + t + ahead), lk = ld + 2 * blk_k;
               if (blk_k == 0) ok = wait_bounded(wctx, &sh.q_full[tile_k], qn[tile_k]++ & 1, 0xb500 + tile_k);
               if (ok && tile_k == 0) ok = ring_wait(lk);
               if (!ok) break;
@@ -725,8 +727,8 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     };
     uint32_t blocks = 0;                                         // of all items (the residual ring), also those this tile sits out
     uint32_t turns = 0;                                          // of the score buffers, before this item
-    uint32_t seen = 0;                                           // of this tile's barriers (kv_turns.h)
-    constexpr uint32_t kDone = kSeenDone<C::kBufs>, kFinal = kSeenFinal<C::kBufs>;
+    uint32_t own = 0;                                            // of this tile's turns
+    uint32_t taken = 0;                                          // items this tile took part in
     Item it;
     bool ok = true;
     while (true) {
@@ -801,13 +803,12 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       row.lim = a.causal ? max(0, min(it.len, it.len - it.n + my_token + 1)) : it.len;
       const int least = a.causal ? max(0, min(it.len, it.len - it.n + tok0 + 1)) : it.len;       // of the tile's first row
       float vref = 1.f;
-      for (int j = 0; j < nb && ok; ++j) {
+      for (int j = 0; j < nb && ok; ++j, ++own) {
         const uint32_t buf = turn_buffer<C::kBufs>(turns + j * nt + tile);
         const uint32_t n = (blocks + j) % kBlockSlots;
         const uint32_t t_p = tmem + lanes + C::kN * buf, t_s = t_p + part * kMyKeys;
         ok = wait_bounded(wctx, &sh.blk_full[n], ((blocks + j) / kBlockSlots) & 1, 0xb900);
-        if (ok) ok = wait_bounded(wctx, &sh.s_full[tile][buf], seen_parity(seen, buf), 0xba00 + buf);
-        seen = seen_next(seen, buf);
+        if (ok) ok = wait_bounded(wctx, &sh.s_full[tile][score_barrier(own)], score_parity(own), 0xba00 + buf);
         __syncwarp();
         tc_fence_after();
         const int key0 = (it.blk0 + j) * C::kN, lim = row.lim - key0 - part * kMyKeys;
@@ -858,7 +859,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           }
           if (!any || raised) break;
           // Some row has outgrown its reference (or holds a NaN): take this block's maximum in and rescale O, for which the products
-          // before have to be done (they are, when this block's scores came after them).
+          // before have to be done.
           raised = true;
           const float mine_top = top_of() - kHeadroom, top = over ? mine_top : -INFINITY;
           const float m = fmaxf(fmaxf(row.m, top), exchange(top));
@@ -868,10 +869,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           row.nm = nm;
           row.most = m == -INFINITY ? 0.f : kRaiseAbove;
           if (j > 0) {
-            if (nt < C::kBufs) {
-              const uint32_t b = turn_buffer<C::kBufs>(turns + (j - 1) * nt + tile);
-              ok = wait_bounded(wctx, &sh.o_done[tile][b], seen_parity(seen, kDone + b) ^ 1u, 0xbb00 + tile) && ok;
-            }
+            ok = wait_bounded(wctx, &sh.o_done[tile], done_parity(own), 0xbb00 + tile) && ok;
             __syncwarp();
             tc_fence_after();
             rescale(t_o, kMyCols, alpha);
@@ -885,7 +883,6 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[buf]));
-        if (nt < C::kBufs) seen = seen_next(seen, kDone + buf);
       }
       blocks += nb;
       turns += nb * nt;
@@ -894,9 +891,9 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       // ---- O ----
       const bool whole = it.part < 0;
       row.l += exchange(row.l);
-      ok = !pair_any(!wait_bounded(wctx, &sh.o_final[tile], seen_parity(seen, kFinal), 0xbc00 + tile));
+      ok = !pair_any(!wait_bounded(wctx, &sh.o_final[tile], taken & 1, 0xbc00 + tile));
       if (!ok) break;
-      seen = seen_next(seen, kFinal);
+      ++taken;
       tc_fence_after();
       const float inv = (row.l == 0.f ? 0.f : (whole ? 1.f / row.l : 1.f)) * vref;
       const int token = (r * over_group) >> 16;

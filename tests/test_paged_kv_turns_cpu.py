@@ -9,7 +9,7 @@ import pytest
 
 from cutlass_flash_atten_fp8_b200.build import CSRC
 
-# The issuer: kBufs scores ahead, then P V of a turn and the scores that go into its buffer.  The tensor core completes what was issued in
+# The issuer: scores so many turns ahead, then P V of a turn and the next scores.  The tensor core completes what was issued in
 # order.  Two warps a tile, each for itself: an item is there for the next read once all have read the one before.
 MODEL = r"""
 #include <cstdint>
@@ -18,61 +18,64 @@ MODEL = r"""
 #include <vector>
 #include "kv_turns.h"
 struct Item { int blocks, tiles; };
-struct Op { bool pv; int turn, tile; bool done, last; };      // done, last: with a phase of o_done, of o_final
+struct Op { bool pv; int turn, tile; bool last; };            // last: with a phase of o_final
 enum Kind { kRead, kQ, kScores, kProbs, kFinal, kIssue, kAskProbs, kAskQ };
-struct Event { Kind kind; int at, before; bool ask_done; uint32_t seen, dones; };   // at: item, turn or op; before: the tile's turn before it in the item, or -1; dones: o_done's before that one
+struct Event { Kind kind; int at, before; uint32_t k; };      // at: item, turn or op; before: the tile's turn before it in the item, or -1; k: own turn, item
 static bool passes(uint32_t completed, uint32_t parity) { return ((completed & 1u) ^ 1u) == parity; }
 
-template <int kTiles, int kBufs>
+// kAhead 0: as the kernel has it
+template <int kTiles, int kBufs, int kAhead = 0>
 struct Model {
   std::vector<Op> ops;
   std::vector<int> tile_of, s_op, pv_op;                      // of turns
+  std::vector<uint32_t> own_of;
   std::vector<Event> issuer, warp[2];
-  long wrong = 0, wrong_shared = 0, wrong_done = 0;            // with one barrier a buffer for the scores, one a tile for the products
+  long wrong = 0, wrong_shared = 0;                           // wrong_shared: with one barrier a buffer for the scores of both tiles
 
   explicit Model(const std::vector<Item>& items) {
     int turns = 0, asked[2] = {0, 0};
-    uint32_t dones[2] = {0, 0};
-    uint32_t seen[2] = {0, 0};
+    uint32_t own[2] = {0, 0}, taken[2] = {0, 0};
     for (int i = 0; i < static_cast<int>(items.size()); ++i) {
       const int n = items[i].blocks, nt = items[i].tiles;
-      for (int t = 0; t < n * nt; ++t) tile_of.push_back(t % nt);
+      const int ahead = kAhead > 0 ? kAhead : fa8::turns_ahead<kBufs>(nt);
+      for (int t = 0; t < n * nt; ++t) {
+        tile_of.push_back(t % nt);
+        own_of.push_back(own[t % nt] + t / nt);
+      }
       s_op.resize(turns + n * nt);
       pv_op.resize(turns + n * nt);
-      issuer.push_back({kRead, i, 0, false, 0, 0});
-      for (int t = -kBufs; t < n * nt; ++t) {
+      issuer.push_back({kRead, i, 0, 0});
+      for (int t = -ahead; t < n * nt; ++t) {
         if (t >= 0) {
-          issuer.push_back({kAskProbs, turns + t, 0, false, 0, 0});
-          issuer.push_back({kIssue, static_cast<int>(ops.size()), 0, false, 0, 0});
+          issuer.push_back({kAskProbs, turns + t, 0, 0});
+          issuer.push_back({kIssue, static_cast<int>(ops.size()), 0, 0});
           pv_op[turns + t] = static_cast<int>(ops.size());
-          ops.push_back({true, turns + t, t % nt, nt < kBufs, t / nt + 1 == n});
+          ops.push_back({true, turns + t, t % nt, t / nt + 1 == n});
         }
-        const int s = t + kBufs;
+        const int s = t + ahead;
         if (s < n * nt) {
-          if (s < nt) issuer.push_back({kAskQ, s, asked[s]++, false, 0, 0});
-          issuer.push_back({kIssue, static_cast<int>(ops.size()), 0, false, 0, 0});
+          if (s < nt) issuer.push_back({kAskQ, s, asked[s]++, 0});
+          issuer.push_back({kIssue, static_cast<int>(ops.size()), 0, 0});
           s_op[turns + s] = static_cast<int>(ops.size());
-          ops.push_back({false, turns + s, s % nt, false, false});
+          ops.push_back({false, turns + s, s % nt, false});
         }
       }
       for (int tile = 0; tile < kTiles; ++tile) {
         auto& w = warp[tile];
-        w.push_back({kRead, i, 0, false, 0, 0});
+        w.push_back({kRead, i, 0, 0});
         if (tile >= nt) continue;                             // sits the item out
-        w.push_back({kQ, i, 0, false, 0, 0});
+        w.push_back({kQ, i, 0, 0});
         for (int j = 0; j < n; ++j) {
           const int turn = turns + j * nt + tile;
-          w.push_back({kScores, turn, 0, false, seen[tile], 0});
-          seen[tile] = fa8::seen_next(seen[tile], fa8::turn_buffer<kBufs>(turn));
-          w.push_back({kProbs, turn, j > 0 ? turn - nt : -1, j > 0 && nt < kBufs, seen[tile], dones[tile] - 1});
-          dones[tile] += nt < kBufs;
-          if (nt < kBufs) seen[tile] = fa8::seen_next(seen[tile], fa8::kSeenDone<kBufs> + fa8::turn_buffer<kBufs>(turn));
+          w.push_back({kScores, turn, 0, own[tile]});
+          w.push_back({kProbs, turn, j > 0 ? turn - nt : -1, own[tile]++});
         }
-        w.push_back({kFinal, turns + (n - 1) * nt + tile, 0, false, seen[tile], 0});
-        seen[tile] = fa8::seen_next(seen[tile], fa8::kSeenFinal<kBufs>);
+        w.push_back({kFinal, turns + (n - 1) * nt + tile, 0, taken[tile]++});
       }
       turns += n * nt;
     }
+    // scores go into a buffer after the last product that reads it
+    for (int t = kBufs; t < turns; ++t) wrong += !(pv_op[t - kBufs] < s_op[t]);
   }
 
   struct State { int issuer, done, at[2][2]; };               // places in the lists; operations complete
@@ -123,28 +126,20 @@ struct Model {
     switch (e.kind) {
       case kRead: return item_there(s, e.at);
       case kScores: {
-        const uint32_t b = fa8::turn_buffer<kBufs>(e.at);
         const bool have = s_op[e.at] < s.done;
-        auto in_b = [&](const Op& o) { return !o.pv && fa8::turn_buffer<kBufs>(o.turn) == b; };
-        wrong += passes(completed([&](const Op& o) { return in_b(o) && o.tile == tile; }), fa8::seen_parity(e.seen, b)) != have;
-        wrong_shared += passes(completed(in_b), fa8::turn_parity<kBufs>(e.at)) != have;
+        auto mine = [&](const Op& o) { return !o.pv && o.tile == tile && fa8::score_barrier(own_of[o.turn]) == fa8::score_barrier(e.k); };
+        wrong += passes(completed(mine), fa8::score_parity(e.k)) != have;
+        auto in_buffer = [&](const Op& o) { return !o.pv && fa8::turn_buffer<kBufs>(o.turn) == fa8::turn_buffer<kBufs>(e.at); };
+        wrong_shared += passes(completed(in_buffer), fa8::turn_parity<kBufs>(e.at)) != have;
         return have;
       }
       case kProbs:
-        if (e.ask_done) {
-          const bool have = pv_op[e.before] < s.done;
-          const uint32_t b = fa8::turn_buffer<kBufs>(e.before);
-          auto of_tile = [&](const Op& o) { return o.done && o.tile == tile; };
-          wrong += passes(completed([&](const Op& o) { return of_tile(o) && fa8::turn_buffer<kBufs>(o.turn) == b; }),
-                          fa8::seen_parity(e.seen, fa8::kSeenDone<kBufs> + b) ^ 1u) != have;
-          wrong_done += passes(completed(of_tile), e.dones & 1u) != have;
-        }
-        // otherwise the product before it came before these scores
-        else if (e.before >= 0) wrong += !(pv_op[e.before] < s.done);
+        if (e.before >= 0)
+          wrong += passes(completed([&](const Op& o) { return o.pv && o.tile == tile; }), fa8::done_parity(e.k)) != (pv_op[e.before] < s.done);
         return true;
       case kFinal: {
         const bool have = pv_op[e.at] < s.done;
-        wrong += passes(completed([&](const Op& o) { return o.last && o.tile == tile; }), fa8::seen_parity(e.seen, fa8::kSeenFinal<kBufs>)) != have;
+        wrong += passes(completed([&](const Op& o) { return o.last && o.tile == tile; }), e.k & 1u) != have;
         return have;
       }
       default: return true;
@@ -200,9 +195,9 @@ struct Model {
   }
 };
 
-template <int kTiles, int kBufs>
+template <int kTiles, int kBufs, int kAhead = 0>
 void all() {
-  long wrong = 0, shared_two = 0, shared_mixed = 0, done = 0, stuck = 0, runs = 0;
+  long wrong = 0, shared_two = 0, shared_mixed = 0, stuck = 0, runs = 0;
   std::vector<std::vector<Item>> lists;
   for (int a = 1; a <= 3; ++a)
     for (int at = 1; at <= kTiles; ++at)
@@ -213,21 +208,21 @@ void all() {
             for (int ct = 1; ct <= kTiles; ++ct) lists.push_back({{a, at}, {b, bt}, {2, ct}});
         }
   for (const auto& items : lists) {
-    Model<kTiles, kBufs> m(items);
+    Model<kTiles, kBufs, kAhead> m(items);
     stuck += !m.run();
     bool mixed = false;
     for (const Item& i : items) mixed = mixed || i.tiles < kTiles;
     wrong += m.wrong;
     (mixed ? shared_mixed : shared_two) += m.wrong_shared;
-    done += m.wrong_done;
     ++runs;
   }
-  std::printf("%ld %ld %ld %ld %ld %ld\n", runs, wrong, stuck, shared_two, shared_mixed, done);
+  std::printf("%ld %ld %ld %ld %ld\n", runs, wrong, stuck, shared_two, shared_mixed);
 }
 int main() {
   all<2, 2>();
   all<2, 3>();
   all<1, 2>();
+  all<2, 3, 3>();
   return 0;
 }
 """
@@ -241,20 +236,20 @@ def test_waits_pass_exactly_when_they_should(tmp_path):
     src.write_text(MODEL)
     subprocess.run([cxx, "-std=c++17", "-O2", "-I" + CSRC, str(src), "-o", exe], check=True)
     out = subprocess.run([exe], check=True, capture_output=True, text=True).stdout
-    for line, tiles, buffers in zip(out.splitlines(), (2, 2, 1), (2, 3, 2)):
-        runs, wrong, stuck, shared_two, shared_mixed, done = map(int, line.split())
+    *kernel, far = (tuple(map(int, line.split())) for line in out.splitlines())
+    for (runs, wrong, stuck, shared_two, shared_mixed), tiles in zip(kernel, (2, 2, 1)):
         assert runs > 10 and wrong == 0 and stuck == 0
         # a barrier per buffer for both tiles would do only while no tile sits an item out
         assert shared_two == 0 and (shared_mixed > 0) == (tiles == 2)
-        # one for all products of a tile while two buffers are all there are
-        assert (done > 0) == (buffers == 3)
+    # scores three turns ahead, also of one tile, would be too many for these barriers
+    assert far[1] > 0
+
 
 
 def test_the_kernel_uses_these_rules():
     with open(os.path.join(CSRC, "fa8_kv_prefill.cu")) as f:
         text = f.read()
-    for part in ("turn_buffer<C::kBufs>(turns + j * nt + tile)", "&sh.s_full[tile][buf], seen_parity(seen, buf)", "seen = seen_next(seen, buf)",
-                 "tc_commit(smem_u32(&sh.s_full[tile][b]))", "&sh.p_full[b], turn_parity<C::kBufs>(turn)",
-                 "&sh.o_done[tile][b], seen_parity(seen, kDone + b) ^ 1u", "if (nt < C::kBufs) seen = seen_next(seen, kDone + buf)",
-                 "&sh.o_final[tile], seen_parity(seen, kFinal)", "seen = seen_next(seen, kFinal)"):
+    for part in ("ahead = turns_ahead<C::kBufs>(nt)", "turn_buffer<C::kBufs>(turns + t + ahead)", "turn_buffer<C::kBufs>(turns + j * nt + tile)",
+                 "&sh.s_full[tile][score_barrier(own)], score_parity(own)", "tc_commit(smem_u32(&sh.s_full[tile][score_barrier(scored >> tile)]))",
+                 "&sh.p_full[b], turn_parity<C::kBufs>(turn)", "&sh.o_done[tile], done_parity(own)", "&sh.o_final[tile], taken & 1"):
         assert part in text, part
