@@ -122,6 +122,12 @@ struct Wait {
   int* status;
   volatile int* host_status;
 };
+// (Not in line: there are two dozen waits, and the two status words would be held in registers for them.  In line, four prompts of 4096
+// at head dim 128 took 478 us and 1024 tokens over 16384 keys 327; so they take 452 and 323.)
+__device__ __noinline__ void give_up(const Wait& w, int code) {
+  *w.abort = 1;
+  report_expired_wait(w.status, w.host_status, code);
+}
 __device__ __forceinline__ bool wait_bounded(const Wait& w, uint64_t* barrier, uint32_t parity, int code) {
   const uint32_t bar = smem_u32(barrier);
   if (mbar_try_wait(bar, parity)) return true;
@@ -132,8 +138,7 @@ __device__ __forceinline__ bool wait_bounded(const Wait& w, uint64_t* barrier, u
     if ((++spins & 31u) == 0) {
       if (*w.abort) return false;
       if (global_timer_ns() - t0 > kLimitNs) {
-        *w.abort = 1;
-        report_expired_wait(w.status, w.host_status, code);
+        give_up(w, code);
         return false;
       }
     }
