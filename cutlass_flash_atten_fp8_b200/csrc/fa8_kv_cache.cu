@@ -128,10 +128,22 @@ __device__ __forceinline__ uint2 to_fp8x8(const uint4& x, float inv) {
   return make_uint2(fp8_pair<kE5M2>(a.x * inv, a.y * inv) | (fp8_pair<kE5M2>(b.x * inv, b.y * inv) << 16),
                     fp8_pair<kE5M2>(c.x * inv, c.y * inv) | (fp8_pair<kE5M2>(d.x * inv, d.y * inv) << 16));
 }
+// x / d to fp32's precision, for any d: 1 / d is taken as hi + lo, lo from the remainder 1 - d hi (0 for powers of two), and x hi with its rounding
+// error; both are exact by a fused multiplication.
+__device__ __forceinline__ float quotient(float x, float hi, float lo) {
+  const float p = x * hi;
+  return fabsf(p) < INFINITY ? p + fmaf(x, lo, fmaf(x, hi, -p)) : p;
+}
+template <bool kBf16, bool kE5M2>
+__device__ __forceinline__ uint32_t divided_to_fp8x4(uint32_t x, uint32_t y, float hi, float lo) {
+  const float2 a = half_pair<kBf16>(x), b = half_pair<kBf16>(y);
+  return fp8_pair<kE5M2>(quotient(a.x, hi, lo), quotient(a.y, hi, lo)) | (fp8_pair<kE5M2>(quotient(b.x, hi, lo), quotient(b.y, hi, lo)) << 16);
+}
 
-// kWarp: a unit to a warp, several a CTA; otherwise a unit to a CTA.
+// kWarp: a unit to a warp, several a CTA; otherwise a unit to a CTA, of which two of 512 threads are to fit an SM (64 registers; with the 76
+// that the compiler would take, 16 x 2000 tokens at head dim 256 took 116 us for 80).
 template <bool kBf16, bool kE5M2, bool kWarp, int kHold>
-__global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_append_kernel(const KvArgs a, const KvRows kin, const KvRows vin,
+__global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads, kWarp ? 0 : 2) kv_append_kernel(const KvArgs a, const KvRows kin, const KvRows vin,
                                                                                             int64_t units, uint32_t magic) {
   __shared__ float part[kMaxThreads / 32];
   start_after_predecessor();
@@ -195,14 +207,21 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : kMaxThreads) kv_ap
     }
   }
   if (tid == 0) *descale = d;                             // every thread has read the old one: the reduction lies between
-  const float inv = 1.f / d;
   uint2* const dst = reinterpret_cast<uint2*>(y + w.off * D);
+  // Scales of pages that were filled in another way need not be powers of two, and x (1 / d) rounds twice: such pages' rows are read again.
+  const float inv = 1.f / d;
+  const bool exact = (__float_as_uint(d) & 0x7fffffu) == 0u;
+  const int n_held = exact ? n : 0;
 #pragma unroll
   for (int h = 0; h < kHold; ++h) {
     const int i = tid + h * n_threads;
-    if (i < n) dst[i] = to_fp8x8<kBf16, kE5M2>(hold[h], inv);
+    if (i < n_held) dst[i] = to_fp8x8<kBf16, kE5M2>(hold[h], inv);
   }
-  for (int i = tid + kHold * n_threads; i < n; i += n_threads) dst[i] = to_fp8x8<kBf16, kE5M2>(ld_global(src(i)), inv);
+  const float lo = exact ? 0.f : fmaf(-d, inv, 1.f) * inv;
+  for (int i = tid + (exact ? kHold * n_threads : 0); i < n; i += n_threads) {
+    const uint4 v = ld_global(src(i));
+    dst[i] = make_uint2(divided_to_fp8x4<kBf16, kE5M2>(v.x, v.y, inv, lo), divided_to_fp8x4<kBf16, kE5M2>(v.z, v.w, inv, lo));
+  }
 }
 
 template <bool kBf16, bool kE5M2, bool kWarp, int kHold>

@@ -507,6 +507,30 @@ def test_values_of_the_smallest_scale_still_count_in_the_denominators(n, keys, l
     check_attention(q, cache, table, lens, False, 6.0, cu, out, lse)
 
 
+@pytest.mark.parametrize("n", [1, 5, 90])
+@pytest.mark.parametrize("half,fp8", [(torch.float16, E4M3), (torch.bfloat16, E5M2), (torch.float16, E5M2)])
+@pytest.mark.parametrize("D", [64, 256])
+def test_append_to_pages_whose_scale_is_no_power_of_two(n, half, fp8, D):
+    """Such a scale is kept where the new tokens fit it.  New values are odd numbers of half fp8 steps times 63 2^-7: they lie
+    half-way between two fp8 numbers when divided by the scale, but not when multiplied by its rounded reciprocal."""
+    Hk, P = 2, 128
+    seqs = [(n, 20 + n), (n, 7 + n)]
+    cu, T, lens = ranges(seqs)
+    cache, table = filled(Hk, D, P, fp8, seqs, seed=98)
+    for d in cache[2:]:
+        d.fill_(63 * 2.0 ** -7)
+    g = torch.Generator().manual_seed(99)
+    mid = 2.0 * torch.randint(8, 16, (T, Hk, D), generator=g) + 1 if fp8 == E4M3 else 2.0 * torch.randint(4, 8, (T, Hk, D), generator=g) + 1
+    x = (mid * 63 * 2.0 ** -7).to(half)
+    exact = x.double() == mid.double() * 63 * 2.0 ** -7
+    assert bool(exact.all()) or half is torch.bfloat16
+    dev, where = PagedKVCache(*to(DEV, *cache)), to(DEV, table, lens)
+    paged_kv_append(dev, x.to(DEV), -x.to(DEV), *where)
+    check_status(DEV)
+    for w, got in zip(po.append(cache, x, -x, table, lens), dev):
+        assert torch.equal(w.float().nan_to_num(-1.0), got.cpu().float().nan_to_num(-1.0))
+
+
 def test_page_table_of_wider_rows():
     """A view of a table that has more columns: as many as the longest sequence of this call needs."""
     seqs, H, Hk, D, P = [(1, 50), (1, 90), (1, 33)], 4, 2, 64, 16
