@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
   __shared__ __align__(16) float s_scale[kWarps * C::kStages][8];
   // the first unit of the item that a warp's last, and (where it had several) its first segment is of; -1: whole items only
   __shared__ int s_last[kWarps], s_head[kWarps];
-  __shared__ bool s_single[kWarps], s_nan[kWarps];       // (s_nan: NaNs were taken out of the segment's V)
+  __shared__ bool s_single[kWarps], s_special[kWarps];       // (s_special: NaNs or infinities were taken out of the segment's V)
   __shared__ Segment s_item[kLone ? 1 : kWarps];
   __shared__ float s_m[C::kRows], s_l[C::kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
   // partial sums of warp w: [row][column], then the rows' references and sums
   auto part_of = [&](int w) { return reinterpret_cast<float*>(smem_raw + (ring0 - smem_u32(smem_raw)) + w * C::kRingBytes); };
   if (lane == 0) {
-    s_nan[warp] = false;
+    s_special[warp] = false;
     for (int i = 0; i < C::kStages; ++i) mbar_init(bars + 8 * i, 1);
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -571,8 +571,8 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
           const int row = W == 64 ? ((16 * i) ^ ((i & 32) ? flip : 0u)) >> 6 : (i >> 3) % kStepKeys;
           if (key0 + row >= vis || (kHalves > 1 && row >= 16 ? kd[1] : kd[0]) == -1.f) continue;
           uint4 v = ld_shared16(sv + 16 * i);
-          if (drop_nans<kE5M2>(v)) {
-            s_nan[warp] = true;
+          if (drop_specials<kE5M2>(v)) {
+            s_special[warp] = true;
             st_shared_v4(sv + 16 * i, v.x, v.y, v.z, v.w);
             fence_proxy_async_smem();                     // before the next copy to this place
           }
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
             const uint4 v = ld_shared16(sv + blk * C::kTile + row * 128 + ((g ^ (row & 7)) << 4));
             vr[i][0] = v.x; vr[i][1] = v.y; vr[i][C::kVWords - 2] = v.z; vr[i][C::kVWords - 1] = v.w;
           }
-          // nothing of keys that do not count, not even a NaN times zero
+          // nothing of keys that do not count, not even a NaN or an infinity times zero
           if (!whole && (key0 + row >= vis || kd[i >> 2] == -1.f)) {
 #pragma unroll
             for (int w = 0; w < C::kVWords; ++w) vr[i][w] = 0u;
@@ -708,18 +708,18 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       }
     }
     __syncwarp();
-    if (s_nan[warp]) {
+    if (s_special[warp]) {
 #pragma unroll 1
       for (int in = 0; in < n_rows; ++in) {
         const int r = row0 + in;
         uint16_t* const po = static_cast<uint16_t*>(a.o) + (static_cast<int64_t>(s.first + r / a.group) * a.heads_q + h * a.group + r % a.group) * D;
-        write_nans<kE5M2>(a.c, seq, h, max(least / kStepKeys, step0) * kStepKeys, min(seen(r), last * kStepKeys), lane, D, [&](int col) {
-          if (alone) po[col] = 0x7fff;                     // a NaN in either type
-          else part[in * part_row + col] = NAN;
+        write_specials<kE5M2>(a.c, seq, h, max(least / kStepKeys, step0) * kStepKeys, min(seen(r), last * kStepKeys), lane, D, [&](int col, float sum) {
+          if (alone) po[col] = with_special(po[col], sum, a.bf16);
+          else part[in * part_row + col] += sum;
         });
       }
       __syncwarp();
-      s_nan[warp] = false;
+      s_special[warp] = false;
       __syncwarp();
     }
     if (!more) break;

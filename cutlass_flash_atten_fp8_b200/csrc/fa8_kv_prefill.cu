@@ -8,7 +8,7 @@
 // A CTA per SM, warps with roles, work items of two tiles (one at head dims above 128) of one sequence and K/V head:
 //   producer   looks up items and pages, copies K and V tiles of kN keys from the pages (fp8) into shared memory
 //   widening   four warps turn a tile into fp16, in the layout that the products want, times the power of two by which its pages' scales
-//              differ from the item's first page; keys past the last one become zeros (a NaN there must not meet a zero P).  Eight warps
+//              differ from the item's first page; keys past the last one become zeros (a NaN or an infinity there must not meet a zero P).  Eight warps
 //              were no faster (330 us for 1024 tokens over 16384 keys, four 322)
 //   issuer     one thread: S = Q K^T into tensor memory, O += P V with P from tensor memory
 //   softmax    eight warps a tile, two to 32 rows (four, a row to a thread, took 26 % longer): each has half of a block's keys, P = 2^(c s - m) over
@@ -105,7 +105,7 @@ struct Shared {
   uint64_t drain, given;
   uint4 answer;                          // to the request for another CTA's item
   Item item[kItemSlots];                 // seq < 0: no more
-  int with_nan[kItemSlots];              // NaNs of V of keys that only some of the item's rows see were taken out (see drop_nans)
+  int with_special_v[kItemSlots];        // NaNs or infinities of V of keys that only some of the item's rows see were taken out (drop_specials)
   uint32_t factor[C::kRaw][C::kGroups];  // fp16 pair to multiply a group of 16 keys by
   int valid[C::kRaw];                    // rows of the tile that are keys
   int complete[C::kRaw];                 // all are, and of pages that exist
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
     it = sh.item[slot];
     return true;
   };
-  // From the block of this key on NaNs of V are left to the end: the item's rows do not all see its keys.
+  // From the block of this key on NaNs and infinities of V are left to the end: the item's rows do not all see its keys.
   auto apart = [&](const Item& i) { return a.causal ? max(0, min(i.len, i.len - i.n + i.token0 + 1)) / C::kN : 0x7fffffff; };
   auto item_read = [&] { mbar_arrive(smem_u32(&sh.item_empty[n_items++ % kItemSlots])); };
 
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
         if (!ok) return;
         if (lane == 0) {
           sh.item[slot] = it;
-          sh.with_nan[slot] = 0;
+          sh.with_special_v[slot] = 0;
           mbar_arrive(smem_u32(&sh.item_full[slot]));
         }
         ++n_items;
@@ -652,9 +652,9 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           for (int p = w; p < kParts; p += 4) {
             if (sh.factor[st][p / C::kCols / 2] == 0u || (p / C::kCols) * 8 + r8 >= valid) continue;
             uint4 x = ld_shared16(from(p));
-            if (drop_nans<kE5M2>(x)) {
+            if (drop_specials<kE5M2>(x)) {
               st_shared16(from(p), x);
-              sh.with_nan[(n_items - 1) % kItemSlots] = 1;
+              sh.with_special_v[(n_items - 1) % kItemSlots] = 1;
             }
           }
           __syncwarp();
@@ -962,7 +962,7 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
       }
       pair_sync();                                               // both warps are through with these rows of Q's memory
       const int slot = (n_items - 1) % kItemSlots;               // still this item's: no more than one other waits
-      if (*static_cast<volatile int*>(&sh.with_nan[slot]) != 0) {
+      if (*static_cast<volatile int*>(&sh.with_special_v[slot]) != 0) {
         const Item i = sh.item[slot];
         const int token0 = i.token0 + tile * tile_tokens, rows = min(tile_tokens, i.n_tokens - tile * tile_tokens) * group;
 #pragma unroll 1
@@ -970,10 +970,14 @@ __global__ void __launch_bounds__(PCfg<W>::kThreads, 1) kv_prefill_kernel(const 
           const int t = (q * over_group) >> 16;
           const int64_t to = ((static_cast<int64_t>(i.first) + token0 + t) * a.heads_q + i.head * group + (q - t * group)) * a.c.head_dim;
           float* const partial = plan.partial_o + static_cast<int64_t>(i.part) * a.c.tokens * a.heads_q * a.c.head_dim;
-          write_nans<kE5M2>(a.c, i.seq, i.head, max(apart(i), i.blk0) * C::kN, min(i.len - i.n + token0 + t + 1, i.blk1 * C::kN),
-                            part * kMyCols + lane, min(a.c.head_dim, (part + 1) * kMyCols), [&](int col) {
-            if (i.part < 0) static_cast<uint16_t*>(a.o)[to + col] = 0x7fff;       // a NaN in either type
-            else partial[to + col] = NAN;
+          write_specials<kE5M2>(a.c, i.seq, i.head, max(apart(i), i.blk0) * C::kN, min(i.len - i.n + token0 + t + 1, i.blk1 * C::kN),
+                            part * kMyCols + lane, min(a.c.head_dim, (part + 1) * kMyCols), [&](int col, float sum) {
+            if (i.part < 0) {
+              uint16_t* const p = static_cast<uint16_t*>(a.o) + to + col;
+              *p = with_special(*p, sum, a.bf16);
+            } else {
+              partial[to + col] += sum;
+            }
           });
         }
         __syncwarp();

@@ -150,13 +150,13 @@ __device__ __forceinline__ float to_reference(float m, float m_new, float& l) {
   return half * half;
 }
 
-// A product adds 0 * V for keys that a row's mask leaves out, and a NaN there would stay one.  So where rows of a tile see different
-// keys, NaNs of V are taken out of the tile before the product, and the rows that do see them get theirs afterwards, in what was
-// stored for them (write_nans).
+// A product adds 0 * V for keys that a row's mask leaves out, and a NaN or an infinity there would become a NaN.  So where rows of a tile
+// see different keys, they are taken out of V's tile before the product, and the rows that do see them get theirs afterwards, in what was
+// stored for them (write_specials).  e4m3 has NaN 0x7f and no infinities, e5m2 NaN from 0x7d on and infinity 0x7c.
 template <bool kE5M2>
-__device__ __forceinline__ bool drop_nans(uint4& x) {
-  // sign bits of the bytes that hold a NaN
-  auto of = [](uint32_t w) { return ((w & 0x7f7f7f7fu) + (kE5M2 ? 0x03030303u : 0x01010101u)) & 0x80808080u; };
+__device__ __forceinline__ bool drop_specials(uint4& x) {
+  // sign bits of the bytes that hold one
+  auto of = [](uint32_t w) { return ((w & 0x7f7f7f7fu) + (kE5M2 ? 0x04040404u : 0x01010101u)) & 0x80808080u; };
   const uint32_t n[4] = {of(x.x), of(x.y), of(x.z), of(x.w)};
   if ((n[0] | n[1] | n[2] | n[3]) == 0u) return false;
   x.x &= ~((n[0] >> 7) * 0xffu);
@@ -165,23 +165,32 @@ __device__ __forceinline__ bool drop_nans(uint4& x) {
   x.w &= ~((n[3] >> 7) * 0xffu);
   return true;
 }
-// Calls put(column) for the columns col, col + 32 ... below `end` in which a key from lo to hi - 1 of a sequence holds a NaN.  Goes through the
-// pool byte by byte, but only after a NaN has been met.
+// Calls put(column, value) for the columns col, col + 32 ... below `end` in which a key from lo to hi - 1 of a sequence holds a NaN or an
+// infinity: what they add up to.  Goes through the pool byte by byte, but only after one has been met.
 template <bool kE5M2, typename Put>
-__device__ __forceinline__ void write_nans(const KvArgs& a, int seq, int head, int lo, int hi, int col, int end, Put put) {
+__device__ __forceinline__ void write_specials(const KvArgs& a, int seq, int head, int lo, int hi, int col, int end, Put put) {
 #pragma unroll 1
   for (; col < end; col += 32) {
+    float sum = 0.f;
 #pragma unroll 1
     for (int key = lo; key < hi; ++key) {
       const int page = ld_int(a.table + static_cast<int64_t>(seq) * a.table_stride + (key >> a.page_shift));
       if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.num_pages)) continue;
       const int64_t row = ((static_cast<int64_t>(page) * a.heads + head) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
-      if ((a.v[row * a.head_dim + col] & 0x7f) >= (kE5M2 ? 0x7d : 0x7f)) {
-        put(col);
-        break;
-      }
+      const int x = a.v[row * a.head_dim + col];
+      if ((x & 0x7f) < (kE5M2 ? 0x7c : 0x7f)) continue;
+      sum += kE5M2 && (x & 0x7f) == 0x7c ? (x & 0x80 ? -INFINITY : INFINITY) : NAN;
+      if (sum != sum) break;
     }
+    if (sum != 0.f) put(col, sum);
   }
+}
+// What was stored for a row and column, plus such a sum.  (Of the halves, infinities of either sign together are a NaN, all of whose bits are set.)
+__device__ __forceinline__ uint16_t with_special(uint16_t old, float sum, bool bf16) {
+  const int inf = bf16 ? 0x7f80 : 0x7c00, had = old & 0x7fff;
+  const uint16_t sign = sum < 0.f ? 0x8000 : 0;
+  if (sum != sum || had > inf || (had == inf && (old & 0x8000) != sign)) return 0x7fff;
+  return static_cast<uint16_t>(sign | inf);
 }
 
 }  // namespace fa8

@@ -203,7 +203,8 @@ def flash_attention_paged_kv(q: torch.Tensor, cache, page_table: torch.Tensor, s
     q: float16 or bfloat16 [tokens, heads, head_dim], a view with strides allowed; heads a multiple of the cache's (query
     head h reads K/V head h // (heads // heads_kv)).  With is_causal new token i of sequence b sees the keys up to its
     own position, seqlens[b] - n_b + i; without it every key of its sequence.  A row that sees no key is zeros (its
-    log-sum-exp -inf); a NaN reaches the rows that see its key and no others.  Scores, softmax and sums are fp32; K and V enter exactly as the cache holds them.
+    log-sum-exp -inf); a NaN reaches the rows that see its key and no others (an infinity, which an e5m2 cache may hold, too, as an
+    infinity or a NaN).  Scores, softmax and sums are fp32; K and V enter exactly as the cache holds them.
     Returns [O], O in q's type [tokens, heads, head_dim] (`out` if given: contiguous), and with return_lse the fp32
     [tokens, heads] log-sum-exp of the scaled scores.  Rows outside cu_seqlens are left as they were.  Stream-ordered;
     nothing synchronises."""

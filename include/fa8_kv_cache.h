@@ -101,7 +101,8 @@ typedef struct fa8_kv_attention_params {
 } fa8_kv_attention_params;
 
 /* Attention of the new tokens' queries over their sequences' pages.  What a row does not see does not
- * count, whatever is held there: a NaN reaches the rows that see its key, in the columns that hold it. */
+ * count, whatever is held there.  A NaN of V reaches the rows that see its key, in the columns that hold it; an infinity (e5m2; not
+ * from fa8_kv_append) too, as an infinity or, where a row's probability of the key is too small for the products, as a NaN. */
 int fa8_kv_attention(const fa8_kv_attention_params* params, void* cuda_stream);
 
 /* Bytes of workspace for a call of these sizes on a device of `sm_count` SMs; host arithmetic only.

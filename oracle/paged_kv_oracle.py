@@ -100,9 +100,10 @@ def attention(q, cache, page_table, seqlens, causal, scale, cu_seqlens=None):
         p = p / torch.where(l == 0, 1.0, l)
         # what a row does not see does not count, whatever is held there
         seen = (s > -math.inf) | torch.isnan(s)
-        nan = torch.einsum("hij,jhd->ihd", seen.double(), torch.isnan(vq).double()) > 0
-        vq = torch.where(torch.isnan(vq), 0.0, vq)
-        o[first:first + n] = torch.where(nan, math.nan, torch.einsum("hij,jhd->ihd", p, vq))
+        nan, up, down = (torch.einsum("hij,jhd->ihd", seen.double(), of.double()) > 0 for of in (torch.isnan(vq), vq == math.inf, vq == -math.inf))
+        vq = torch.where(torch.isfinite(vq), vq, 0.0)
+        special = torch.where(up, math.inf, 0.0) + torch.where(down, -math.inf, 0.0) + torch.where(nan, math.nan, 0.0)
+        o[first:first + n] = torch.einsum("hij,jhd->ihd", p, vq) + special
         a[first:first + n] = torch.einsum("hij,jhd->ihd", p, vq.abs())
         lse[first:first + n] = (m + torch.log(l)).squeeze(-1).t()
     return o, lse, a

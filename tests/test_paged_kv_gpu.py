@@ -531,6 +531,39 @@ def test_append_to_pages_whose_scale_is_no_power_of_two(n, half, fp8, D):
         assert torch.equal(w.float().nan_to_num(-1.0), got.cpu().float().nan_to_num(-1.0))
 
 
+@pytest.mark.parametrize("seqs", [[(3, 40), (4, 300)], [(40, 200), (5, 5)], [(150, 500), (300, 300), (129, 140)], [(260, 3000)]], ids=["drafts", "pieces", "prompts", "parts"])
+@pytest.mark.parametrize("H,Hk,D,P", [(2, 2, 64, 16), (8, 2, 128, 32), (3, 1, 256, 64), (2, 1, 32, 128)])
+@pytest.mark.parametrize("half", [torch.float16, torch.bfloat16])
+def test_infinities_in_keys_that_only_some_rows_see(seqs, H, Hk, D, P, half):
+    """e5m2 has infinities.  Of V they reach the rows that see them, as an infinity or a NaN, in the columns that hold them, and
+    leave the others alone; of K those whose scores they make infinite, as the definition has it."""
+    cu, T, lens = ranges(seqs)
+    cache, table = filled(Hk, D, P, E5M2, seqs, seed=92)
+    for b, (n, s) in enumerate(seqs):
+        for i, col, value in ((n - 1, 3, math.inf), (n // 2, D - 1, -math.inf), (n // 2, 17, math.inf), (n - 1, 17, -math.inf),
+                              (max(0, n - 130), 0, math.inf), (n - 1, 0, math.nan)):
+            key = s - n + i
+            cache[1][int(table[b, key // P]), 0, key % P, col] = value
+        if Hk > 1:                                                # in another head than V's
+            key = s - n + n // 3
+            cache[0][int(table[b, key // P]), Hk - 1, key % P, 7] = math.inf
+    q = rows(T, H, D, half, 93, False, cu, seqs)
+    where = to(DEV, table, lens, cu)
+    out, lse = flash_attention_paged_kv(q, to(DEV, *cache), where[0], where[1], True, 0.1, cu_seqlens=where[2], return_lse=True)
+    check_status(DEV)
+    want, want_lse, A = po.attention(q.cpu(), cache, table, lens, True, 0.1, cu)
+    got = out.double().cpu()
+    held = torch.isfinite(want)
+    assert bool(held.any()) and bool(torch.isinf(want).any())
+    assert torch.equal(torch.isfinite(got), held)
+    signed = torch.isinf(want) & torch.isinf(got)
+    assert torch.equal(got[signed], want[signed])                 # never of the other sign
+    assert bool(torch.isnan(got[torch.isnan(want)]).all())
+    assert torch.equal(torch.isnan(lse.cpu()), torch.isnan(want_lse))
+    limit = torch.finfo(half).eps / 2 * want.abs() + 1.25 * 2.0 ** -11 * A + 2.0 ** -25
+    assert bool(((got - want).abs() <= limit)[held].all())
+
+
 def test_page_table_of_wider_rows():
     """A view of a table that has more columns: as many as the longest sequence of this call needs."""
     seqs, H, Hk, D, P = [(1, 50), (1, 90), (1, 33)], 4, 2, 64, 16
