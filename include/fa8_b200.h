@@ -35,6 +35,8 @@ extern "C" {
 #define FA8_ERR_UNSUPPORTED (-2)    /* shape or layout outside what the kernel implements */
 #define FA8_ERR_CUDA (-3)           /* a CUDA runtime/driver call failed; see fa8_last_error_detail */
 #define FA8_ERR_DEVICE_TIMEOUT (-4) /* a bounded wait inside the kernel expired (status word != 0) */
+#define FA8_ERR_BAD_INDEX (-5)      /* a kernel of fa8_kv_cache.h, which shares the status words, found a page number, length
+                                       or token range out of range; from fa8_fwd and fa8_check_status too */
 
 /* Layout of V.  The reference requires the caller to pass V transposed,
  * [batch, heads, head_dim, seqlen] (test.py:71, csrc/flash_attention.cu:376-379). */
@@ -108,7 +110,8 @@ typedef struct fa8_fwd_params {
  * Failure reporting without a synchronisation: a kernel whose bounded wait ran out also stores
  * its code in a word of pinned host memory the library owns.  Every call looks at that word
  * first; if an earlier launch on this device left a code there, the call returns
- * FA8_ERR_DEVICE_TIMEOUT (fa8_last_error_detail names the code), enqueues nothing but the
+ * FA8_ERR_DEVICE_TIMEOUT, or FA8_ERR_BAD_INDEX if it was a call of fa8_kv_cache.h that found an
+ * index out of range (fa8_last_error_detail names the code), enqueues nothing but the
  * clearing of the status words, and the call after it starts clean.  So a caller that never
  * calls fa8_check_status still hears of a failed launch, at the latest from the first call made
  * after that launch ended (the reference exits the process, include/attention_api.cuh:20-29).
@@ -116,7 +119,7 @@ typedef struct fa8_fwd_params {
 int fa8_fwd(const fa8_fwd_params* params, void* cuda_stream);
 
 /* Reads a status word back after synchronising `cuda_stream`: FA8_OK,
- * FA8_ERR_DEVICE_TIMEOUT (code copied to *code_out if not NULL) or FA8_ERR_CUDA.
+ * FA8_ERR_DEVICE_TIMEOUT or FA8_ERR_BAD_INDEX (code copied to *code_out if not NULL) or FA8_ERR_CUDA.
  * status_word NULL = the library's own word of the current device, which is cleared once
  * its code has been reported; a caller's word is left for the caller to clear.
  * Replaces the reference's cudaDeviceSynchronize + CUDA_ERROR_CHECK
@@ -209,7 +212,7 @@ const char* fa8_last_error_detail(void);
  * fa8_quantize_e4m3_segments, 107 the library-owned status word and host-side failure flag,
  * sequence lengths free of the multiple-of-16 rule except for transposed V, 108
  * fa8_quantize_e4m3_segments_noalloc, 109 fa8_work_plan; new fields go at the end of
- * fa8_fwd_params). */
+ * fa8_fwd_params).  FA8_ERR_BAD_INDEX came with fa8_kv_version() 100. */
 int fa8_version(void);
 
 #ifdef __cplusplus

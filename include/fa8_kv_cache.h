@@ -25,7 +25,8 @@
  * can hold or below n_b (append, read), token ranges that decrease or leave the tensor - reach the
  * device only, so the kernels check them: such a page or sequence is left out (read: zeros;
  * attention: its keys do not count), nothing outside the tensors is touched, and FA8_ERR_BAD_INDEX
- * is reported the way expired waits are, by fa8_check_status and by the next call on the device.
+ * is reported the way expired waits are, by fa8_check_status and by the next call on the device, be it
+ * of this header or fa8_fwd.  Calls that were enqueued before are computed.
  *
  * Limits (FA8_ERR_UNSUPPORTED past them): table_width * page_size, tokens and tokens * heads up to
  * 2^31 - 256, num_pages * heads_kv up to 2^31 - 1, 65536 heads_kv.
@@ -40,8 +41,6 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
-
-#define FA8_ERR_BAD_INDEX (-5) /* a kernel found a page number, length or token range out of range */
 
 typedef struct fa8_kv_cache {
   void* k;                   /* 16-byte aligned, as v */

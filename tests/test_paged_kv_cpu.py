@@ -147,3 +147,26 @@ def test_oracle_attention_is_softmax():
             torch.testing.assert_close(lse[i, h], torch.logsumexp(s, 0))
     assert bool((o[3] == 0).all()) and bool((lse[3] == -float("inf")).all())              # one key, two new tokens: the first sees none
     torch.testing.assert_close(o[4, 0], po.keys_values(cache, table, 1, 1)[1][0, 0])
+
+
+def test_every_status_is_declared_for_callers_of_the_forward_alone(tmp_path):
+    """fa8_fwd and fa8_check_status return what a call of the paged cache left in the status words they share, so its code is in their
+    header, with the value that the package uses; the other header adds to it."""
+    import shutil
+    import subprocess
+    names = {n: v for n, v in vars(_lib).items() if n == "FA8_OK" or n.startswith("FA8_ERR_")}
+    assert names["FA8_ERR_BAD_INDEX"] == -5
+    text = open(os.path.join(REPO_DIR, "include", "fa8_b200.h")).read()
+    for name, value in names.items():
+        assert re.search(rf"#define {name} \(?{value}\)?\s", text), name
+    about = re.findall(r"/\*(.*?)\*/\s*(?:int|const char\*|int64_t) (fa8_\w+)\(", text, flags=re.S)
+    for function in ("fa8_fwd", "fa8_check_status"):
+        assert any("FA8_ERR_BAD_INDEX" in words for words, name in about if name == function), function
+    cc = shutil.which("gcc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    for headers in (["fa8_b200.h"], ["fa8_kv_cache.h"], ["fa8_kv_cache.h", "fa8_b200.h"]):
+        source = "".join(f'#include "{h}"\n' for h in headers) + "int code = FA8_ERR_BAD_INDEX;\n"
+        (tmp_path / "c.c").write_text(source)
+        subprocess.run([cc, "-Wall", "-Werror", "-std=c99", "-I" + os.path.join(REPO_DIR, "include"), "-c", str(tmp_path / "c.c"),
+                        "-o", str(tmp_path / "c.o")], check=True)
