@@ -1,11 +1,11 @@
 // Attention of a few new tokens' queries over the pages of the fp8 cache (decoding), sm_100a.
 //
-//   x_j = c (q . k8_j) dk_j,   m >= x_j + log2 dv_j - 14,   O = sum_j 2^(x_j - m) dv_j v8_j / sum_j 2^(x_j - m)
+//   x_j = c (q . k8_j) dk_j,   m >= x_j + [log2 dv_j] - 14,   O = sum_j 2^(x_j - m) dv_j v8_j / sum_j 2^(x_j - m)
 //
-// with c = softmax_scale log2(e) and dk_j, dv_j the scales of key j's page.  The reference m of a row is taken over x + log2 dv,
-// so that what is rounded to fp16, P_j = 2^(x_j - m) dv_j, is at most 2^14 whatever the pages' scales; the sum of the
+// with c = softmax_scale log2(e), dk_j and dv_j the scales of key j's page, [] the whole part.  The reference m of a row is taken over x + [log2 dv],
+// so that what is rounded to fp16, P_j = 2^(x_j - m) dv_j, is below 2^15 whatever the pages' scales; the sum of the
 // denominators is of unrounded fp32 numbers.  m starts 6 below the first keys' maximum, so that P has its full precision twenty
-// binades down, and is raised to 6 below the maximum so far, and what was summed rescaled, only when some P would pass 2^14.  Keys and
+// binades down, and is raised to 6 below the maximum so far, and what was summed rescaled, only when some P might pass 2^15.  Keys and
 // queries enter the products exactly: every fp8 value is an fp16 value, and bf16 queries are brought into fp16's range by a power
 // of two per row (what that cuts off is below 2^-39 of the row's largest).
 //
@@ -45,7 +45,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr float kHeadroom = 6.f, kRaiseBy = 14.f;       // log2 of the largest P under a fresh reference, and at all
+constexpr float kHeadroom = 6.f, kRaiseBy = 14.f;       // log2 of the largest P, as by the whole part of log2 dv, under a fresh reference, and at all
 // log2 of the smallest scale of V that the reference m follows: exponentials reach 2^(kRaiseBy + 80), of which fp32 adds up 2^31
 constexpr float kLog2Least = -80.f;
 constexpr unsigned long long kLimitNs = 2000000000ull; // bound of every wait
@@ -130,8 +130,10 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
   constexpr int kWarps = C::kWarps, kStepKeys = C::kStepKeys, kHalves = C::kHalves;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_bar[kWarps * C::kStages];
-  // scales of K of the step's halves (-1: no page), those of V, log2 of those
-  __shared__ __align__(16) float s_scale[kWarps * C::kStages][8];
+  // Scales of K of the step's halves (-1: no page), then those of V.  (What is static, 1 KB of the system's and the rings are to fit 196 KB: past
+  // that the L1 cache gives up 32 KB more.  With sixteen bytes more a stage, for log2 of V's, 8 sequences of 4000 keys and 32 rows at
+  // head dim 128 took 46 us for 43.)
+  __shared__ __align__(16) float s_scale[kWarps * C::kStages][4];
   // the first unit of the item that a warp's last, and (where it had several) its first segment is of; -1: whole items only
   __shared__ int s_last[kWarps], s_head[kWarps];
   __shared__ bool s_single[kWarps], s_special[kWarps];       // (s_special: NaNs or infinities were taken out of the segment's V)
@@ -367,12 +369,12 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       }
       __syncwarp();
     };
-    // Lane l looks after the step's half l & 1: the scale of K (l < 2), -1 where there is no page, that of V (l < 4), or its log2.
+    // Lane l looks after the step's half l & 1: the scale of K (l & 2 = 0), -1 where there is no page, or that of V.
     auto put_scales = [&](int step, int st) {
       const int key = step * kStepKeys + (lane & (kHalves - 1)) * 16;
       const int src = ((key >> a.c.page_shift) - page0) & 31;
       const float kd = __shfl_sync(0xffffffffu, kd_of, src), vd = __shfl_sync(0xffffffffu, vd_of, src);
-      if (lane < 6) s_scale[warp * C::kStages + st][lane] = lane < 2 ? (key < vis ? kd : -1.f) : (lane < 4 ? vd : fmaxf(__log2f(vd), kLog2Least));
+      if (lane < 4) s_scale[warp * C::kStages + st][lane] = (lane & 2) ? vd : (key < vis ? kd : -1.f);
     };
     // (Code that runs once a launch is kept short: its instructions have to be fetched past the pages that are being read.)
     {
@@ -472,8 +474,10 @@ __global__ void __launch_bounds__(32 * ACfg<W, RB>::kWarps, 1) kv_attend_kernel(
       }
       const uint32_t sk = ring + stage * C::kStageBytes, sv = sk + C::kBlocks * C::kTile;
       const float4 scale = *reinterpret_cast<const float4*>(s_scale[warp * C::kStages + stage]);
-      const float2 logs = *reinterpret_cast<const float2*>(s_scale[warp * C::kStages + stage] + 4);
-      const float kd[2] = {scale.x, scale.y}, dv[2] = {scale.z, scale.w}, lv[2] = {logs.x, logs.y};
+      const float kd[2] = {scale.x, scale.y}, dv[2] = {scale.z, scale.w};
+      // For the reference the whole part of log2 dv will do, which lets P be 2^15: of the exponent e, 2^23 + e + 127 as a float less 2^23 + 127.
+      auto log2_of = [](float d) { return fmaxf(__uint_as_float(0x4b000000u | (__float_as_uint(d) >> 23)) - 8388735.f, kLog2Least); };
+      const float lv[2] = {log2_of(dv[0]), log2_of(dv[1])};
       // a step that holds keys past some row's last, or of a page that is out of range
       const int key0 = step * kStepKeys;
       const bool whole = key0 + kStepKeys <= least && kd[0] != -1.f && (kHalves == 1 || kd[1] != -1.f);
