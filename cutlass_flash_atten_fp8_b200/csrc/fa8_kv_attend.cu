@@ -22,10 +22,10 @@
 //     are dealt out depends on all lengths of the call, hence so do the last bits.
 //   * Few short items go to a cluster of one to eight CTAs each (lone_split), which adds up over distributed shared memory: one launch.
 //
-// Measured at head dim 128, 32 heads over 8 (GPU time): 16 sequences of 8192 keys 52 us, 5.1 TB/s, of which 36 us are the steps, at
+// Measured at head dim 128, 32 heads over 8 (GPU time): 16 sequences of 8192 keys 52.6 us, 5.1 TB/s, of which 36 us are the steps, at
 // 7.5 TB/s, and the rest what goes before and after them: lengths 1.3 us, page numbers 1.2, the first pages 1, adding up 1.5, the combining
-// kernel 2.  One of 131072 keys 53 us; one of 600 keys 7 us.  At head dim 64, 64 sequences of 20 to 8000 keys, 36 us: instructions (a key's
-// 64 bytes cost as many as to convert and multiply whatever the rows).
+// kernel 2.  One of 131072 keys 54 us; one of 600 keys 7 us.  At head dim 64, 64 sequences of 20 to 8000 keys, 36 us: 58 % of the issue slots, the rest
+// mostly instructions that wait for the one before (a key's 64 bytes cost as many to convert and multiply whatever the rows).
 //
 // Operand layouts are those of fa8_decode_sm100.cu: S = Q K^T with the query rows as M (16, eight of them padding
 // when there are eight) and eight keys as N, the k index permuted alike in both operands; O^T = V^T P^T with 16 output

@@ -7,9 +7,9 @@
 //   a = max |x| of the new rows,  2^e = the smallest power of two with a <= MAX 2^e,
 //   d = 2^e in a page that starts anew, max(d, 2^e) otherwise;  older x8 <- fp8(x8 d_old / d),  x8 = fp8(x / d)
 //
-// Bound by memory: two bytes in and one out per element (append; the reverse for read).  Measured: 16 prompts, 257 MB, 47 us, 5.4 TB/s,
+// Bound by memory: two bytes in and one out per element (append; the reverse for read).  Measured: 16 prompts, 257 MB, 49 us, 5.3 TB/s,
 // against 39 at the rate of a copy; read of 8 x 8192 tokens at head dim 64, 201 MB, 36 us against 31; a token of each of 128 sequences
-// 3.3 us and of one 2.4, a launch's latency and a chain of loads (where the token is, its page, its old scale).
+// 3.4 us and of one 2.4, a launch's latency and a chain of loads (where the token is, its page, its old scale).
 #include <cuda_runtime.h>
 
 #include "fa8_kernel.h"

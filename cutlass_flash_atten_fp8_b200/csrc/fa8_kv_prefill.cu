@@ -9,7 +9,7 @@
 //   producer   looks up items and pages, copies K and V tiles of kN keys from the pages (fp8) into shared memory
 //   widening   four warps turn a tile into fp16, in the layout that the products want, times the power of two by which its pages' scales
 //              differ from the item's first page; keys past the last one become zeros (a NaN or an infinity there must not meet a zero P).  Eight warps
-//              were no faster (330 us for 1024 tokens over 16384 keys, four 322)
+//              were no faster (330 us for 1024 tokens over 16384 keys where four took 322)
 //   issuer     one thread: S = Q K^T into tensor memory, O += P V with P from tensor memory
 //   softmax    eight warps a tile, two to 32 rows (four, a row to a thread, took 26 % longer): each has half of a block's keys, P = 2^(c s - m) over
 //              S as it lies, and at the end half of O's columns
@@ -20,8 +20,8 @@
 // binades down, and is raised, and O rescaled, when the sum of P over half a block nears fp16's largest number.  Scales that differ by
 // more than fp16 can take in, or are no powers of two, go through a slower form of the softmax that multiplies them in (`residual`).
 //
-// Measured: 1024 tokens, 32 heads over 8, over 16384 keys, head dim 128: 322 us, 826 TFLOP/s, half of what a plain fp16 product
-// reaches on this GPU; four prompts of 4096: 466 us.  A block of 128 keys takes some 4000 cycles for two tiles where the tensor cores are busy for
+// Measured: 1024 tokens, 32 heads over 8, over 16384 keys, head dim 128: 323 us, 824 TFLOP/s, half of what a plain fp16 product
+// reaches on this GPU; four prompts of 4096: 451 us.  A block of 128 keys takes some 4000 cycles for two tiles where the tensor cores are busy for
 // 2048: a tile's chain S, softmax (1024 cycles of exponentials alone, 2350 beside the other tile's), P V is longer than the other tile's
 // work.  A quarter of the exponentials by a polynomial instead gained 2 % and was left out.
 #include <cuda_runtime.h>
@@ -51,9 +51,9 @@ template <int W>
 struct PCfg {
   static constexpr int kTiles = W == 256 ? 1 : 2;
   static constexpr int kN = W == 256 ? 64 : 128;               // keys of a block
-  // Score buffers, which the blocks of both tiles take in turn: what tensor memory holds beside O.  The scores of a block go out kBufs
-  // blocks ahead, so a tile whose turn it is finds its next scores ready when there are more buffers than tiles: 8 prompts of 2048 at
-  // head dim 64 took 340 us with two, 311 with three.  (Four of 64 keys would do that at head dim 128, but a product of N = 64 is
+  // Score buffers, which the blocks of both tiles take in turn: what tensor memory holds beside O.  The scores go out as many turns ahead, one more
+  // than the item's tiles at most (kv_turns.h), so a tile whose turn it is finds its next scores ready when there are more buffers than tiles: 8 prompts of 2048 at
+  // head dim 64 took 340 us with two, 311 with three (305 since).  (Four of 64 keys would do that at head dim 128, but a product of N = 64 is
   // bound by reading Q from shared memory: 80 cycles a step of 16 against 64 for N = 128.)
   static constexpr int kBufs = W == 64 ? 3 : 2;
   static constexpr int kGroups = kN / 16;                      // of keys that share a page
@@ -1087,12 +1087,15 @@ cudaError_t launch_one(const CUtensorMap& tk, const CUtensorMap& tv, const KvAtt
 // the smaller blocks at 256.  This kernel reads them once for 256 (128) rows, but starts later.  Measured, few rows / this one, us
 // (H = 4 Hk; 8 K/V heads at head dim 128, otherwise 4):
 //   rows of a sequence      32             64             128            32, D 64   64      128      32, D 256  64      128
-//   1 x 16000 keys          31 / 39        42 / 41        65 / 45        17 / 33  18 / 34  24 / 35   30 / 51  43 / 52  69 / 56
-//   8 x  4000               42 / 45        67 / 47       117 / 53        17 / 27  23 / 28  37 / 28   42 / 45  70 / 47 129 / 50
-//  32 x  1000               48 / 48        79 / 49       140 / 55        19 / 21  28 / 22  43 / 24   47 / 40  80 / 40 150 / 42
-//   1 x  1000               13 / 21        14 / 22        15 / 24        10 / 17  10 / 17  10 / 19   13 / 27  14 / 28  15 / 33
-// and 16 sequences of 17 to 300 new tokens and up to 512 keys, a row a token, 47 / 27.  They meet near 300000 blocks times keys.  The host
-// knows how many keys the page table can hold, and takes that.
+//   1 x 16000 keys          32 / 30        42 / 33        65 / 35        17 / 25  19 / 25  25 / 26   30 / 42  43 / 43  70 / 47
+//   8 x  4000               43 / 44        68 / 46       119 / 51        17 / 24  24 / 26  37 / 26   43 / 42  71 / 45 129 / 48
+//  32 x  1000               49 / 49        80 / 51       141 / 55        19 / 21  29 / 22  44 / 24   47 / 39  80 / 40 150 / 42
+//   1 x  1000               13 / 20        15 / 21        15 / 24        10 / 16  10 / 17  10 / 18   13 / 20  14 / 22  15 / 26
+// and 16 sequences of 17 to 300 new tokens and up to 512 keys, a row a token, 48 / 27.  They meet near 300000 blocks times keys (sooner where one
+// long sequence is all there is).  The host knows how many keys the page table can hold, and takes that.
+//
+// The rule goes by the mean sequence, since the host does not know the lengths, so that a call of many single tokens and one long piece runs in the kernel
+// for few rows as a whole: 255 tokens over 4096 keys with 1024 tokens over 16384, head dim 128, take 2480 us, in two calls 360 + 270.
 constexpr int64_t kFewRowsMost = 128, kFewRowsKeys = 300000, kBlockKeys = 400;
 bool kv_prefill_takes(const KvAttendSizes& z) {
   const int64_t group = z.heads_q / z.heads, rows = (z.tokens * group + z.batch - 1) / z.batch, block = width_of(z.head_dim) == 256 ? 16 : 32;

@@ -9,7 +9,8 @@ begin in the token-major tensors ([tokens, heads, head_dim]; None: the tokens di
     paged_kv_append(cache, k, v, page_table, seqlens)
     o = flash_attention_paged_kv(q, cache, page_table, seqlens, True, scale)[0]
 
-and a batch of prompts, or of prompts and single tokens, the same with cu_seqlens.  The numbers in the three int32
+and a batch of prompts, or of prompts and single tokens, the same with cu_seqlens (which kernel attends goes by the mean
+number of new tokens: many single tokens beside a long prompt are faster as a call of their own).  The numbers in the three int32
 tensors stay on the device (the calls can be captured into a CUDA graph and replayed with others in their place); one
 that is out of range is left out by the kernels and raises in check_status() or at the next call.
 """
